@@ -330,6 +330,82 @@ x17ai_DiagnosticBuffer *x17ai_b200_attn_decode_i8_noalloc(
 	uint32_t const *kv_lens, int8_t const *sink_k, int8_t const *sink_v,
 	float const *attn_temperature, int8_t *out, float *l, size_t window_size, size_t n_splits);
 
+/*
+ * The paged key-value cache: no counterpart in the reference. A serving host keeps the keys and values of its sequences in pages
+ * of a pool and names each sequence's pages, in order of position, in one row of a page table.
+ *   pages int8 [n_pages][n_kv_heads][page_size][K(D) | V(D)]: a page of one head is one run of memory
+ *   page_scales f32 [n_pages][n_kv_heads][page_size][2] (K, V): the scaled calls; value = scale * code. The others: FixedI8
+ *   page_table int32 [n_seqs][max_pages]; entries behind a sequence's last page are not read
+ * n_heads is a multiple of n_kv_heads: query head h attends key head h / (n_heads / n_kv_heads).
+ * What the calls read as indexes from device memory (sequences, positions, pages) is checked there: a token with an index out
+ * of range is not stored, a key on a page outside the pool is not attended to, and the status words (x17ai_b200_read_status)
+ * hold code 16 with the token or sequence as detail.
+ */
+typedef struct x17ai_PagedConfig {
+	size_t n_heads;
+	size_t n_kv_heads;
+	size_t head_dim;   /* 32, 64 or 128 */
+	size_t page_size;  /* tokens of a page: a power of two from 16 to 1024 */
+	size_t q_stride;   /* elements per row of q and q_out, a multiple of 16 */
+	size_t kv_stride;  /* of kv and kv_out */
+	size_t o_stride;   /* of out */
+	size_t rotary_dim; /* leading dims of a head that are rotated by position: a multiple of 32, 0 = none */
+	int32_t adjacent_pairs; /* 0: dims (i, i + rotary_dim / 2) form a pair; 1: dims (2 i, 2 i + 1) */
+	int32_t reserved;
+} x17ai_PagedConfig;
+
+x17ai_DiagnosticBuffer *x17ai_b200_paged_check_config(x17ai_PagedConfig const *cfg);
+
+/*
+ * Puts new tokens into the cache, their keys and queries rotated by position on the way.
+ *   q [tokens][q_stride] int8 (or NULL, then q_out too), head h at columns h*D; kv [tokens][kv_stride] int8, key head h at
+ *   columns 2*h*D: [K(D) | V(D)] (what the KV projection writes); seqs, positions int32 [tokens]: row of the page table and
+ *   position of each token; a negative sequence marks a row of padding, which is left alone everywhere.
+ *   rope int16 [rope_rows][rotary_dim / 2][2]: cos, sin of each position's angles in units of 2^-14; NULL with rotary_dim 0.
+ *   (x, y) -> clamp((x cos - y sin + 2^13) >> 14, +-127), clamp((x sin + y cos + 2^13) >> 14, +-127) in integers; dims that are
+ *   not rotated, and V, are copied.
+ *   q_out [tokens][q_stride]; kv_out [tokens][kv_stride] or NULL: the rows as stored, for the prefill attention of the same
+ *   tokens. Outputs must not overlap inputs. Two tokens of a call must not share a place.
+ */
+x17ai_DiagnosticBuffer *x17ai_b200_paged_append(
+	x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, int8_t const *q, int8_t const *kv, size_t tokens,
+	int32_t const *seqs, int32_t const *positions, int32_t const *page_table, size_t n_seqs, size_t max_pages,
+	int16_t const *rope, size_t rope_rows, int8_t *pages, size_t n_pages, int8_t *q_out, int8_t *kv_out);
+
+/*
+ * The same from bf16 rows, rotated in f32 and then quantised with one scale per token and head (q_scale [tokens][n_heads]; the
+ * keys' and values' go to page_scales): scale = absmax / 127, code = rint(x * (127 / absmax)); a head whose largest magnitude is
+ * at most 2^-100 gives zeros and scale 0. Finite inputs; a head with an infinity or NaN gets codes without meaning.
+ */
+x17ai_DiagnosticBuffer *x17ai_b200_paged_append_scaled(
+	x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, uint16_t const *q_bf16, uint16_t const *kv_bf16, size_t tokens,
+	int32_t const *seqs, int32_t const *positions, int32_t const *page_table, size_t n_seqs, size_t max_pages,
+	int16_t const *rope, size_t rope_rows, int8_t *pages, float *page_scales, size_t n_pages, int8_t *q_out, float *q_scale);
+
+/*
+ * Attention of n_tokens (1 to 64) new tokens of each of `batch` sequences over the cache: token i of sequence b has position
+ * n = kv_lens[b] + i and attends keys n - W' .. n - 1 and the sink, as row n of x17ai_b200_attn_fwd_i8 does (a token does not
+ * see itself; the keys of the new tokens in front of it are in the cache already). One token is a decode step, several are
+ * drafted tokens that are checked in one pass over the cache.
+ *   q, out: row b * n_tokens + i, strides q_stride and o_stride; page_table [batch][max_pages]; kv_lens int32 [batch] (clamped to
+ *   0 .. max_pages * page_size); out FixedI8 (X17AI_DTYPE_INT8) or bf16 (X17AI_DTYPE_BF16, value = code / 8);
+ *   l [batch * n_tokens][n_heads] or NULL: log2(255 * sum) + max, as the other int8 kernels write it.
+ * Scores are exact integer products, probabilities keep 22 bits, sums are f32. n_splits: CTAs that share a sequence's keys
+ * (1 to 16; 0 = chosen); their parts meet in the shared memory of a cluster, no scratch memory is used.
+ */
+x17ai_DiagnosticBuffer *x17ai_b200_paged_decode(
+	x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, int8_t const *q,
+	int8_t const *pages, size_t n_pages, int32_t const *page_table, size_t max_pages, int32_t const *kv_lens,
+	int8_t const *sink_k, int8_t const *sink_v, float const *attn_temperature, void *out, int32_t out_dtype, float *l,
+	size_t window_size, size_t n_splits);
+
+/* The same over a scaled cache, with q_scale [batch * n_tokens][n_heads] and bf16 output; sinks are FixedI8 as before. */
+x17ai_DiagnosticBuffer *x17ai_b200_paged_decode_scaled(
+	x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, int8_t const *q,
+	float const *q_scale, int8_t const *pages, float const *page_scales, size_t n_pages, int32_t const *page_table,
+	size_t max_pages, int32_t const *kv_lens, int8_t const *sink_k, int8_t const *sink_v, float const *attn_temperature,
+	uint16_t *out_bf16, float *l, size_t window_size, size_t n_splits);
+
 /* Epilogues of the GEMM (src/device/cuda/gemm.rs: ScaleEpilogue :60-110, RMSNormEpilogue
  * :112-166, ResidualEpilogue :168-212, GeGluEpilogue :214-255) */
 enum {

@@ -75,6 +75,11 @@ class QkvgConfig(Structure):
                 ("inp_scale", c_double), ("out_scale", c_double), ("eps", c_double)]
 
 
+class PagedConfig(Structure):
+    _fields_ = [(n, c_size_t) for n in ("n_heads", "n_kv_heads", "head_dim", "page_size", "q_stride", "kv_stride", "o_stride",
+                                        "rotary_dim")] + [("adjacent_pairs", c_int32), ("reserved", c_int32)]
+
+
 class GemmMeta(Structure):
     _fields_ = [("threads_per_block", c_size_t), ("smem_bytes", c_size_t), ("m_per_block", c_size_t),
                 ("n_per_block", c_size_t)]
@@ -118,6 +123,15 @@ SIGNATURES = {
                                          c_size_t] + [c_void_p] * 6 + [c_size_t, c_size_t]),
     "x17ai_b200_attn_decode_i8_noalloc": (DIAG, [c_void_p, POINTER(AttnConfig), c_size_t, c_void_p, c_void_p, c_size_t,
                                                  c_size_t] + [c_void_p] * 6 + [c_size_t, c_size_t]),
+    "x17ai_b200_paged_check_config": (DIAG, [POINTER(PagedConfig)]),
+    "x17ai_b200_paged_append": (DIAG, [c_void_p, POINTER(PagedConfig), c_void_p, c_void_p, c_size_t] + [c_void_p] * 3
+                                + [c_size_t] * 2 + [c_void_p, c_size_t, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "x17ai_b200_paged_append_scaled": (DIAG, [c_void_p, POINTER(PagedConfig), c_void_p, c_void_p, c_size_t] + [c_void_p] * 3
+                                       + [c_size_t] * 2 + [c_void_p, c_size_t, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "x17ai_b200_paged_decode": (DIAG, [c_void_p, POINTER(PagedConfig), c_size_t, c_size_t, c_void_p, c_void_p, c_size_t, c_void_p,
+                                       c_size_t] + [c_void_p] * 5 + [c_int32, c_void_p, c_size_t, c_size_t]),
+    "x17ai_b200_paged_decode_scaled": (DIAG, [c_void_p, POINTER(PagedConfig), c_size_t, c_size_t] + [c_void_p] * 4 + [c_size_t, c_void_p,
+                                              c_size_t] + [c_void_p] * 6 + [c_size_t, c_size_t]),
     "x17ai_b200_gemm_meta": (DIAG, [POINTER(GemmConfig), POINTER(GemmMeta)]),
     "x17ai_b200_gemm_fwd": (DIAG, [c_void_p, POINTER(GemmConfig), c_void_p, c_size_t, c_void_p, c_size_t,
                                    c_void_p, c_void_p, c_void_p]),

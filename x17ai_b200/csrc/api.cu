@@ -21,6 +21,7 @@
 #include "diag.hpp"
 #include "gemm.cuh"
 #include "gemm_rows.cuh"
+#include "paged.cuh"
 #include "rms_norm.cuh"
 
 using x17::make_diag;
@@ -821,6 +822,177 @@ x17ai_DiagnosticBuffer *decode_go(char const *who, cudaStream_t s, size_t head_d
 							: decode_go_dim<32>(who, s, batch, p);
 }
 
+// ---- paged cache ---------------------------------------------------------------------------------
+
+bool power_of_two(size_t n) { return n != 0 && (n & (n - 1)) == 0; }
+
+x17ai_DiagnosticBuffer *check_paged_config(x17ai_PagedConfig const *cfg, char const *who) {
+	char const *const bad = "x17ai_b200: bad paged cache config";
+	if (cfg == nullptr) return make_diag("x17ai_b200: null config", who, ": null config");
+	size_t const h = cfg->n_heads, hk = cfg->n_kv_heads, d = cfg->head_dim;
+	if (h == 0 || hk == 0 || h > 65535 || h % hk != 0) {
+		return make_diag(bad, who, ": paged cache config requires n_heads > 0 and a multiple of n_kv_heads, got ", h, " and ", hk);
+	}
+	if (d != 32 && d != 64 && d != 128) {
+		return make_diag(bad, who, ": paged cache config requires head_dim 32, 64 or 128, got ", d);
+	}
+	if (!power_of_two(cfg->page_size) || cfg->page_size < 16 || cfg->page_size > 1024) {
+		return make_diag(bad, who, ": paged cache config requires page_size 16, 32, ... 1024, got ", cfg->page_size);
+	}
+	if (cfg->q_stride < h * d || cfg->o_stride < h * d || cfg->kv_stride < 2 * hk * d) {
+		return make_diag(bad, who, ": paged cache config requires q_stride and o_stride >= n_heads * head_dim (", h * d,
+						 ") and kv_stride >= 2 * n_kv_heads * head_dim (", 2 * hk * d, "), got ", cfg->q_stride, ", ", cfg->o_stride,
+						 ", ", cfg->kv_stride);
+	}
+	if (cfg->q_stride % 16 != 0 || cfg->kv_stride % 16 != 0 || cfg->o_stride % 16 != 0) {
+		return make_diag(bad, who, ": paged cache strides must be multiples of 16 elements");
+	}
+	if (cfg->rotary_dim > d || cfg->rotary_dim % 32 != 0) {
+		return make_diag(bad, who, ": paged cache config requires rotary_dim a multiple of 32 up to head_dim, got ", cfg->rotary_dim);
+	}
+	return nullptr;
+}
+
+x17ai_DiagnosticBuffer *paged_pool(char const *who, x17ai_PagedConfig const *cfg, int8_t const *pages, float const *scales,
+								   bool scaled, size_t n_pages, int32_t const *table, size_t n_seqs, size_t max_pages,
+								   x17::PagedPool *pool) {
+	if (n_pages == 0 || n_seqs == 0 || max_pages == 0) {
+		return make_diag("x17ai_b200: empty paged cache", who, ": pages and page_table must not be empty");
+	}
+	if (n_pages >= (size_t(1) << 31) || n_seqs >= (size_t(1) << 31) || max_pages >= ((size_t(1) << 31) / cfg->page_size)) {
+		return make_diag("x17ai_b200: paged cache out of range", who, ": paged cache shape out of range (n_pages ", n_pages,
+						 ", max_pages ", max_pages, ")");
+	}
+	if (pages == nullptr || table == nullptr || (scaled && scales == nullptr)) {
+		return make_diag("x17ai_b200: null tensor", who, ": null tensor argument");
+	}
+	if (!aligned16(pages) || !aligned16(scales)) {
+		return make_diag("x17ai_b200: misaligned tensor", who, ": tensors must be 16-byte aligned");
+	}
+	pool->pages = const_cast<int8_t *>(pages);
+	pool->scales = scaled ? const_cast<float *>(scales) : nullptr;
+	pool->table = table;
+	pool->n_pages = uint32_t(n_pages);
+	pool->n_seqs = uint32_t(n_seqs);
+	pool->max_pages = uint32_t(max_pages);
+	pool->page_shift = 0;
+	while ((size_t(1) << pool->page_shift) < cfg->page_size) ++pool->page_shift;
+	pool->n_kv_heads = uint32_t(cfg->n_kv_heads);
+	return nullptr;
+}
+
+template <bool SCALED>
+x17ai_DiagnosticBuffer *paged_append(char const *who, x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, void const *q,
+									 void const *kv, size_t tokens, int32_t const *seqs, int32_t const *positions,
+									 int32_t const *table, size_t n_seqs, size_t max_pages, int16_t const *rope, size_t rope_rows,
+									 int8_t *pages, float *scales, size_t n_pages, int8_t *q_out, float *q_scale, int8_t *kv_out) {
+	if (auto *d = check_paged_config(cfg, who)) return d;
+	// (the grid has one warp per token and head, four to a CTA)
+	if (tokens == 0 || tokens >= (size_t(1) << 31) || tokens * (cfg->n_heads + 2 * cfg->n_kv_heads) >= (size_t(1) << 33)) {
+		return make_diag("x17ai_b200: bad token count", who, ": input kv has zero size or too many rows");
+	}
+	x17::PagedAppendParams p{};
+	if (auto *d = paged_pool(who, cfg, pages, scales, SCALED, n_pages, table, n_seqs, max_pages, &p.pool)) return d;
+	if (!kv || !seqs || !positions || (q != nullptr) != (q_out != nullptr) || (SCALED && (q != nullptr) != (q_scale != nullptr))) {
+		return make_diag("x17ai_b200: null tensor", who, ": null tensor argument (q and its outputs come together)");
+	}
+	if ((cfg->rotary_dim != 0) != (rope != nullptr) || (rope != nullptr && rope_rows == 0)) {
+		return make_diag("x17ai_b200: bad rope table", who, ": a rope table is given exactly where the config has a rotary_dim");
+	}
+	if (!aligned16(q) || !aligned16(kv) || !aligned16(rope) || !aligned16(q_out) || !aligned16(kv_out)) {
+		return make_diag("x17ai_b200: misaligned tensor", who, ": tensors must be 16-byte aligned");
+	}
+	StreamScope scope(stream, who);
+	if (scope.diag) return scope.diag;
+	p.q = q;
+	p.kv = kv;
+	p.seqs = seqs;
+	p.positions = positions;
+	p.rope = rope;
+	p.q_out = q_out;
+	p.kv_out = kv_out;
+	p.q_scale = q_scale;
+	p.q_stride = cfg->q_stride;
+	p.kv_stride = cfg->kv_stride;
+	p.tokens = uint32_t(tokens);
+	p.n_heads = uint32_t(cfg->n_heads);
+	p.rope_rows = uint32_t(rope_rows < (size_t(1) << 31) ? rope_rows : (size_t(1) << 31));
+	p.rotary = uint32_t(cfg->rotary_dim);
+	p.adjacent = cfg->adjacent_pairs != 0;
+	p.status = scope.state().status;
+	cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+	size_t const items = tokens * ((q != nullptr ? cfg->n_heads : 0) + 2 * cfg->n_kv_heads);
+	auto go = [&](auto dim) {
+		constexpr uint32_t D = decltype(dim)::value;
+		(void)launch(Kernel<&x17::paged_append_kernel<D, SCALED>>{}, dim3(unsigned((items + 3) / 4)), 128, 0, s, dim3(NO_CLUSTER), p);
+	};
+	if (cfg->head_dim == 128) go(std::integral_constant<uint32_t, 128>{});
+	else if (cfg->head_dim == 64) go(std::integral_constant<uint32_t, 64>{});
+	else go(std::integral_constant<uint32_t, 32>{});
+	return launch_result(who);
+}
+
+template <bool SCALED>
+x17ai_DiagnosticBuffer *paged_decode(char const *who, x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, size_t batch,
+									 size_t n_tokens, int8_t const *q, float const *q_scale, int8_t const *pages, float const *scales,
+									 size_t n_pages, int32_t const *table, size_t max_pages, int32_t const *kv_lens,
+									 int8_t const *sink_k, int8_t const *sink_v, float const *temperature, void *out, int32_t out_dtype,
+									 float *l, size_t window_size, size_t n_splits) {
+	if (auto *d = check_paged_config(cfg, who)) return d;
+	if (batch == 0 || n_tokens == 0) return make_diag("x17ai_b200: empty decode input", who, ": decode input q has zero size");
+	if (batch > 65535 || n_tokens > 64) {
+		return make_diag("x17ai_b200: decode shape out of range", who, ": at most 65535 sequences of 64 new tokens, got ", batch, " of ",
+						 n_tokens);
+	}
+	if (n_splits > 16) return make_diag("x17ai_b200: decode shape out of range", who, ": n_splits is at most 16, got ", n_splits);
+	if (window_size % 16 != 0) {
+		return make_diag("x17ai_b200: bad window", who, ": attention window_size must be zero or divisible by 16, got ", window_size);
+	}
+	if (out_dtype != X17AI_DTYPE_BF16 && (SCALED || out_dtype != X17AI_DTYPE_INT8)) {
+		return make_diag("x17ai_b200: bad output type", who, ": output is bf16", SCALED ? "" : " or FixedI8");
+	}
+	x17::PagedDecodeParams p{};
+	if (auto *d = paged_pool(who, cfg, pages, scales, SCALED, n_pages, table, batch, max_pages, &p.pool)) return d;
+	if (!q || !kv_lens || !sink_k || !sink_v || !temperature || !out || (SCALED && !q_scale)) {
+		return make_diag("x17ai_b200: null tensor", who, ": null tensor argument");
+	}
+	if (!aligned16(q) || !aligned16(sink_k) || !aligned16(sink_v) || !aligned16(out)) {
+		return make_diag("x17ai_b200: misaligned tensor", who, ": tensors must be 16-byte aligned");
+	}
+	StreamScope scope(stream, who);
+	if (scope.diag) return scope.diag;
+	p.q = q;
+	p.q_scale = q_scale;
+	p.kv_lens = kv_lens;
+	p.sink_k = sink_k;
+	p.sink_v = sink_v;
+	p.temperature = temperature;
+	p.out = out;
+	p.l = l;
+	p.q_stride = cfg->q_stride;
+	p.o_stride = cfg->o_stride;
+	p.n_heads = uint32_t(cfg->n_heads);
+	p.n_tokens = uint32_t(n_tokens);
+	p.window = window_size == 0 || window_size > 0xFFFFFFF0u ? 0xFFFFFFFFu : uint32_t(window_size);
+	p.status = scope.state().status;
+	cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+	auto go = [&](auto dim, auto out_i8) {
+		constexpr uint32_t D = decltype(dim)::value;
+		(void)launch(Kernel<&x17::paged_decode_kernel<D, SCALED, decltype(out_i8)::value>>{},
+					 dim3(unsigned(cfg->n_heads * n_tokens), unsigned(batch)), 128, 0, s, dim3(NO_CLUSTER), p);
+	};
+	auto go_dim = [&](auto dim) {
+		if constexpr (!SCALED) {
+			if (out_dtype == X17AI_DTYPE_INT8) return go(dim, std::true_type{});
+		}
+		go(dim, std::false_type{});
+	};
+	if (cfg->head_dim == 128) go_dim(std::integral_constant<uint32_t, 128>{});
+	else if (cfg->head_dim == 64) go_dim(std::integral_constant<uint32_t, 64>{});
+	else go_dim(std::integral_constant<uint32_t, 32>{});
+	return launch_result(who);
+}
+
 // ---- decode without allocation -------------------------------------------------------------------
 // Scratch for the split-KV partials of x17ai_b200_attn_decode_i8_noalloc. It lives in the
 // library image: every GPU that loads the library holds these 4 MiB until the process exits.
@@ -1291,6 +1463,45 @@ x17ai_DiagnosticBuffer *x17ai_b200_attn_decode_i8_noalloc(
 										l, window_size, n_splits);
 	if (!decode_in_cluster(n_splits)) p.scratch = scratch;  // every split writes its whole slot before the merge reads it
 	return decode_go(who, s, cfg->head_dim, batch, p);
+}
+
+x17ai_DiagnosticBuffer *x17ai_b200_paged_check_config(x17ai_PagedConfig const *cfg) {
+	return check_paged_config(cfg, "x17ai_b200_paged_check_config()");
+}
+
+x17ai_DiagnosticBuffer *x17ai_b200_paged_append(
+	x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, int8_t const *q, int8_t const *kv, size_t tokens,
+	int32_t const *seqs, int32_t const *positions, int32_t const *page_table, size_t n_seqs, size_t max_pages,
+	int16_t const *rope, size_t rope_rows, int8_t *pages, size_t n_pages, int8_t *q_out, int8_t *kv_out) {
+	return paged_append<false>("x17ai_b200_paged_append()", stream, cfg, q, kv, tokens, seqs, positions, page_table, n_seqs, max_pages,
+							   rope, rope_rows, pages, nullptr, n_pages, q_out, nullptr, kv_out);
+}
+
+x17ai_DiagnosticBuffer *x17ai_b200_paged_append_scaled(
+	x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, uint16_t const *q_bf16, uint16_t const *kv_bf16, size_t tokens,
+	int32_t const *seqs, int32_t const *positions, int32_t const *page_table, size_t n_seqs, size_t max_pages,
+	int16_t const *rope, size_t rope_rows, int8_t *pages, float *page_scales, size_t n_pages, int8_t *q_out, float *q_scale) {
+	return paged_append<true>("x17ai_b200_paged_append_scaled()", stream, cfg, q_bf16, kv_bf16, tokens, seqs, positions, page_table, n_seqs,
+							  max_pages, rope, rope_rows, pages, page_scales, n_pages, q_out, q_scale, nullptr);
+}
+
+x17ai_DiagnosticBuffer *x17ai_b200_paged_decode(
+	x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, int8_t const *q,
+	int8_t const *pages, size_t n_pages, int32_t const *page_table, size_t max_pages, int32_t const *kv_lens,
+	int8_t const *sink_k, int8_t const *sink_v, float const *attn_temperature, void *out, int32_t out_dtype, float *l,
+	size_t window_size, size_t n_splits) {
+	return paged_decode<false>("x17ai_b200_paged_decode()", stream, cfg, batch, n_tokens, q, nullptr, pages, nullptr, n_pages, page_table,
+							   max_pages, kv_lens, sink_k, sink_v, attn_temperature, out, out_dtype, l, window_size, n_splits);
+}
+
+x17ai_DiagnosticBuffer *x17ai_b200_paged_decode_scaled(
+	x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, int8_t const *q,
+	float const *q_scale, int8_t const *pages, float const *page_scales, size_t n_pages, int32_t const *page_table,
+	size_t max_pages, int32_t const *kv_lens, int8_t const *sink_k, int8_t const *sink_v, float const *attn_temperature,
+	uint16_t *out_bf16, float *l, size_t window_size, size_t n_splits) {
+	return paged_decode<true>("x17ai_b200_paged_decode_scaled()", stream, cfg, batch, n_tokens, q, q_scale, pages, page_scales, n_pages,
+							  page_table, max_pages, kv_lens, sink_k, sink_v, attn_temperature, out_bf16, X17AI_DTYPE_BF16, l, window_size,
+							  n_splits);
 }
 
 x17ai_DiagnosticBuffer *x17ai_b200_gemm_meta(x17ai_GemmConfig const *cfg, x17ai_GemmMeta *meta) {

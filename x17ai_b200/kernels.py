@@ -351,6 +351,179 @@ class AttnKernel(_Configured):
             n_splits))
 
 
+# ---- the paged key-value cache ---------------------------------------------------------------------
+
+ROPE_ONE = 1 << 14   # cos and sin of a rope table are int16 in units of 2^-14
+
+
+def rope_table(n_positions: int, rotary_dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
+    """The rotation of positions 0 .. n_positions - 1 for PagedAttnKernel.append: int16 [n_positions, rotary_dim / 2, 2], (cos, sin)
+    of position * base^(-2 i / rotary_dim) in units of 2^-14. Angles are taken in 64 bits. A table made elsewhere (another
+    spacing of the angles, or scaled positions) does as well."""
+    if n_positions <= 0 or rotary_dim <= 0 or rotary_dim % 32 != 0:
+        raise X17Error(f"rope table requires positions and a rotary_dim that is a multiple of 32, got {n_positions} and {rotary_dim}")
+    f = float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    a = torch.arange(n_positions, dtype=torch.float64).unsqueeze(1) * f
+    return torch.stack((a.cos(), a.sin()), dim=-1).mul_(ROPE_ONE).round_().to(torch.int16).to(device)
+
+
+@dataclass(frozen=True)
+class PagedConfig:
+    """Heads, pages and row strides (elements) of a paged cache. n_heads is a multiple of n_kv_heads; page_size a power of two
+    from 16 to 1024; rotary_dim the leading dims of a head that append rotates (a multiple of 32, 0 = none), in pairs
+    (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with adjacent_pairs."""
+    n_heads: int
+    n_kv_heads: int
+    head_dim: int
+    page_size: int
+    q_stride: int
+    kv_stride: int
+    o_stride: int
+    rotary_dim: int = 0
+    adjacent_pairs: bool = False
+
+    def _c(self):
+        return _lib.PagedConfig(self.n_heads, self.n_kv_heads, self.head_dim, self.page_size, self.q_stride, self.kv_stride,
+                                self.o_stride, self.rotary_dim, int(self.adjacent_pairs), 0)
+
+
+class PagedAttnKernel(_Configured):
+    """A key-value cache in pages: new tokens go in with append / append_scaled, decode / decode_scaled attend over it
+    (x17ai_b200_paged_append and the entry points beside it in the header).
+
+      pages        int8 [n_pages, n_kv_heads, page_size, 2 * head_dim], per token [K | V]
+      page_scales  f32 [n_pages, n_kv_heads, page_size, 2] (K, V), the scaled calls; the others hold FixedI8 codes
+      page_table   int32 [n_seqs, max_pages]: a sequence's pages in order of position; entries behind its last page are not read
+
+    Sequences, positions and pages are checked on the device: what is out of range is left out and recorded in the status words
+    (read_status: code 16). Nothing is allocated, so the calls can be captured into graphs, and two of them can run at once as
+    far as they do not write the same rows."""
+
+    def __init__(self, config: PagedConfig):
+        self.config = config
+        self._lib = _lib.load()
+        cfg = self._c_config[1]
+        check(self._lib.x17ai_b200_paged_check_config(ctypes.byref(cfg)))
+
+    def pages(self, n_pages: int, device="cuda") -> torch.Tensor:
+        """A pool of empty pages."""
+        c = self.config
+        return torch.zeros((n_pages, c.n_kv_heads, c.page_size, 2 * c.head_dim), dtype=torch.int8, device=device)
+
+    def page_scales(self, n_pages: int, device="cuda") -> torch.Tensor:
+        c = self.config
+        return torch.zeros((n_pages, c.n_kv_heads, c.page_size, 2), dtype=torch.float32, device=device)
+
+    def _pool(self, op, pages, page_scales, page_table, n_seqs=None):
+        """(pages, sequences, pages per sequence) after the checks that all calls share."""
+        c = self.config
+        want = (c.n_kv_heads, c.page_size, 2 * c.head_dim)
+        if pages.dim() != 4 or pages.shape[0] == 0 or tuple(pages.shape[1:]) != want:
+            raise X17Error(f"{op} input pages must have shape [n_pages, {', '.join(map(str, want))}], got {list(pages.shape)}")
+        _dtype_and_device(op, "pages", pages, DTYPE_INT8)
+        if page_scales is not None:
+            want = (pages.shape[0], c.n_kv_heads, c.page_size, 2)
+            if tuple(page_scales.shape) != want:
+                raise X17Error(f"{op} input page_scales must have shape {list(want)}, got {list(page_scales.shape)}")
+            _dtype_and_device(op, "page_scales", page_scales, DTYPE_F32)
+        seqs, max_pages = matrix_shape(op, "page_table", page_table, (n_seqs, None), DTYPE_I32_RAW)
+        return pages.shape[0], seqs, max_pages
+
+    def _append_shapes(self, op, q, kv, seqs, positions, page_table, pages, page_scales, q_out, q_scale, rope, kv_out, dtype):
+        c = self.config
+        tokens, _ = matrix_shape(op, "kv", kv, (None, c.kv_stride), dtype)
+        vector_shape(op, "seqs", seqs, tokens, DTYPE_I32_RAW)
+        vector_shape(op, "positions", positions, tokens, DTYPE_I32_RAW)
+        n_pages, n_seqs, max_pages = self._pool(op, pages, page_scales, page_table)
+        if (q is None) != (q_out is None):
+            raise X17Error(f"{op} takes q and q_out together")
+        if q is not None:
+            matrix_shape(op, "q", q, (tokens, c.q_stride), dtype)
+            matrix_shape(op, "q_out", q_out, (tokens, c.q_stride), DTYPE_INT8)
+        if kv_out is not None:
+            matrix_shape(op, "kv_out", kv_out, (tokens, c.kv_stride), DTYPE_INT8)
+        if (rope is None) != (c.rotary_dim == 0):
+            raise X17Error(f"{op} takes a rope table exactly where the config has a rotary_dim ({c.rotary_dim})")
+        if rope is not None:
+            if rope.dim() != 3 or rope.shape[0] == 0 or tuple(rope.shape[1:]) != (c.rotary_dim // 2, 2) or rope.dtype != torch.int16:
+                raise X17Error(f"{op} input rope must be int16 [positions, {c.rotary_dim // 2}, 2], got {rope.dtype} {list(rope.shape)}")
+            if not rope.is_cuda or not rope.is_contiguous():
+                raise X17Error(f"{op} input rope must be a contiguous tensor on device cuda")
+        return tokens, n_seqs, max_pages, n_pages
+
+    def append(self, stream, q, kv, seqs, positions, page_table, pages, q_out, rope=None, kv_out=None):
+        """Puts new tokens into the cache: `kv` int8 [tokens, kv_stride] (per key head [K | V], as the KV projection writes it) goes
+        to position positions[t] of sequence seqs[t], keys rotated; the queries `q` [tokens, q_stride] are rotated into `q_out`
+        (both None: keys and values alone). `kv_out`: the rows as stored, for the prefill attention of the same tokens. A
+        negative sequence marks a row of padding. Two tokens of a call must not share a place; outputs must not overlap inputs."""
+        tokens, n_seqs, max_pages, n_pages = self._append_shapes(
+            "paged append", q, kv, seqs, positions, page_table, pages, None, q_out, None, rope, kv_out, DTYPE_INT8)
+        cfg = self.config._c()
+        check(self._lib.x17ai_b200_paged_append(
+            stream.handle, ctypes.byref(cfg), _ptr(q), _ptr(kv), tokens, _ptr(seqs), _ptr(positions), _ptr(page_table), n_seqs,
+            max_pages, _ptr(rope), 0 if rope is None else rope.shape[0], _ptr(pages), n_pages, _ptr(q_out), _ptr(kv_out)))
+
+    def append_scaled(self, stream, q, kv, seqs, positions, page_table, pages, page_scales, q_out, q_scale, rope=None):
+        """The same from bf16 rows, rotated in f32 and quantised with one scale per token and head (absmax / 127): codes into
+        `pages`, scales into `page_scales`, queries into `q_out` int8 and `q_scale` f32 [tokens, n_heads]."""
+        op = "paged append"
+        tokens, n_seqs, max_pages, n_pages = self._append_shapes(
+            op, q, kv, seqs, positions, page_table, pages, page_scales, q_out, q_scale, rope, None, DTYPE_BF16)
+        if (q is None) != (q_scale is None):
+            raise X17Error(f"{op} takes q and q_scale together")
+        if q_scale is not None:
+            matrix_shape(op, "q_scale", q_scale, (tokens, self.config.n_heads), DTYPE_F32)
+        cfg = self.config._c()
+        check(self._lib.x17ai_b200_paged_append_scaled(
+            stream.handle, ctypes.byref(cfg), _ptr(q), _ptr(kv), tokens, _ptr(seqs), _ptr(positions), _ptr(page_table), n_seqs,
+            max_pages, _ptr(rope), 0 if rope is None else rope.shape[0], _ptr(pages), _ptr(page_scales), n_pages, _ptr(q_out),
+            _ptr(q_scale)))
+
+    def _decode_shapes(self, q, pages, page_scales, page_table, kv_lens, sink_k, sink_v, attn_temperature, out, l, out_dtype):
+        c, op = self.config, "paged decode"
+        batch = kv_lens.shape[0] if kv_lens.dim() == 1 else 0
+        if batch == 0 or kv_lens.dtype not in (torch.int32, torch.uint32) or not kv_lens.is_cuda or not kv_lens.is_contiguous():
+            raise X17Error(f"{op} input kv_lens must be a contiguous int32 [sequences] on device cuda, got {kv_lens.dtype} {list(kv_lens.shape)}")
+        rows, _ = matrix_shape(op, "q", q, (None, c.q_stride), DTYPE_INT8)
+        if rows % batch != 0:
+            raise X17Error(f"{op} input q has {rows} rows, which is no multiple of the {batch} sequences")
+        n_pages, _, max_pages = self._pool(op, pages, page_scales, page_table, batch)
+        matrix_shape(op, "sink_k", sink_k, (c.n_heads, c.head_dim), DTYPE_INT8)
+        matrix_shape(op, "sink_v", sink_v, (c.n_heads, c.head_dim), DTYPE_INT8)
+        vector_shape(op, "attn_temperature", attn_temperature, c.n_heads, DTYPE_F32)
+        matrix_shape(op, "out", out, (rows, c.o_stride), out_dtype)
+        if l is not None:
+            matrix_shape(op, "l", l, (rows, c.n_heads), DTYPE_F32)
+        return batch, rows // batch, n_pages, max_pages
+
+    def decode(self, stream, q, pages, page_table, kv_lens, sink_k, sink_v, attn_temperature, out, l=None, window_size=0,
+               n_splits=0):
+        """New tokens over the cache: `q` [sequences * n, q_stride] holds n (1 to 64) new tokens of each sequence, token i of
+        sequence b at position kv_lens[b] + i, which attends the keys in front of that position (the last `window_size` of them,
+        0 = all) and the sink, as AttnKernel.decode does. `out` [rows, o_stride] int8 (FixedI8) or bf16; `l` [rows, n_heads].
+        A sequence of length 0 sees the sink alone (a row of padding costs no more). `n_splits`: CTAs that share a sequence's
+        keys, 1 to 16, 0 = chosen."""
+        out_dtype = DTYPE_BF16 if out.dtype == torch.bfloat16 else DTYPE_INT8
+        batch, n, n_pages, max_pages = self._decode_shapes(
+            q, pages, None, page_table, kv_lens, sink_k, sink_v, attn_temperature, out, l, out_dtype)
+        cfg = self.config._c()
+        check(self._lib.x17ai_b200_paged_decode(
+            stream.handle, ctypes.byref(cfg), batch, n, _ptr(q), _ptr(pages), n_pages, _ptr(page_table), max_pages, _ptr(kv_lens),
+            _ptr(sink_k), _ptr(sink_v), _ptr(attn_temperature), _ptr(out), out_dtype, _ptr(l), window_size, n_splits))
+
+    def decode_scaled(self, stream, q, q_scale, pages, page_scales, page_table, kv_lens, sink_k, sink_v, attn_temperature, out,
+                      l=None, window_size=0, n_splits=0):
+        """The same over a cache with scales: `q_scale` f32 [rows, n_heads], `out` bf16."""
+        batch, n, n_pages, max_pages = self._decode_shapes(
+            q, pages, page_scales, page_table, kv_lens, sink_k, sink_v, attn_temperature, out, l, DTYPE_BF16)
+        matrix_shape("paged decode", "q_scale", q_scale, (batch * n, self.config.n_heads), DTYPE_F32)
+        cfg = self.config._c()
+        check(self._lib.x17ai_b200_paged_decode_scaled(
+            stream.handle, ctypes.byref(cfg), batch, n, _ptr(q), _ptr(q_scale), _ptr(pages), _ptr(page_scales), n_pages,
+            _ptr(page_table), max_pages, _ptr(kv_lens), _ptr(sink_k), _ptr(sink_v), _ptr(attn_temperature), _ptr(out), _ptr(l),
+            window_size, n_splits))
+
+
 @dataclass(frozen=True)
 class GemmConfig:
     """GemmConfig + one epilogue config (gemm.rs:60-366). b is [b_rows, a_cols] (trans = true)."""
