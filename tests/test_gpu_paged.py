@@ -203,12 +203,16 @@ def _cache(rng, table, n_pages, Hk, page, D, scaled, ends):
     return pages, scales, seqs
 
 
-def _decode_bounds(n, top, mean):
+def _decode_bounds(n, top, mean, v, v_scale):
     """Absolute bounds of (value, l). A score carries eight roundings of 2^-24 (temperature, scales, products), a probability
     16 steps of 2^-24 more (exponential, 22 bits kept), a sum over n keys in any order at most n / 4 + 64 in a chain of four
-    partial sums or more; numerator and denominator each have them."""
+    partial sums or more; numerator and denominator each have them. A weight's low part is rounded to f16, whose smallest step is
+    2^-24: half of it, in units of 2^(m - 8) for a score m that is in the total, is at most 2^-33 of the total, and it multiplies
+    |code| times a unit no larger than twice the largest v_scale: with a weight of 2^-60 the value is gone."""
     rel = (8 * top * np.log(2) + 16 + n / 4 + 64) * 2.0 ** -24
-    return 2 * rel * mean, rel / np.log(2) + 8 * 2.0 ** -24 * (top + 8 + np.log2(n + 1))
+    heads = len(mean)
+    far = 2.0 ** -32 * (v_scale.max(initial=0) * np.abs(v.astype(np.float64)).sum(0)).repeat(heads // v.shape[1], axis=0)
+    return 2 * rel * mean + far, rel / np.log(2) + 8 * 2.0 ** -24 * (top + 8 + np.log2(n + 1))
 
 
 def _check_decode(got, got_l, want, want_l, bound, bound_l, fixed):
@@ -249,7 +253,7 @@ def _run_decode(stream, H, Hk, D, page, lens, new, window, scaled, fixed, splits
             row, n = b * new + i, lens[b] + i
             want, want_l, mean, top = o_paged.attend(q[row, :H * D].reshape(H, D), q_scale[row], k[:n], ks[:n], v[:n], vs[:n], sk, sv, temp,
                                                      window)
-            bound, bound_l = _decode_bounds(n, top[:, None], mean)
+            bound, bound_l = _decode_bounds(n, top[:, None], mean, v[:n], vs[:n])
             _check_decode(got[row, :H * D].reshape(H, D), None if got_l is None else got_l[row], want, want_l, bound, bound_l[:, 0], fixed)
 
 
@@ -373,7 +377,7 @@ def test_decode_leaves_out_bad_pages(scaled, splits):
         # the temperature goes by the length, not by the keys that are left
         fix = np.float32(np.log2(n + 4) / np.log2(len(k) + 4))
         want, want_l, mean, top = o_paged.attend(q[b].reshape(H, D), q_scale[b], k, ks, v, vs, sk, sv, temp * fix, 0)
-        bound, bound_l = _decode_bounds(n, top[:, None], mean)
+        bound, bound_l = _decode_bounds(n, top[:, None], mean, v, vs)
         _check_decode(out[b].float().cpu().numpy().reshape(H, D), l[b].cpu().numpy(), want, want_l, bound + 1e-6 * mean, bound_l[:, 0] + 1e-5,
                       False)
 
@@ -402,7 +406,7 @@ def test_offsets_beyond_32_bits(stream):
     assert not pages[n_pages - 2].any() and not pages[:n_pages - 3].any()
     eighth = np.full((n, Hk), 0.125)
     want, want_l, mean, top = o_paged.attend(q.reshape(H, D), np.full(H, 0.125), x[:, :, 0], eighth, x[:, :, 1], eighth, sk, sv, temp, 0)
-    bound, bound_l = _decode_bounds(n, top[:, None], mean)
+    bound, bound_l = _decode_bounds(n, top[:, None], mean, x[:, :, 1], eighth)
     _check_decode(out.float().cpu().numpy().reshape(H, D), l[0].cpu().numpy(), want, want_l, bound, bound_l[:, 0], False)
 
 

@@ -150,6 +150,17 @@ cudaError_t allow_smem(Kernel<KERNEL>, StreamScope const &on, uint32_t bytes) {
 	return e;
 }
 
+// Lets a kernel be launched in clusters of more than eight CTAs, once per kernel and context.
+template <auto KERNEL>
+cudaError_t allow_wide_clusters(Kernel<KERNEL>, StreamScope const &on) {
+	static std::atomic<uint64_t> allowed_in[MAX_DEVICES];
+	std::atomic<uint64_t> &last = allowed_in[on.device];
+	if (last.load(std::memory_order_acquire) == on.state().id) return cudaSuccess;
+	cudaError_t const e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+	if (e == cudaSuccess) last.store(on.state().id, std::memory_order_release);
+	return e;
+}
+
 // Launches with the attribute that lets the kernel's set-up run under the tail of the kernel in front of it
 // (pdl_wait in ptx.cuh), in clusters where `cluster` is not 0. Back to back: the smallest attention 8.2 -> 6.8 us a
 // launch, RMSNorm of 16 rows 3.3 -> 2.8, the few-row GEMMs 1 to 3 us less.
@@ -932,6 +943,15 @@ x17ai_DiagnosticBuffer *paged_append(char const *who, x17ai_CudaStreamHandle *st
 	return launch_result(who);
 }
 
+// CTAs that share a sequence's keys: enough to fill the chip, none with fewer than 128 keys.
+size_t paged_splits(size_t ctas, size_t keys, int sm_count) {
+	size_t const want = size_t(sm_count) * 3;
+	size_t n = ctas >= want ? 1 : (want + ctas - 1) / ctas;
+	size_t const most = keys / 128 > 0 ? keys / 128 : 1;
+	n = n > most ? most : n;
+	return n > 8 ? 8 : n;
+}
+
 template <bool SCALED>
 x17ai_DiagnosticBuffer *paged_decode(char const *who, x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, size_t batch,
 									 size_t n_tokens, int8_t const *q, float const *q_scale, int8_t const *pages, float const *scales,
@@ -974,22 +994,37 @@ x17ai_DiagnosticBuffer *paged_decode(char const *who, x17ai_CudaStreamHandle *st
 	p.n_heads = uint32_t(cfg->n_heads);
 	p.n_tokens = uint32_t(n_tokens);
 	p.window = window_size == 0 || window_size > 0xFFFFFFF0u ? 0xFFFFFFFFu : uint32_t(window_size);
+	p.out_i8 = out_dtype == X17AI_DTYPE_INT8;
 	p.status = scope.state().status;
 	cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-	auto go = [&](auto dim, auto out_i8) {
+	// the rows of a key head in as few CTAs of at most eight as they need, evenly
+	size_t const rows = cfg->n_heads / cfg->n_kv_heads * n_tokens;
+	p.chunks = uint32_t((rows + x17::paged_cfg::ROWS - 1) / x17::paged_cfg::ROWS);
+	p.chunk_rows = uint32_t((rows + p.chunks - 1) / p.chunks);
+	p.chunks = uint32_t((rows + p.chunk_rows - 1) / p.chunk_rows);
+	size_t const ctas = cfg->n_kv_heads * p.chunks * batch;
+	size_t const capacity = max_pages * cfg->page_size;
+	size_t const keys = p.window < capacity ? p.window : capacity;
+	if (n_splits == 0) n_splits = paged_splits(ctas, keys, scope.state().sm_count);
+	cudaError_t ce = cudaSuccess;
+	auto go = [&](auto dim) {
 		constexpr uint32_t D = decltype(dim)::value;
-		(void)launch(Kernel<&x17::paged_decode_kernel<D, SCALED, decltype(out_i8)::value>>{},
-					 dim3(unsigned(cfg->n_heads * n_tokens), unsigned(batch)), 128, 0, s, dim3(NO_CLUSTER), p);
+		using K = Kernel<&x17::paged_decode_kernel<D, SCALED>>;
+		constexpr uint32_t ring = x17::paged_cfg::RING_BYTES<D, SCALED>;
+		ce = allow_smem(K{}, scope, ring + x17::paged_cfg::part_bytes<D>(x17::paged_cfg::MAX_SPLITS, x17::paged_cfg::ROWS));
+		if (ce == cudaSuccess) ce = allow_wide_clusters(K{}, scope);
+		if (ce != cudaSuccess) return;
+		(void)launch(K{}, dim3(unsigned(cfg->n_kv_heads * p.chunks), unsigned(batch), unsigned(n_splits)), x17::paged_cfg::THREADS,
+					 ring + x17::paged_cfg::part_bytes<D>(uint32_t(n_splits), p.chunk_rows), s,
+					 n_splits > 1 ? dim3(1, 1, unsigned(n_splits)) : dim3(NO_CLUSTER), p);
 	};
-	auto go_dim = [&](auto dim) {
-		if constexpr (!SCALED) {
-			if (out_dtype == X17AI_DTYPE_INT8) return go(dim, std::true_type{});
-		}
-		go(dim, std::false_type{});
-	};
-	if (cfg->head_dim == 128) go_dim(std::integral_constant<uint32_t, 128>{});
-	else if (cfg->head_dim == 64) go_dim(std::integral_constant<uint32_t, 64>{});
-	else go_dim(std::integral_constant<uint32_t, 32>{});
+	if (cfg->head_dim == 128) go(std::integral_constant<uint32_t, 128>{});
+	else if (cfg->head_dim == 64) go(std::integral_constant<uint32_t, 64>{});
+	else go(std::integral_constant<uint32_t, 32>{});
+	if (ce != cudaSuccess) {
+		(void)cudaGetLastError();
+		return make_diag("x17ai_b200: kernel attributes", who, ": kernel attributes: ", cudaGetErrorString(ce));
+	}
 	return launch_result(who);
 }
 

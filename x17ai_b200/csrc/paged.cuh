@@ -52,7 +52,9 @@ struct PagedDecodeParams {
 	f32 *l;                 // [batch * n_tokens][n_heads] or null
 	u64 q_stride, o_stride;
 	u32 n_heads, n_tokens;
+	u32 chunk_rows, chunks; // rows (query heads of a group x new tokens) of a CTA, CTAs that a key head's rows take
 	u32 window;             // 0xFFFFFFFF = unbounded
+	bool out_i8;
 	u32 *status;
 };
 
@@ -144,89 +146,430 @@ paged_append_kernel(const PagedAppendParams p) {
 	}
 }
 
-// One CTA per (query head, new token): four warps take every fourth key, a lane D / 32 dims.
-template <u32 D, bool SCALED, bool OUT_I8>
-__global__ void __launch_bounds__(128)
-paged_decode_kernel(const PagedDecodeParams p) {
-	pdl_launch_dependents();
-	pdl_wait();
-	constexpr u32 V = D / 32;
-	u32 const warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-	u32 const head = blockIdx.x / p.n_tokens, tok = blockIdx.x % p.n_tokens, b = blockIdx.y;
-	u32 const kvh = head / (p.n_heads / p.pool.n_kv_heads);
-	u64 const row = u64(b) * p.n_tokens + tok;
-	u32 const capacity = p.pool.max_pages << p.pool.page_shift;
-	u32 const n = min(u32(max(p.kv_lens[b], 0)) + tok, capacity);
-	u32 const seen = min(n, p.window), lo = n - seen;
-	f32 const q_scale = SCALED ? p.q_scale[row * p.n_heads + head] : 0.125f;
-	f32 const base = f32(D == 128 ? 0.08838834764831845 : D == 64 ? 0.125 : 0.17677669529663687);
-	f32 const temp = base * log2f(f32(seen + 4)) * p.temperature[head] * q_scale;
-	f32 q[V], o[V];
-	f32 dot = 0.0f;
+// ---- decode ------------------------------------------------------------------------------------
+//
+// A pass over a cache is bound by HBM: the kernel's job is to keep enough bytes in flight and to stay out of their way. One
+// CTA works on the rows (query heads of a group, times new tokens; eight at most) that share a key head, so a key is read
+// once for all of them; up to 16 CTAs (a cluster) share a sequence's keys, four warps a CTA's. A warp takes 16 or 32 keys a
+// step (4 KB) out of a ring of its own in shared memory that it fills itself, three steps ahead, with cp.async: no barrier
+// among warps until the end. A page of a head is one run of memory and a step's page is known long before (32 entries of the page table
+// sit in a warp's lanes), so pages cost no more than a contiguous cache.
+//
+// Scores: mma m16n8k32 (s8 x s8 -> s32, exact), rows as its M, keys as its N; a lane's bytes of a key row are consecutive, the
+// query's are permuted the same way. Probabilities keep 22 bits: e = hi + lo in f16, hi as rows 0-7 and lo as rows 8-15
+// of mma m16n8k16 (f16 x f16 -> f32), which would be empty otherwise. V's codes are exact in f16 (integer added to 1024 as
+// bits). Weights are 2^(x - m + 8) against a maximum m that moves only when a score passes it by 6: between 2^-38 and 2^14 of
+// m's nothing is lost to f16's range. m starts at the sink's score, so no key and no row leaves it undefined.
+
+namespace paged_cfg {
+constexpr u32 WARPS = 4, THREADS = WARPS * 32;
+constexpr u32 STAGES = 4;
+constexpr u32 ROWS = 8;          // rows of a CTA
+constexpr u32 MAX_SPLITS = 16;   // CTAs of a cluster
+constexpr f32 SHIFT = 8.0f, ARG_MAX = 14.0f;   // weights are 2^(x - m + SHIFT), at most 2^ARG_MAX (f16 ends below 2^16)
+template <u32 D>
+constexpr u32 KEYS = D == 128 ? 16 : 32;       // of a step
+template <u32 D>
+constexpr u32 ROW_BYTES = 2 * D + 16;          // of a key in the ring: rows 16 bytes off each other's banks
+template <u32 D, bool SCALED>
+constexpr u32 STAGE_BYTES = KEYS<D> * (ROW_BYTES<D> + (SCALED ? 8 : 0));
+template <u32 D, bool SCALED>
+constexpr u32 RING_BYTES = WARPS * STAGES * STAGE_BYTES<D, SCALED>;
+// the parts of a cluster's CTAs, in the first one: [splits][rows][D + 2] f32
+template <u32 D>
+constexpr u32 part_bytes(u32 splits, u32 rows) {
+	return splits > 1 ? splits * rows * (D + 2) * 4 : 0;
+}
+}  // namespace paged_cfg
+
+X17_DEV void cp_async_16(u32 dst, void const *src) {
+	asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+X17_DEV void cp_async_8(u32 dst, void const *src) {
+	asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+X17_DEV void cp_async_commit() {
+	asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <u32 N>
+X17_DEV void cp_async_wait() {
+	asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// c[0], c[1]: row lane / 4, columns 2 (lane % 4) and the next one; rows 8-15 of A are zero, their sums are not kept
+X17_DEV void mma_s8(i32 (&c)[2], u32 a0, u32 a2, u32 b0, u32 b1) {
+	i32 unused2, unused3;
+	asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%9, %10, %5, %5};"
+		: "=r"(c[0]), "=r"(c[1]), "=r"(unused2), "=r"(unused3)
+		: "r"(a0), "r"(0), "r"(a2), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]));
+}
+X17_DEV void mma_f16(f32 (&c)[4], u32 const (&a)[4], u32 b0, u32 b1) {
+	asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+		: "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+		: "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+X17_DEV u32 f32x2_to_f16x2(f32 lo, f32 hi) {
+	u32 r;
+	asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+	return r;
+}
+X17_DEV void f16x2_values(u32 h2, f32 &lo, f32 &hi) {
+	asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}" : "=f"(lo), "=f"(hi) : "r"(h2));
+}
+// byte J of a and of b, signed, as f16x2: the bits 0x6400 + (code + 128) are 1024 + 128 + code
+template <u32 J>
+X17_DEV u32 codes_to_f16x2(u32 a, u32 b) {
+	u32 const t = (__byte_perm(a, b, (J + 4) << 8 | J) & 0x00FF00FFu) ^ 0x64806480u;
+	u32 r;
+	asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(t), "r"(0xE480E480u));
+	return r;
+}
+// N words (1, 2, 4 or 8) from shared memory
+template <u32 N>
+X17_DEV void ld_shared_words(u32 addr, u32 (&w)[N]) {
+	if constexpr (N == 1) {
+		asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(addr) : "memory");
+	} else if constexpr (N == 2) {
+		asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr) : "memory");
+	} else {
 #pragma unroll
-	for (u32 j = 0; j < V; ++j) {
-		q[j] = f32(p.q[row * p.q_stride + head * D + j * 32 + lane]);
-		dot += q[j] * f32(p.sink_k[head * D + j * 32 + lane]);
-		o[j] = 0.0f;
-	}
-	auto reduce = [](f32 v) {
-#pragma unroll
-		for (u32 mask = 16; mask > 0; mask >>= 1) v += __shfl_xor_sync(0xffffffffu, v, mask);
-		return v;
-	};
-	f32 const sink = reduce(dot) * (temp * 0.125f);
-	f32 m = sink, sum = 0.0f;
-	for (u32 key = lo + warp; key < n; key += 4) {
-		u32 page, slot;
-		if (!paged_slot(p.pool, i32(b), i32(key), page, slot)) {
-			if (lane == 0) report_status(p.status, ST_BAD_INDEX, b);
-			continue;
+		for (u32 i = 0; i < N; i += 4) {
+			uint4 const v = ld_shared_v4(addr + i * 4);
+			w[i] = v.x;
+			w[i + 1] = v.y;
+			w[i + 2] = v.z;
+			w[i + 3] = v.w;
 		}
-		u64 const at = p.pool.row(page, kvh, slot);
-		i8 const *k = p.pool.pages + at * 2 * D;
-		f32 d = 0.0f;
+	}
+}
+template <u32 N>
+X17_DEV void ld_global_words(i8 const *p, u32 (&w)[N]) {
+	if constexpr (N % 4 == 0) {
 #pragma unroll
-		for (u32 j = 0; j < V; ++j) d += q[j] * f32(k[j * 32 + lane]);
-		f32 const x = reduce(d) * (temp * (SCALED ? p.pool.scales[at * 2] : 0.125f));
-		if (x > m) {
-			f32 const a = exp2f(m - x);
+		for (u32 i = 0; i < N; i += 4) {
+			uint4 const v = reinterpret_cast<uint4 const *>(p)[i / 4];
+			w[i] = v.x;
+			w[i + 1] = v.y;
+			w[i + 2] = v.z;
+			w[i + 3] = v.w;
+		}
+	} else {
+		uint2 const v = *reinterpret_cast<uint2 const *>(p);
+		w[0] = v.x;
+		w[1] = v.y;
+	}
+}
+
+// One output: the keys' (m, s, v), m being a maximum less SHIFT that is no smaller than the sink's, with the sink token.
+template <u32 D>
+X17_DEV void paged_finish(PagedDecodeParams const &p, u32 b, u32 kvh, u32 row0, u32 r, u32 d, f32 m, f32 s, f32 v, f32 sink) {
+	u32 const group = p.n_heads / p.pool.n_kv_heads;
+	u32 const row = row0 + r, head = kvh * group + row % group;
+	u64 const out_row = u64(b) * p.n_tokens + row / group;
+	f32 const a = ex2_approx(sink - m + paged_cfg::SHIFT);
+	s += a;
+	v = __fmaf_rn(f32(p.sink_v[u64(head) * D + d]) * 0.125f, a, v);
+	v = __fdiv_rn(v, s);
+	u64 const at = out_row * p.o_stride + head * D + d;
+	if (p.out_i8) static_cast<i8 *>(p.out)[at] = i8(f32_to_fixedi8(v * 8.0f));
+	else static_cast<u16 *>(p.out)[at] = u16(cvt_bf16x2(v, 0.0f));
+	if (d == 0 && p.l != nullptr) p.l[out_row * p.n_heads + head] = log2f(255.0f * s) + m;
+}
+
+// Grid (key head and chunk of rows, sequence, split); the splits of one (x, y) are a cluster.
+template <u32 D, bool SCALED>
+__global__ void __launch_bounds__(paged_cfg::THREADS, 3)
+paged_decode_kernel(const PagedDecodeParams p) {
+	using namespace paged_cfg;
+	constexpr u32 KS = KEYS<D>, SUBS = KS / 16;      // a step's runs of 16 keys lie in one page each
+	constexpr u32 KW = D / 16;                       // words of a key row that a lane holds
+	constexpr u32 VW = D / 32;                       // words of a value row that a lane holds
+	constexpr u32 RB = ROW_BYTES<D>;
+	constexpr u32 NEG_INF = 0xFF800000u;
+	extern __shared__ __align__(16) u8 smem[];
+	__shared__ f32 sh_sink[ROWS], sh_m[WARPS][ROWS], sh_s[WARPS][ROWS];
+	u32 const warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+	u32 const g = lane >> 2, t = lane & 3;
+	u32 const splits = gridDim.z;
+
+	if (splits > 1) cluster_arrive();   // "this CTA runs"
+	pdl_wait();
+	u32 const group = p.n_heads / p.pool.n_kv_heads;
+	u32 const kvh = blockIdx.x / p.chunks, chunk = blockIdx.x % p.chunks, b = blockIdx.y;
+	u32 const n_rows_all = group * p.n_tokens;
+	u32 const row0 = chunk * p.chunk_rows;
+	u32 const rows = min(p.chunk_rows, n_rows_all - row0);
+	i32 const len = p.kv_lens[b];
+
+	// this lane's row: a head of the group for one of the new tokens (rows behind the last one repeat it and are not stored)
+	u32 const my_row = row0 + min(g, rows - 1);
+	u32 const tok = my_row / group, head = kvh * group + my_row % group;
+	u64 const q_row = u64(b) * p.n_tokens + tok;
+	u32 qw[KW], skw[KW];
+	ld_global_words(p.q + q_row * p.q_stride + head * D + t * (D / 4), qw);
+	ld_global_words(p.sink_k + u64(head) * D + t * (D / 4), skw);
+	f32 temp = p.temperature[head];
+	if constexpr (SCALED) temp *= p.q_scale[q_row * p.n_heads + head];
+
+	u32 const capacity = p.pool.max_pages << p.pool.page_shift;
+	auto length = [&](u32 tk) { return min(u32(max(len, 0)) + tk, capacity); };
+	auto first = [&](u32 n) { return n - min(n, p.window); };
+	u32 const tok_lo = row0 / group, tok_hi = (row0 + rows - 1) / group;
+	u32 const n = length(tok), lo = first(n);                       // of this lane's row
+	u32 const n_hi = length(tok_hi), lo_all = first(length(tok_lo));   // the union of the rows' keys: [lo_all, n_hi)
+	u32 const n_min = length(tok_lo), lo_max = first(n_hi);            // what every row sees: [lo_max, n_min)
+
+	// the CTA's steps of KS keys from `base` on, dealt out to its warps in turn
+	u32 const base = lo_all & ~15u;
+	u32 const n_steps = n_hi > base ? (n_hi - base + KS - 1) / KS : 0;
+	u32 const per_cta = (n_steps + splits - 1) / splits;
+	u32 const step_lo = min(blockIdx.z * per_cta, n_steps), step_hi = min(step_lo + per_cta, n_steps);
+	u32 const n_own = step_hi - step_lo > warp ? (step_hi - step_lo - warp + WARPS - 1) / WARPS : 0;
+
+	u32 const ring = smem_u32(smem) + warp * STAGES * STAGE_BYTES<D, SCALED>;
+	u32 bad = 0;                       // bit stage * SUBS + sub: that run's page is none
+	u32 page_now = 0, page_next = 0;   // page table entries of the warp's runs, one a lane
+	auto run_key = [&](u32 run) { return base + ((step_lo + warp + run / SUBS * WARPS) * SUBS + run % SUBS) * 16; };
+	auto page_entry = [&](u32 run) -> u32 {
+		u32 const key = run_key(run);
+		return run < n_own * SUBS && key < n_hi ? u32(p.pool.table[u64(b) * p.pool.max_pages + (key >> p.pool.page_shift)]) : 0u;
+	};
+	page_next = page_entry(lane);
+	auto issue = [&](u32 i) {
+		if (i < n_own) {
+			u32 const stage = i % STAGES, dst0 = ring + stage * STAGE_BYTES<D, SCALED>;
+			if (i * SUBS % 32 == 0) {
+				page_now = page_next;
+				page_next = page_entry(i * SUBS + 32 + lane);
+			}
+#pragma unroll
+			for (u32 j = 0; j < SUBS; ++j) {
+				u32 const page = __shfl_sync(0xffffffffu, page_now, (i * SUBS + j) & 31);
+				u32 const key = run_key(i * SUBS + j);
+				u32 const bit = 1u << (stage * SUBS + j);
+				bool const ok = page < p.pool.n_pages;
+				bad = ok ? bad & ~bit : bad | bit;
+				if (!ok) {
+					if (lane == 0 && key < n_hi) report_status(p.status, ST_BAD_INDEX, b);
+				} else if (key < n_hi) {
+					u64 const row = p.pool.row(page, kvh, key & ((1u << p.pool.page_shift) - 1));
+					i8 const *src = p.pool.pages + row * 2 * D;
+					constexpr u32 CHUNKS = 2 * D / 16;   // of a row
+#pragma unroll
+					for (u32 c = 0; c < CHUNKS / 2; ++c) {
+						u32 const at = c * 32 + lane;
+						cp_async_16(dst0 + (j * 16 + at / CHUNKS) * RB + at % CHUNKS * 16, src + at * 16);
+					}
+					if constexpr (SCALED) {
+						if (lane < 16) cp_async_8(dst0 + KS * RB + (j * 16 + lane) * 8, p.pool.scales + (row + lane) * 2);
+					}
+				}
+			}
+		}
+		cp_async_commit();
+	};
+#pragma unroll
+	for (u32 i = 0; i + 1 < STAGES; ++i) issue(i);
+
+	// temperature D^-1/2 log2(min(W', n) + 4) temp_h, times the scales that are not the key's
+	constexpr f32 ROOT = f32(D == 128 ? 0.08838834764831845 : D == 64 ? 0.125 : 0.17677669529663687);
+	temp *= ROOT * log2f(f32(n - lo + 4)) * (SCALED ? 1.0f : 0.015625f);
+	i32 dot = 0;
+#pragma unroll
+	for (u32 i = 0; i < KW; ++i) dot = __dp4a(i32(qw[i]), i32(skw[i]), dot);
+	dot += __shfl_xor_sync(0xffffffffu, dot, 1);
+	dot += __shfl_xor_sync(0xffffffffu, dot, 2);
+	f32 const sink = f32(dot) * (SCALED ? temp * 0.125f : temp);
+	f32 neg_m = SHIFT - sink, sum = 0.0f;
+	f32 v_unit = 0.0f, v_inv = 0.0f;   // SCALED: weights carry v_scale / v_unit, a power of two no smaller than any seen
+	f32 o[D / 8][4];
+#pragma unroll
+	for (u32 i = 0; i < D / 8; ++i) {
+#pragma unroll
+		for (u32 j = 0; j < 4; ++j) o[i][j] = 0.0f;
+	}
+
+#pragma unroll 1
+	for (u32 i = 0; i < n_own; ++i) {
+		cp_async_wait<STAGES - 2>();
+		__syncwarp();
+		issue(i + STAGES - 1);
+		u32 const stage = i % STAGES, src = ring + stage * STAGE_BYTES<D, SCALED>;
+		u32 const key0 = base + (step_lo + warp + i * WARPS) * KS;
+		// ---- scores ----
+		f32 arg[KS / 8][2];
+		f32 vs[KS / 8][2];
+#pragma unroll
+		for (u32 n8 = 0; n8 < KS / 8; ++n8) {
+			u32 kw[KW];
+			ld_shared_words(src + (n8 * 8 + g) * RB + t * (D / 4), kw);
+			i32 c[2] = {0, 0};
+#pragma unroll
+			for (u32 k = 0; k < KW; k += 2) mma_s8(c, qw[k], qw[k + 1], kw[k], kw[k + 1]);
+			if constexpr (SCALED) {
+				uint4 const s4 = ld_shared_v4(src + KS * RB + (n8 * 8 + t * 2) * 8);
+				arg[n8][0] = __fmaf_rn(f32(c[0]) * __uint_as_float(s4.x), temp, neg_m);
+				arg[n8][1] = __fmaf_rn(f32(c[1]) * __uint_as_float(s4.z), temp, neg_m);
+				vs[n8][0] = __uint_as_float(s4.y);
+				vs[n8][1] = __uint_as_float(s4.w);
+			} else {
+				arg[n8][0] = __fmaf_rn(f32(c[0]), temp, neg_m);
+				arg[n8][1] = __fmaf_rn(f32(c[1]), temp, neg_m);
+			}
+		}
+		u32 const bad_now = bad >> (stage * SUBS) & ((1u << SUBS) - 1);
+		if (key0 < lo_max || key0 + KS > n_min || bad_now != 0) {
+#pragma unroll
+			for (u32 n8 = 0; n8 < KS / 8; ++n8) {
+#pragma unroll
+				for (u32 e = 0; e < 2; ++e) {
+					u32 const key = key0 + n8 * 8 + t * 2 + e;
+					if (key < lo || key >= n || (bad_now >> (n8 / 2) & 1)) {
+						arg[n8][e] = __uint_as_float(NEG_INF);
+						vs[n8][e] = 0.0f;   // (what lies there may be anything)
+					}
+				}
+			}
+		}
+		// ---- the maximum, when a score has passed it ----
+		f32 top = arg[0][0];
+#pragma unroll
+		for (u32 n8 = 0; n8 < KS / 8; ++n8) top = fmaxf(top, fmaxf(arg[n8][0], arg[n8][1]));
+		if (__any_sync(0xffffffffu, top > ARG_MAX)) {
+			top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+			top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+			f32 const up = fmaxf(top - SHIFT, 0.0f), a = ex2_approx(-up);
+			neg_m -= up;
 			sum *= a;
 #pragma unroll
-			for (u32 j = 0; j < V; ++j) o[j] *= a;
-			m = x;
+			for (u32 n8 = 0; n8 < KS / 8; ++n8) {
+				arg[n8][0] -= up;
+				arg[n8][1] -= up;
+			}
+#pragma unroll
+			for (u32 j = 0; j < D / 8; ++j) {
+#pragma unroll
+				for (u32 e = 0; e < 4; ++e) o[j][e] *= a;
+			}
 		}
-		f32 const e = exp2f(x - m);
-		f32 const w = e * (SCALED ? p.pool.scales[at * 2 + 1] : 0.125f);
-		sum += e;
+		if constexpr (SCALED) {
+			f32 most = vs[0][0];
 #pragma unroll
-		for (u32 j = 0; j < V; ++j) o[j] += w * f32(k[D + j * 32 + lane]);
+			for (u32 n8 = 0; n8 < KS / 8; ++n8) most = fmaxf(most, fmaxf(vs[n8][0], vs[n8][1]));
+			if (__any_sync(0xffffffffu, most > v_unit)) {
+#pragma unroll
+				for (u32 mask = 16; mask > 0; mask >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, mask));
+				f32 const unit = __uint_as_float(__float_as_uint(fminf(most, 0x1p125f)) & 0x7F800000u) * 2.0f;
+				f32 const a = v_unit * __frcp_rn(unit);   // powers of two
+				v_unit = unit;
+				v_inv = __frcp_rn(unit);
+#pragma unroll
+				for (u32 j = 0; j < D / 8; ++j) {
+#pragma unroll
+					for (u32 e = 0; e < 4; ++e) o[j][e] *= a;
+				}
+			}
+		}
+		// ---- weights and values ----
+#pragma unroll
+		for (u32 j = 0; j < SUBS; ++j) {
+			u32 a[4];
+#pragma unroll
+			for (u32 h = 0; h < 2; ++h) {
+				f32 e0 = ex2_approx(arg[2 * j + h][0]), e1 = ex2_approx(arg[2 * j + h][1]);
+				sum += e0 + e1;
+				if constexpr (SCALED) {
+					e0 *= vs[2 * j + h][0] * v_inv;
+					e1 *= vs[2 * j + h][1] * v_inv;
+				}
+				a[2 * h] = f32x2_to_f16x2(e0, e1);
+				f32 h0, h1;
+				f16x2_values(a[2 * h], h0, h1);
+				a[2 * h + 1] = f32x2_to_f16x2(e0 - h0, e1 - h1);
+			}
+			u32 const v0 = src + (j * 16 + t * 2) * RB + D + g * (D / 8);
+			u32 va[VW], vb[VW], vc[VW], vd[VW];
+			ld_shared_words(v0, va);
+			ld_shared_words(v0 + RB, vb);
+			ld_shared_words(v0 + 8 * RB, vc);
+			ld_shared_words(v0 + 9 * RB, vd);
+#pragma unroll
+			for (u32 w = 0; w < VW; ++w) {
+				mma_f16(o[4 * w], a, codes_to_f16x2<0>(va[w], vb[w]), codes_to_f16x2<0>(vc[w], vd[w]));
+				mma_f16(o[4 * w + 1], a, codes_to_f16x2<1>(va[w], vb[w]), codes_to_f16x2<1>(vc[w], vd[w]));
+				mma_f16(o[4 * w + 2], a, codes_to_f16x2<2>(va[w], vb[w]), codes_to_f16x2<2>(vc[w], vd[w]));
+				mma_f16(o[4 * w + 3], a, codes_to_f16x2<3>(va[w], vb[w]), codes_to_f16x2<3>(vc[w], vd[w]));
+			}
+		}
 	}
-	__shared__ f32 sh_o[4][D], sh_m[4], sh_s[4];
+	cp_async_wait<0>();
+	sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+	sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+
+	// ---- merge the warps: [warp][row][D] in the ring's place ----
+	__syncthreads();
+	f32 *parts = reinterpret_cast<f32 *>(smem);
+	if (g < rows) {
+		f32 const unit = SCALED ? v_unit : 0.125f;
+		// a lane's columns of tile j are dims (2 t) D / 8 + j and (2 t + 1) D / 8 + j
+		f32 *dst = parts + (warp * ROWS + g) * D + 2 * t * (D / 8);
 #pragma unroll
-	for (u32 j = 0; j < V; ++j) sh_o[warp][j * 32 + lane] = o[j];
-	if (lane == 0) {
-		sh_m[warp] = m;
-		sh_s[warp] = sum;
+		for (u32 j = 0; j < D / 8; j += 4) {
+			*reinterpret_cast<float4 *>(dst + j) = make_float4((o[j][0] + o[j][2]) * unit, (o[j + 1][0] + o[j + 1][2]) * unit,
+															   (o[j + 2][0] + o[j + 2][2]) * unit, (o[j + 3][0] + o[j + 3][2]) * unit);
+			*reinterpret_cast<float4 *>(dst + D / 8 + j) = make_float4((o[j][1] + o[j][3]) * unit, (o[j + 1][1] + o[j + 1][3]) * unit,
+																	   (o[j + 2][1] + o[j + 2][3]) * unit, (o[j + 3][1] + o[j + 3][3]) * unit);
+		}
+		if (t == 0) {
+			sh_m[warp][g] = -neg_m;   // m - SHIFT
+			sh_s[warp][g] = sum;
+			if (warp == 0) sh_sink[g] = sink - SHIFT;
+		}
 	}
 	__syncthreads();
-	u32 const d = threadIdx.x;
-	if (d >= D) return;
-	f32 top = sink;
+	if (splits > 1) cluster_wait();   // the first CTA runs (asked for at entry): its shared memory can be written
+	f32 *recv = reinterpret_cast<f32 *>(smem + RING_BYTES<D, SCALED>);
+	for (u32 at = threadIdx.x; at < rows * D; at += THREADS) {
+		u32 const r = at / D, d = at % D;
+		f32 m = sh_m[0][r];
 #pragma unroll
-	for (u32 w = 0; w < 4; ++w) top = fmaxf(top, sh_m[w]);
-	f32 const es = exp2f(sink - top);
-	f32 total = es, acc = es * f32(p.sink_v[head * D + d]) * 0.125f;
+		for (u32 w = 1; w < WARPS; ++w) m = fmaxf(m, sh_m[w][r]);
+		f32 s = 0.0f, v = 0.0f;
 #pragma unroll
-	for (u32 w = 0; w < 4; ++w) {
-		f32 const a = exp2f(sh_m[w] - top);
-		total += a * sh_s[w];
-		acc += a * sh_o[w][d];
+		for (u32 w = 0; w < WARPS; ++w) {
+			f32 const a = ex2_approx(sh_m[w][r] - m);
+			s = __fmaf_rn(sh_s[w][r], a, s);
+			v = __fmaf_rn(parts[(w * ROWS + r) * D + d], a, v);
+		}
+		if (splits > 1) {
+			u32 const dst = map_to_cta(smem_u32(recv + (blockIdx.z * rows + r) * (D + 2)), 0);
+			st_cluster_f32(dst + d * 4, v);
+			if (d == 0) {
+				st_cluster_f32(dst + D * 4, m);
+				st_cluster_f32(dst + D * 4 + 4, s);
+			}
+		} else {
+			paged_finish<D>(p, b, kvh, row0, r, d, m, s, v, sh_sink[r]);
+		}
 	}
-	f32 const v = __fdiv_rn(acc, total);
-	u64 const at = row * p.o_stride + head * D + d;
-	if constexpr (OUT_I8) static_cast<i8 *>(p.out)[at] = i8(f32_to_fixedi8(v * 8.0f));
-	else static_cast<u16 *>(p.out)[at] = u16(cvt_bf16x2(v, 0.0f));
-	if (d == 0 && p.l != nullptr) p.l[row * p.n_heads + head] = log2f(255.0f * total) + top;
+	pdl_launch_dependents();   // not earlier: a next call's clusters would be packed onto the few SMs with room
+	if (splits > 1) {
+		__syncwarp();
+		cluster_arrive();              // this CTA's part is stored
+		if (blockIdx.z != 0) return;
+		cluster_wait();
+		for (u32 at = threadIdx.x; at < rows * D; at += THREADS) {
+			u32 const r = at / D, d = at % D;
+			f32 m = sh_sink[r], s = 0.0f, v = 0.0f;
+			for (u32 z = 0; z < splits; ++z) m = fmaxf(m, recv[(z * rows + r) * (D + 2) + D]);
+			for (u32 z = 0; z < splits; ++z) {
+				f32 const *part = recv + (z * rows + r) * (D + 2);
+				f32 const a = ex2_approx(part[D] - m);
+				s = __fmaf_rn(part[D + 1], a, s);
+				v = __fmaf_rn(part[d], a, v);
+			}
+			paged_finish<D>(p, b, kvh, row0, r, d, m, s, v, sh_sink[r]);
+		}
+	}
 }
 
 }  // namespace x17
