@@ -156,19 +156,29 @@ paged_append_kernel(const PagedAppendParams p) {
 // sit in a warp's lanes), so pages cost no more than a contiguous cache.
 //
 // Scores: mma m16n8k32 (s8 x s8 -> s32, exact), rows as its M, keys as its N; a lane's bytes of a key row are consecutive, the
-// query's are permuted the same way. Probabilities keep 22 bits: e = hi + lo in f16, hi as rows 0-7 and lo as rows 8-15
-// of mma m16n8k16 (f16 x f16 -> f32), which would be empty otherwise. V's codes are exact in f16 (integer added to 1024 as
+// query's are permuted the same way. Values: mma m16n8k16 (f16 x f16 -> f32) with V transposed as its first operand (dims as M)
+// and the weights as the second (rows as N), which is how the scores' fragments lie; accumulators are a lane's 16 dims of two rows.
+// Weights keep 22 bits: e = hi + lo in f16, two products into the same sums. V's codes are exact in f16 (integer added to 1024 as
 // bits). Weights are 2^(x - m + 8) against a maximum m that moves only when a score passes it by 6: between 2^-38 and 2^14 of
 // m's nothing is lost to f16's range. m starts at the sink's score, so no key and no row leaves it undefined.
 
 namespace paged_cfg {
 constexpr u32 WARPS = 4, THREADS = WARPS * 32;
-constexpr u32 STAGES = 4;
+#ifndef PG_STAGES
+#define PG_STAGES 4
+#endif
+#ifndef PG_CTAS
+#define PG_CTAS 3
+#endif
+#ifndef PG_KEYS
+#define PG_KEYS 16
+#endif
+constexpr u32 STAGES = PG_STAGES;
 constexpr u32 ROWS = 8;          // rows of a CTA
 constexpr u32 MAX_SPLITS = 16;   // CTAs of a cluster
 constexpr f32 SHIFT = 8.0f, ARG_MAX = 14.0f;   // weights are 2^(x - m + SHIFT), at most 2^ARG_MAX (f16 ends below 2^16)
 template <u32 D>
-constexpr u32 KEYS = D == 128 ? 16 : 32;       // of a step
+constexpr u32 KEYS = D == 128 ? PG_KEYS : 32;       // of a step
 template <u32 D>
 constexpr u32 ROW_BYTES = 2 * D + 16;          // of a key in the ring: rows 16 bytes off each other's banks
 template <u32 D, bool SCALED>
@@ -277,7 +287,7 @@ X17_DEV void paged_finish(PagedDecodeParams const &p, u32 b, u32 kvh, u32 row0, 
 
 // Grid (key head and chunk of rows, sequence, split); the splits of one (x, y) are a cluster.
 template <u32 D, bool SCALED>
-__global__ void __launch_bounds__(paged_cfg::THREADS, 3)
+__global__ void __launch_bounds__(paged_cfg::THREADS, PG_CTAS)
 paged_decode_kernel(const PagedDecodeParams p) {
 	using namespace paged_cfg;
 	constexpr u32 KS = KEYS<D>, SUBS = KS / 16;      // a step's runs of 16 keys lie in one page each
@@ -381,9 +391,10 @@ paged_decode_kernel(const PagedDecodeParams p) {
 	f32 const sink = f32(dot) * (SCALED ? temp * 0.125f : temp);
 	f32 neg_m = SHIFT - sink, sum = 0.0f;
 	f32 v_unit = 0.0f, v_inv = 0.0f;   // SCALED: weights carry v_scale / v_unit, a power of two no smaller than any seen
-	f32 o[D / 8][4];
+	// tile j: dims g D / 8 + 2 j ([0], [1]) and + 2 j + 1 ([2], [3]) of rows 2 t ([0], [2]) and 2 t + 1 ([1], [3])
+	f32 o[D / 16][4];
 #pragma unroll
-	for (u32 i = 0; i < D / 8; ++i) {
+	for (u32 i = 0; i < D / 16; ++i) {
 #pragma unroll
 		for (u32 j = 0; j < 4; ++j) o[i][j] = 0.0f;
 	}
@@ -438,6 +449,7 @@ paged_decode_kernel(const PagedDecodeParams p) {
 			top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
 			top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
 			f32 const up = fmaxf(top - SHIFT, 0.0f), a = ex2_approx(-up);
+			f32 const a0 = __shfl_sync(0xffffffffu, a, t * 8), a1 = __shfl_sync(0xffffffffu, a, t * 8 + 4);
 			neg_m -= up;
 			sum *= a;
 #pragma unroll
@@ -446,9 +458,11 @@ paged_decode_kernel(const PagedDecodeParams p) {
 				arg[n8][1] -= up;
 			}
 #pragma unroll
-			for (u32 j = 0; j < D / 8; ++j) {
-#pragma unroll
-				for (u32 e = 0; e < 4; ++e) o[j][e] *= a;
+			for (u32 j = 0; j < D / 16; ++j) {
+				o[j][0] *= a0;
+				o[j][1] *= a1;
+				o[j][2] *= a0;
+				o[j][3] *= a1;
 			}
 		}
 		if constexpr (SCALED) {
@@ -463,7 +477,7 @@ paged_decode_kernel(const PagedDecodeParams p) {
 				v_unit = unit;
 				v_inv = __frcp_rn(unit);
 #pragma unroll
-				for (u32 j = 0; j < D / 8; ++j) {
+				for (u32 j = 0; j < D / 16; ++j) {
 #pragma unroll
 					for (u32 e = 0; e < 4; ++e) o[j][e] *= a;
 				}
@@ -472,7 +486,7 @@ paged_decode_kernel(const PagedDecodeParams p) {
 		// ---- weights and values ----
 #pragma unroll
 		for (u32 j = 0; j < SUBS; ++j) {
-			u32 a[4];
+			u32 hi[2], low[2];
 #pragma unroll
 			for (u32 h = 0; h < 2; ++h) {
 				f32 e0 = ex2_approx(arg[2 * j + h][0]), e1 = ex2_approx(arg[2 * j + h][1]);
@@ -481,10 +495,10 @@ paged_decode_kernel(const PagedDecodeParams p) {
 					e0 *= vs[2 * j + h][0] * v_inv;
 					e1 *= vs[2 * j + h][1] * v_inv;
 				}
-				a[2 * h] = f32x2_to_f16x2(e0, e1);
+				hi[h] = f32x2_to_f16x2(e0, e1);
 				f32 h0, h1;
-				f16x2_values(a[2 * h], h0, h1);
-				a[2 * h + 1] = f32x2_to_f16x2(e0 - h0, e1 - h1);
+				f16x2_values(hi[h], h0, h1);
+				low[h] = f32x2_to_f16x2(e0 - h0, e1 - h1);
 			}
 			u32 const v0 = src + (j * 16 + t * 2) * RB + D + g * (D / 8);
 			u32 va[VW], vb[VW], vc[VW], vd[VW];
@@ -494,10 +508,14 @@ paged_decode_kernel(const PagedDecodeParams p) {
 			ld_shared_words(v0 + 9 * RB, vd);
 #pragma unroll
 			for (u32 w = 0; w < VW; ++w) {
-				mma_f16(o[4 * w], a, codes_to_f16x2<0>(va[w], vb[w]), codes_to_f16x2<0>(vc[w], vd[w]));
-				mma_f16(o[4 * w + 1], a, codes_to_f16x2<1>(va[w], vb[w]), codes_to_f16x2<1>(vc[w], vd[w]));
-				mma_f16(o[4 * w + 2], a, codes_to_f16x2<2>(va[w], vb[w]), codes_to_f16x2<2>(vc[w], vd[w]));
-				mma_f16(o[4 * w + 3], a, codes_to_f16x2<3>(va[w], vb[w]), codes_to_f16x2<3>(vc[w], vd[w]));
+				u32 const x[4] = {codes_to_f16x2<0>(va[w], vb[w]), codes_to_f16x2<1>(va[w], vb[w]), codes_to_f16x2<0>(vc[w], vd[w]),
+								  codes_to_f16x2<1>(vc[w], vd[w])};
+				u32 const y[4] = {codes_to_f16x2<2>(va[w], vb[w]), codes_to_f16x2<3>(va[w], vb[w]), codes_to_f16x2<2>(vc[w], vd[w]),
+								  codes_to_f16x2<3>(vc[w], vd[w])};
+				mma_f16(o[2 * w], x, hi[0], hi[1]);
+				mma_f16(o[2 * w + 1], y, hi[0], hi[1]);
+				mma_f16(o[2 * w], x, low[0], low[1]);
+				mma_f16(o[2 * w + 1], y, low[0], low[1]);
 			}
 		}
 	}
@@ -508,22 +526,22 @@ paged_decode_kernel(const PagedDecodeParams p) {
 	// ---- merge the warps: [warp][row][D] in the ring's place ----
 	__syncthreads();
 	f32 *parts = reinterpret_cast<f32 *>(smem);
-	if (g < rows) {
-		f32 const unit = SCALED ? v_unit : 0.125f;
-		// a lane's columns of tile j are dims (2 t) D / 8 + j and (2 t + 1) D / 8 + j
-		f32 *dst = parts + (warp * ROWS + g) * D + 2 * t * (D / 8);
+	f32 const unit = SCALED ? v_unit : 0.125f;
 #pragma unroll
-		for (u32 j = 0; j < D / 8; j += 4) {
-			*reinterpret_cast<float4 *>(dst + j) = make_float4((o[j][0] + o[j][2]) * unit, (o[j + 1][0] + o[j + 1][2]) * unit,
-															   (o[j + 2][0] + o[j + 2][2]) * unit, (o[j + 3][0] + o[j + 3][2]) * unit);
-			*reinterpret_cast<float4 *>(dst + D / 8 + j) = make_float4((o[j][1] + o[j][3]) * unit, (o[j + 1][1] + o[j + 1][3]) * unit,
-																	   (o[j + 2][1] + o[j + 2][3]) * unit, (o[j + 3][1] + o[j + 3][3]) * unit);
+	for (u32 e = 0; e < 2; ++e) {
+		if (2 * t + e < rows) {
+			f32 *dst = parts + (warp * ROWS + 2 * t + e) * D + g * (D / 8);
+#pragma unroll
+			for (u32 j = 0; j < D / 16; j += 2) {
+				*reinterpret_cast<float4 *>(dst + 2 * j) =
+					make_float4(o[j][e] * unit, o[j][e + 2] * unit, o[j + 1][e] * unit, o[j + 1][e + 2] * unit);
+			}
 		}
-		if (t == 0) {
-			sh_m[warp][g] = -neg_m;   // m - SHIFT
-			sh_s[warp][g] = sum;
-			if (warp == 0) sh_sink[g] = sink - SHIFT;
-		}
+	}
+	if (t == 0) {
+		sh_m[warp][g] = -neg_m;   // m - SHIFT
+		sh_s[warp][g] = sum;
+		if (warp == 0) sh_sink[g] = sink - SHIFT;
 	}
 	__syncthreads();
 	if (splits > 1) cluster_wait();   // the first CTA runs (asked for at entry): its shared memory can be written
