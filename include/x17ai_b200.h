@@ -356,6 +356,10 @@ typedef struct x17ai_PagedConfig {
 
 x17ai_DiagnosticBuffer *x17ai_b200_paged_check_config(x17ai_PagedConfig const *cfg);
 
+/* Bytes of scratch memory that a decode call of this shape on the stream's device needs. */
+x17ai_DiagnosticBuffer *x17ai_b200_paged_scratch_bytes(
+	x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, size_t *bytes);
+
 /*
  * Puts new tokens into the cache, their keys and queries rotated by position on the way.
  *   q [tokens][q_stride] int8 (or NULL, then q_out too), head h at columns h*D; kv [tokens][kv_stride] int8, key head h at
@@ -390,21 +394,23 @@ x17ai_DiagnosticBuffer *x17ai_b200_paged_append_scaled(
  *   q, out: row b * n_tokens + i, strides q_stride and o_stride; page_table [batch][max_pages]; kv_lens int32 [batch] (clamped to
  *   0 .. max_pages * page_size); out FixedI8 (X17AI_DTYPE_INT8) or bf16 (X17AI_DTYPE_BF16, value = code / 8);
  *   l [batch * n_tokens][n_heads] or NULL: log2(255 * sum) + max, as the other int8 kernels write it.
- * Scores are exact integer products, probabilities keep 22 bits, sums are f32. n_splits: CTAs that share a sequence's keys
- * (1 to 16; 0 = chosen); their parts meet in the shared memory of a cluster, no scratch memory is used.
+ * Scores are exact integer products, probabilities keep 22 bits, sums are f32. The work is dealt out evenly whatever the lengths
+ * are, and the parts of a sequence meet in scratch memory: with scratch NULL it is taken from and given back to a pool of the
+ * library in stream order (in a captured graph it belongs to the graph); otherwise x17ai_b200_paged_scratch_bytes says how many
+ * bytes it must have (16-byte aligned), nothing is allocated, and calls that may run at the same time need one each.
  */
 x17ai_DiagnosticBuffer *x17ai_b200_paged_decode(
 	x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, int8_t const *q,
 	int8_t const *pages, size_t n_pages, int32_t const *page_table, size_t max_pages, int32_t const *kv_lens,
 	int8_t const *sink_k, int8_t const *sink_v, float const *attn_temperature, void *out, int32_t out_dtype, float *l,
-	size_t window_size, size_t n_splits);
+	size_t window_size, void *scratch, size_t scratch_bytes);
 
 /* The same over a scaled cache, with q_scale [batch * n_tokens][n_heads] and bf16 output; sinks are FixedI8 as before. */
 x17ai_DiagnosticBuffer *x17ai_b200_paged_decode_scaled(
 	x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, int8_t const *q,
 	float const *q_scale, int8_t const *pages, float const *page_scales, size_t n_pages, int32_t const *page_table,
 	size_t max_pages, int32_t const *kv_lens, int8_t const *sink_k, int8_t const *sink_v, float const *attn_temperature,
-	uint16_t *out_bf16, float *l, size_t window_size, size_t n_splits);
+	uint16_t *out_bf16, float *l, size_t window_size, void *scratch, size_t scratch_bytes);
 
 /* Epilogues of the GEMM (src/device/cuda/gemm.rs: ScaleEpilogue :60-110, RMSNormEpilogue
  * :112-166, ResidualEpilogue :168-212, GeGluEpilogue :214-255) */

@@ -203,16 +203,17 @@ def _cache(rng, table, n_pages, Hk, page, D, scaled, ends):
     return pages, scales, seqs
 
 
-def _decode_bounds(n, top, mean, v, v_scale):
+def _decode_bounds(n, top, mean, v, v_scale, fixed):
     """Absolute bounds of (value, l). A score carries eight roundings of 2^-24 (temperature, scales, products), a probability
     16 steps of 2^-24 more (exponential, 22 bits kept), a sum over n keys in any order at most n / 4 + 64 in a chain of four
     partial sums or more; numerator and denominator each have them. A weight's low part is rounded to f16, whose smallest step is
     2^-24: half of it, in units of 2^(m - 8) for a score m that is in the total, is at most 2^-33 of the total, and it multiplies
-    |code| times a unit no larger than twice the largest v_scale: with a weight of 2^-60 the value is gone."""
+    |code| times a unit no larger than twice the largest v_scale: with a weight of 2^-60 the value is gone. For bf16 output a
+    weight has no low part: half a step of f16, 2^-11 of the weight."""
     rel = (8 * top * np.log(2) + 16 + n / 4 + 64) * 2.0 ** -24
     heads = len(mean)
     far = 2.0 ** -32 * (v_scale.max(initial=0) * np.abs(v.astype(np.float64)).sum(0)).repeat(heads // v.shape[1], axis=0)
-    return 2 * rel * mean + far, rel / np.log(2) + 8 * 2.0 ** -24 * (top + 8 + np.log2(n + 1))
+    return (2 * rel + (0 if fixed else 2.0 ** -11)) * mean + far, rel / np.log(2) + 8 * 2.0 ** -24 * (top + 8 + np.log2(n + 1))
 
 
 def _check_decode(got, got_l, want, want_l, bound, bound_l, fixed):
@@ -224,7 +225,7 @@ def _check_decode(got, got_l, want, want_l, bound, bound_l, fixed):
         assert (np.abs(got_l - want_l) <= bound_l).all(), (np.abs(got_l - want_l) / bound_l).max()
 
 
-def _run_decode(stream, H, Hk, D, page, lens, new, window, scaled, fixed, splits, extra=0, seed=0, with_l=True, cap=None):
+def _run_decode(stream, H, Hk, D, page, lens, new, window, scaled, fixed, own_scratch=False, extra=0, seed=0, with_l=True, cap=None):
     rng = np.random.default_rng([seed, H, D, page, new, len(lens)])
     ends = [n + new - 1 for n in lens]
     table, n_pages = _table(rng, page, [max(e, cap or 0) for e in ends])
@@ -239,11 +240,12 @@ def _run_decode(stream, H, Hk, D, page, lens, new, window, scaled, fixed, splits
     l = torch.full((B * new, H), -7.0, device="cuda") if with_l else None
     t = [_gpu(a) for a in (q, pages, table, np.array(lens, dtype=np.int32), sk, sv, temp)]
     t_qs, t_s = _gpu(q_scale), _gpu(scales)
+    scratch = kern.scratch(stream, B, new).fill_(255) if own_scratch else None   # (what it holds is of no account)
     torch.cuda.synchronize()
     if scaled:
-        kern.decode_scaled(stream, t[0], t_qs, t[1], t_s, *t[2:], out, l, window, splits)
+        kern.decode_scaled(stream, t[0], t_qs, t[1], t_s, *t[2:], out, l, window, scratch)
     else:
-        kern.decode(stream, *t, out, l, window, splits)
+        kern.decode(stream, *t, out, l, window, scratch)
     stream.synchronize()
     got, got_l = out.float().cpu().numpy(), l.cpu().numpy() if with_l else None
     assert (got[:, H * D:] == 55).all()
@@ -253,50 +255,76 @@ def _run_decode(stream, H, Hk, D, page, lens, new, window, scaled, fixed, splits
             row, n = b * new + i, lens[b] + i
             want, want_l, mean, top = o_paged.attend(q[row, :H * D].reshape(H, D), q_scale[row], k[:n], ks[:n], v[:n], vs[:n], sk, sv, temp,
                                                      window)
-            bound, bound_l = _decode_bounds(n, top[:, None], mean, v[:n], vs[:n])
+            bound, bound_l = _decode_bounds(n, top[:, None], mean, v[:n], vs[:n], fixed)
             _check_decode(got[row, :H * D].reshape(H, D), None if got_l is None else got_l[row], want, want_l, bound, bound_l[:, 0], fixed)
 
 
 DECODES = [
-    # H, Hk, D, page, lens, new, window, splits
-    (1, 1, 128, 16, [1], 1, 0, 0),
-    (4, 4, 128, 16, [0, 1, 15, 16, 17, 300], 1, 0, 1),
-    (4, 4, 64, 64, [0, 1, 31, 32, 33, 500], 1, 0, 2),
-    (4, 4, 32, 32, [0, 1, 63, 64, 65, 700], 1, 0, 3),
-    (8, 1, 128, 32, [1000, 3], 1, 0, 8),
-    (6, 2, 64, 128, [129, 1], 1, 0, 0),
-    (20, 4, 128, 64, [777], 1, 0, 16),
-    (16, 1, 64, 16, [90, 2000], 1, 0, 5),
-    (17, 1, 32, 16, [45], 1, 0, 0),
-    (9, 3, 128, 1024, [2050, 1023], 1, 0, 0),
-    (4, 2, 128, 16, [0, 5, 16, 17, 400], 1, 16, 1),
-    (4, 2, 64, 32, [39, 40, 512, 600], 1, 48, 4),
-    (4, 4, 32, 64, [1000], 1, 512, 0),
-    (2, 2, 128, 16, [0, 1, 14, 200], 2, 0, 0),
-    (3, 3, 64, 32, [0, 30, 300], 5, 32, 2),
-    (16, 2, 128, 64, [0, 60, 127], 7, 0, 0),
-    (7, 7, 32, 16, [15, 16], 9, 0, 1),
-    (4, 4, 64, 16, [100], 64, 64, 0),
+    # H, Hk, D, page, lens, new, window
+    (1, 1, 128, 16, [1], 1, 0),
+    (4, 4, 128, 16, [0, 1, 15, 16, 17, 300], 1, 0),
+    (4, 4, 64, 64, [0, 1, 31, 32, 33, 500], 1, 0),
+    (4, 4, 32, 32, [0, 1, 63, 64, 65, 700], 1, 0),
+    (8, 1, 128, 32, [1000, 3], 1, 0),
+    (6, 2, 64, 128, [129, 1], 1, 0),
+    (20, 4, 128, 64, [777], 1, 0),
+    (16, 1, 64, 16, [90, 2000], 1, 0),
+    (17, 1, 32, 16, [45], 1, 0),
+    (9, 3, 128, 1024, [2050, 1023], 1, 0),
+    (4, 2, 128, 16, [0, 5, 16, 17, 400], 1, 16),
+    (4, 2, 64, 32, [39, 40, 512, 600], 1, 48),
+    (4, 4, 32, 64, [1000], 1, 512),
+    (2, 2, 128, 16, [0, 1, 14, 200], 2, 0),
+    (3, 3, 64, 32, [0, 30, 300], 5, 32),
+    (16, 2, 128, 64, [0, 60, 127], 7, 0),
+    (7, 7, 32, 16, [15, 16], 9, 0),
+    (4, 4, 64, 16, [100], 64, 64),
 ]
 
 
-@pytest.mark.parametrize("H,Hk,D,page,lens,new,window,splits", DECODES)
+@pytest.mark.parametrize("H,Hk,D,page,lens,new,window", DECODES)
 @pytest.mark.parametrize("kind", ["bf16", "fixed", "scaled"])
-def test_decode(stream, kind, H, Hk, D, page, lens, new, window, splits):
-    _run_decode(stream, H, Hk, D, page, lens, new, window, kind == "scaled", kind == "fixed", splits)
+def test_decode(stream, kind, H, Hk, D, page, lens, new, window):
+    _run_decode(stream, H, Hk, D, page, lens, new, window, kind == "scaled", kind == "fixed")
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fixed", "scaled"])
-@pytest.mark.parametrize("splits", [0, 1, 4, 7, 16])
-def test_decode_long(stream, kind, splits):
-    """Lengths where every CTA of a cluster takes many steps, wider rows than the heads need, no L."""
-    _run_decode(stream, 8, 2, 128, 64, [5000, 9001], 1, 0, kind == "scaled", kind == "fixed", splits, extra=16, with_l=False)
+@pytest.mark.parametrize("own_scratch", [False, True])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_decode_long(stream, kind, D, own_scratch):
+    """Sequences that many warps share, wider rows than the heads need, no L."""
+    _run_decode(stream, 8, 2, D, 64, [5000, 9001], 1, 0, kind == "scaled", kind == "fixed", own_scratch, extra=16, with_l=False)
 
 
-@pytest.mark.parametrize("splits", [1, 8])
-def test_decode_with_room_behind_the_lengths(stream, splits):
+@pytest.mark.parametrize("kind", ["bf16", "fixed", "scaled"])
+def test_decode_many_sequences(stream, kind):
+    """More (sequence, key head) pairs than warps: a warp goes through several, parts of the first and the last of them; more
+    than 32 sequences, some of them empty."""
+    _run_decode(stream, 16, 16, 64, 16, [(37 * i) % 301 for i in range(150)], 1, 0, kind == "scaled", kind == "fixed")
+    _run_decode(stream, 24, 8, 32, 32, [(91 * i) % 777 for i in range(70)], 3, 64, kind == "scaled", kind == "fixed", seed=1)
+
+
+def test_decode_with_room_behind_the_lengths(stream):
     """A page table with room for far more keys than the sequences have."""
-    _run_decode(stream, 4, 1, 64, 16, [3, 40], 1, 0, False, False, splits, cap=4000)
+    _run_decode(stream, 4, 1, 64, 16, [3, 40], 1, 0, False, False, cap=4000)
+
+
+def test_scratch_that_is_too_small(stream):
+    from x17ai_b200 import X17Error
+    H, D, page = 4, 64, 16
+    kern = _kernel(H, H, D, page)
+    z = lambda dtype, *shape: torch.zeros(shape, dtype=dtype, device="cuda")
+    args = (z(torch.int8, 2, H * D), kern.pages(4), z(torch.int32, 2, 2), z(torch.int32, 2), z(torch.int8, H, D), z(torch.int8, H, D),
+            z(torch.float32, H), z(torch.bfloat16, 2, H * D))
+    scratch = kern.scratch(stream, 2)
+    torch.cuda.synchronize()
+    kern.decode(stream, *args, scratch=scratch)
+    with pytest.raises(X17Error, match="scratch must be 16-byte aligned and have"):
+        kern.decode(stream, *args, scratch=scratch[:-1])
+    with pytest.raises(X17Error, match="scratch must be 16-byte aligned and have"):
+        kern.decode(stream, *args, scratch=torch.cat((scratch, scratch))[8:])
+    with pytest.raises(X17Error, match="64 new tokens"):
+        kern.scratch(stream, 2, 65)
 
 
 def test_decode_scores_far_apart(stream):
@@ -346,8 +374,7 @@ def test_decode_lengths_beyond_the_table(stream):
 
 
 @pytest.mark.parametrize("scaled", [False, True])
-@pytest.mark.parametrize("splits", [1, 4])
-def test_decode_leaves_out_bad_pages(scaled, splits):
+def test_decode_leaves_out_bad_pages(scaled):
     """A key on a page outside the pool is not attended to; the status words say so."""
     from x17ai_b200 import device
     stream = device.CudaStream(0)
@@ -365,9 +392,9 @@ def test_decode_leaves_out_bad_pages(scaled, splits):
     t_qs, t_s = _gpu(q_scale), _gpu(scales)
     torch.cuda.synchronize()
     if scaled:
-        kern.decode_scaled(stream, t[0], t_qs, t[1], t_s, *t[2:], out, l, n_splits=splits)
+        kern.decode_scaled(stream, t[0], t_qs, t[1], t_s, *t[2:], out, l)
     else:
-        kern.decode(stream, *t, out, l, n_splits=splits)
+        kern.decode(stream, *t, out, l)
     stream.synchronize()
     status = stream.read_status()
     assert status[0] >> 16 == BAD_INDEX and status[2] > 0
@@ -377,7 +404,7 @@ def test_decode_leaves_out_bad_pages(scaled, splits):
         # the temperature goes by the length, not by the keys that are left
         fix = np.float32(np.log2(n + 4) / np.log2(len(k) + 4))
         want, want_l, mean, top = o_paged.attend(q[b].reshape(H, D), q_scale[b], k, ks, v, vs, sk, sv, temp * fix, 0)
-        bound, bound_l = _decode_bounds(n, top[:, None], mean, v, vs)
+        bound, bound_l = _decode_bounds(n, top[:, None], mean, v, vs, False)
         _check_decode(out[b].float().cpu().numpy().reshape(H, D), l[b].cpu().numpy(), want, want_l, bound + 1e-6 * mean, bound_l[:, 0] + 1e-5,
                       False)
 
@@ -406,7 +433,7 @@ def test_offsets_beyond_32_bits(stream):
     assert not pages[n_pages - 2].any() and not pages[:n_pages - 3].any()
     eighth = np.full((n, Hk), 0.125)
     want, want_l, mean, top = o_paged.attend(q.reshape(H, D), np.full(H, 0.125), x[:, :, 0], eighth, x[:, :, 1], eighth, sk, sv, temp, 0)
-    bound, bound_l = _decode_bounds(n, top[:, None], mean, x[:, :, 1], eighth)
+    bound, bound_l = _decode_bounds(n, top[:, None], mean, x[:, :, 1], eighth, False)
     _check_decode(out.float().cpu().numpy().reshape(H, D), l[0].cpu().numpy(), want, want_l, bound, bound_l[:, 0], False)
 
 
@@ -475,12 +502,14 @@ def test_serving_steps(stream):
 
 def test_drafted_tokens_equal_single_steps(stream):
     """n tokens of a sequence in one call are n calls of one token at growing lengths: the same keys, to the bounds of a
-    regrouped sum (bf16 values a step apart at most)."""
+    regrouped sum: two roundings to bf16 of 2^-8, and weights that two different maxima round to f16, 2^-11 each of the largest
+    value."""
     H, Hk, D, page, new = 6, 2, 128, 32, 5
     lens = [0, 29, 300]
     rng = np.random.default_rng(21)
     table, n_pages = _table(rng, page, [n + new for n in lens])
-    pages, _, _ = _cache(rng, table, n_pages, Hk, page, D, False, [n + new for n in lens])
+    pages, _, seqs = _cache(rng, table, n_pages, Hk, page, D, False, [n + new for n in lens])
+    most = max(int(np.abs(v.astype(np.int32)).max()) for _, _, v, _ in seqs) / 8
     q, sk, sv, temp = _codes(rng, len(lens) * new, H * D), _codes(rng, H, D), _codes(rng, H, D), np.ones(H, dtype=np.float32)
     kern = _kernel(H, Hk, D, page)
     t_q, t_pages, t_table, t_sk, t_sv, t_temp = (_gpu(a) for a in (q, pages, table, sk, sv, temp))
@@ -497,7 +526,7 @@ def test_drafted_tokens_equal_single_steps(stream):
             torch.cuda.synchronize()
             kern.decode(stream, q_i, t_pages, t_table, lens_i, t_sk, t_sv, t_temp, one, one_l, window)
             stream.synchronize()
-            assert (out[i::new].float() - one.float()).abs().le(2.0 ** -7 * one.float().abs() + 1e-4).all()
+            assert (out[i::new].float() - one.float()).abs().le(2.0 ** -7 * one.float().abs() + 2.0 ** -10 * most + 1e-4).all()
             assert (l[i::new] - one_l).abs().max() <= 1e-4
 
 
@@ -528,7 +557,7 @@ def test_captured_and_replayed():
         s.synchronize()
         with device.CudaGraph(s) as g:
             step()
-        assert g.kernel_nodes == 2
+        assert g.kernel_nodes == 3
         sides.append((s, x, step, g))
     for turn in range(3):
         fresh = [(_gpu(_codes(rng, B, H * D)), _gpu(_codes(rng, B, 2 * Hk * D)), _gpu(rng.integers(0, 199, B).astype(np.int32))) for _ in sides]

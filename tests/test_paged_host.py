@@ -124,6 +124,8 @@ def _decode_args(**kw):
     (dict(out=_c(F32, 6, 512)), "out has dtype torch.float32"),
     (dict(out=_c(BF16, 3, 512)), "out has 3 rows, but should have 6"),
     (dict(l=_c(F32, 8, 6)), "l has 8 rows, but should have 6"),
+    (dict(scratch=_c(I8, 1 << 20)), "scratch must be a contiguous uint8"),
+    (dict(scratch=torch.zeros(1 << 20, dtype=torch.uint8)), "scratch must be a contiguous uint8"),
 ])
 def test_decode_refuses(lib, kw, text):
     from x17ai_b200 import X17Error, kernels as K
@@ -158,11 +160,11 @@ def _entry(lib, name, **kw):
         fn = lib.x17ai_b200_paged_append_scaled
     elif name == "decode":
         a = dict(stream=p, cfg=cfg, batch=3, n_tokens=2, q=p, pages=p, n_pages=9, table=p, max_pages=4, kv_lens=p, sink_k=p, sink_v=p, temp=p,
-                 out=p, out_dtype=0x40, l=0, window=0, n_splits=0)
+                 out=p, out_dtype=0x40, l=0, window=0, scratch=0, scratch_bytes=0)
         fn = lib.x17ai_b200_paged_decode
     else:
         a = dict(stream=p, cfg=cfg, batch=3, n_tokens=2, q=p, q_scale=p, pages=p, scales=p, n_pages=9, table=p, max_pages=4, kv_lens=p,
-                 sink_k=p, sink_v=p, temp=p, out=p, l=0, window=0, n_splits=0)
+                 sink_k=p, sink_v=p, temp=p, out=p, l=0, window=0, scratch=0, scratch_bytes=0)
         fn = lib.x17ai_b200_paged_decode_scaled
     assert set(kw) <= set(a)
     return _lib.take_diag(fn(*{**a, **kw}.values()))
@@ -189,7 +191,6 @@ def _entry(lib, name, **kw):
     ("decode", dict(n_tokens=0), "zero size"),
     ("decode", dict(n_tokens=65), "64 new tokens"),
     ("decode", dict(batch=65536), "at most 65535"),
-    ("decode", dict(n_splits=17), "at most 16"),
     ("decode", dict(window=24), "divisible by 16, got 24"),
     ("decode", dict(out_dtype=0x50), "bf16 or FixedI8"),
     ("decode", dict(kv_lens=0), "null tensor"),

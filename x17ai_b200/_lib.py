@@ -129,9 +129,10 @@ SIGNATURES = {
     "x17ai_b200_paged_append_scaled": (DIAG, [c_void_p, POINTER(PagedConfig), c_void_p, c_void_p, c_size_t] + [c_void_p] * 3
                                        + [c_size_t] * 2 + [c_void_p, c_size_t, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "x17ai_b200_paged_decode": (DIAG, [c_void_p, POINTER(PagedConfig), c_size_t, c_size_t, c_void_p, c_void_p, c_size_t, c_void_p,
-                                       c_size_t] + [c_void_p] * 5 + [c_int32, c_void_p, c_size_t, c_size_t]),
+                                       c_size_t] + [c_void_p] * 5 + [c_int32, c_void_p, c_size_t, c_void_p, c_size_t]),
     "x17ai_b200_paged_decode_scaled": (DIAG, [c_void_p, POINTER(PagedConfig), c_size_t, c_size_t] + [c_void_p] * 4 + [c_size_t, c_void_p,
-                                              c_size_t] + [c_void_p] * 6 + [c_size_t, c_size_t]),
+                                              c_size_t] + [c_void_p] * 6 + [c_size_t, c_void_p, c_size_t]),
+    "x17ai_b200_paged_scratch_bytes": (DIAG, [c_void_p, POINTER(PagedConfig), c_size_t, c_size_t, POINTER(c_size_t)]),
     "x17ai_b200_gemm_meta": (DIAG, [POINTER(GemmConfig), POINTER(GemmMeta)]),
     "x17ai_b200_gemm_fwd": (DIAG, [c_void_p, POINTER(GemmConfig), c_void_p, c_size_t, c_void_p, c_size_t,
                                    c_void_p, c_void_p, c_void_p]),

@@ -46,6 +46,7 @@ struct ContextState {
 	uint32_t *status;  // 4 words of device memory
 	int sm_count;
 	ContextState *next;
+	std::atomic<cudaMemPool_t> pool{nullptr};   // scratch_pool()
 };
 std::atomic<ContextState *> g_contexts{nullptr};   // newest first; entries stay
 std::mutex g_contexts_mutex;                       // for adding one
@@ -146,17 +147,6 @@ cudaError_t allow_smem(Kernel<KERNEL>, StreamScope const &on, uint32_t bytes) {
 	std::atomic<uint64_t> &last = raised_in[on.device];
 	if (last.load(std::memory_order_acquire) == on.state().id) return cudaSuccess;
 	cudaError_t const e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
-	if (e == cudaSuccess) last.store(on.state().id, std::memory_order_release);
-	return e;
-}
-
-// Lets a kernel be launched in clusters of more than eight CTAs, once per kernel and context.
-template <auto KERNEL>
-cudaError_t allow_wide_clusters(Kernel<KERNEL>, StreamScope const &on) {
-	static std::atomic<uint64_t> allowed_in[MAX_DEVICES];
-	std::atomic<uint64_t> &last = allowed_in[on.device];
-	if (last.load(std::memory_order_acquire) == on.state().id) return cudaSuccess;
-	cudaError_t const e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
 	if (e == cudaSuccess) last.store(on.state().id, std::memory_order_release);
 	return e;
 }
@@ -889,6 +879,7 @@ x17ai_DiagnosticBuffer *paged_pool(char const *who, x17ai_PagedConfig const *cfg
 	pool->page_shift = 0;
 	while ((size_t(1) << pool->page_shift) < cfg->page_size) ++pool->page_shift;
 	pool->n_kv_heads = uint32_t(cfg->n_kv_heads);
+	pool->page_rows = uint32_t(cfg->n_kv_heads * cfg->page_size);
 	return nullptr;
 }
 
@@ -943,13 +934,63 @@ x17ai_DiagnosticBuffer *paged_append(char const *who, x17ai_CudaStreamHandle *st
 	return launch_result(who);
 }
 
-// CTAs that share a sequence's keys: enough to fill the chip, none with fewer than 128 keys.
-size_t paged_splits(size_t ctas, size_t keys, int sm_count) {
-	size_t const want = size_t(sm_count) * 3;
-	size_t n = ctas >= want ? 1 : (want + ctas - 1) / ctas;
-	size_t const most = keys / 128 > 0 ? keys / 128 : 1;
-	n = n > most ? most : n;
-	return n > 8 ? 8 : n;
+// Memory that calls take and give back in stream order. A pool of the library's own, which keeps what it has: the default pool
+// gives it back to the system at every synchronise. Created at the first call in a context.
+cudaError_t scratch_pool(StreamScope const &on, cudaMemPool_t *pool) {
+	ContextState &c = *on.context;
+	*pool = c.pool.load(std::memory_order_acquire);
+	if (*pool != nullptr) return cudaSuccess;
+	std::lock_guard<std::mutex> lock(g_contexts_mutex);
+	*pool = c.pool.load(std::memory_order_relaxed);
+	if (*pool != nullptr) return cudaSuccess;
+	cudaMemPoolProps props{};
+	props.allocType = cudaMemAllocationTypePinned;
+	props.location.type = cudaMemLocationTypeDevice;
+	props.location.id = on.device;
+	cudaError_t e = cudaMemPoolCreate(pool, &props);
+	if (e != cudaSuccess) return e;
+	uint64_t keep = UINT64_MAX;
+	e = cudaMemPoolSetAttribute(*pool, cudaMemPoolAttrReleaseThreshold, &keep);
+	if (e != cudaSuccess) {
+		(void)cudaMemPoolDestroy(*pool);
+		return e;
+	}
+	c.pool.store(*pool, std::memory_order_release);
+	return cudaSuccess;
+}
+
+// How a call's rows are dealt out, and what its parts need.
+struct PagedPlan {
+	uint32_t chunk_rows, chunks, tiles, ctas;
+	size_t n_x, ms_bytes, o_bytes, bytes;   // bytes: [o][ms][shared_by]
+};
+PagedPlan paged_plan(x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, int sm_count) {
+	using namespace x17::paged_cfg;
+	PagedPlan plan{};
+	// the rows of a key head in as few chunks of at most two tiles as they need, evenly
+	size_t const rows = cfg->n_heads / cfg->n_kv_heads * n_tokens;
+	size_t const most = (rows + 2 * ROWS - 1) / (2 * ROWS);
+	plan.chunk_rows = uint32_t((rows + most - 1) / most);
+	plan.chunks = uint32_t((rows + plan.chunk_rows - 1) / plan.chunk_rows);
+	plan.tiles = plan.chunk_rows > ROWS ? 2 : 1;
+	plan.n_x = cfg->n_kv_heads * plan.chunks;
+	plan.ctas = uint32_t(sm_count) * (cfg->head_dim == 128 && plan.tiles == 2 ? CTAS<128, 2> : CTAS<128, 1>);
+	static_assert(CTAS<64, 1> == CTAS<128, 1> && CTAS<64, 2> == CTAS<128, 1> && CTAS<32, 1> == CTAS<128, 1> && CTAS<32, 2> == CTAS<128, 1>);
+	size_t const slots = size_t(plan.ctas) * WARPS * 2 * plan.chunk_rows;
+	plan.ms_bytes = slots * sizeof(float4);
+	plan.o_bytes = slots * cfg->head_dim * sizeof(float);
+	plan.bytes = plan.o_bytes + plan.ms_bytes + batch * plan.n_x * sizeof(uint2);
+	return plan;
+}
+
+x17ai_DiagnosticBuffer *check_paged_decode(x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, char const *who) {
+	if (auto *d = check_paged_config(cfg, who)) return d;
+	if (batch == 0 || n_tokens == 0) return make_diag("x17ai_b200: empty decode input", who, ": decode input q has zero size");
+	if (batch > 65535 || n_tokens > 64) {
+		return make_diag("x17ai_b200: decode shape out of range", who, ": at most 65535 sequences of 64 new tokens, got ", batch, " of ",
+						 n_tokens);
+	}
+	return nullptr;
 }
 
 template <bool SCALED>
@@ -957,14 +998,8 @@ x17ai_DiagnosticBuffer *paged_decode(char const *who, x17ai_CudaStreamHandle *st
 									 size_t n_tokens, int8_t const *q, float const *q_scale, int8_t const *pages, float const *scales,
 									 size_t n_pages, int32_t const *table, size_t max_pages, int32_t const *kv_lens,
 									 int8_t const *sink_k, int8_t const *sink_v, float const *temperature, void *out, int32_t out_dtype,
-									 float *l, size_t window_size, size_t n_splits) {
-	if (auto *d = check_paged_config(cfg, who)) return d;
-	if (batch == 0 || n_tokens == 0) return make_diag("x17ai_b200: empty decode input", who, ": decode input q has zero size");
-	if (batch > 65535 || n_tokens > 64) {
-		return make_diag("x17ai_b200: decode shape out of range", who, ": at most 65535 sequences of 64 new tokens, got ", batch, " of ",
-						 n_tokens);
-	}
-	if (n_splits > 16) return make_diag("x17ai_b200: decode shape out of range", who, ": n_splits is at most 16, got ", n_splits);
+									 float *l, size_t window_size, void *scratch, size_t scratch_bytes) {
+	if (auto *d = check_paged_decode(cfg, batch, n_tokens, who)) return d;
 	if (window_size % 16 != 0) {
 		return make_diag("x17ai_b200: bad window", who, ": attention window_size must be zero or divisible by 16, got ", window_size);
 	}
@@ -997,35 +1032,74 @@ x17ai_DiagnosticBuffer *paged_decode(char const *who, x17ai_CudaStreamHandle *st
 	p.out_i8 = out_dtype == X17AI_DTYPE_INT8;
 	p.status = scope.state().status;
 	cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-	// the rows of a key head in as few CTAs of at most eight as they need, evenly
-	size_t const rows = cfg->n_heads / cfg->n_kv_heads * n_tokens;
-	p.chunks = uint32_t((rows + x17::paged_cfg::ROWS - 1) / x17::paged_cfg::ROWS);
-	p.chunk_rows = uint32_t((rows + p.chunks - 1) / p.chunks);
-	p.chunks = uint32_t((rows + p.chunk_rows - 1) / p.chunk_rows);
-	size_t const ctas = cfg->n_kv_heads * p.chunks * batch;
+	PagedPlan const plan = paged_plan(cfg, batch, n_tokens, scope.state().sm_count);
 	size_t const capacity = max_pages * cfg->page_size;
-	size_t const keys = p.window < capacity ? p.window : capacity;
-	if (n_splits == 0) n_splits = paged_splits(ctas, keys, scope.state().sm_count);
+	size_t const keys = p.window < capacity ? p.window + n_tokens + 15 : capacity;
+	if (batch * plan.n_x * (keys / x17::paged_cfg::KS + 2) >= (size_t(1) << 32)) {
+		return make_diag("x17ai_b200: decode shape out of range", who, ": sequences x key heads x keys out of range (room for ", capacity,
+						 " keys in each of ", batch, " sequences)");
+	}
+	p.chunk_rows = plan.chunk_rows;
+	p.chunks = plan.chunks;
+	bool const own = scratch == nullptr;
+	if (!own && (scratch_bytes < plan.bytes || !aligned16(scratch))) {
+		return make_diag("x17ai_b200: scratch too small", who, ": scratch must be 16-byte aligned and have ", plan.bytes, " bytes, got ",
+						 scratch_bytes);
+	}
 	cudaError_t ce = cudaSuccess;
-	auto go = [&](auto dim) {
-		constexpr uint32_t D = decltype(dim)::value;
-		using K = Kernel<&x17::paged_decode_kernel<D, SCALED>>;
+	if (own) {
+		cudaMemPool_t pool;
+		ce = scratch_pool(scope, &pool);
+		if (ce == cudaSuccess) ce = cudaMallocFromPoolAsync(&scratch, plan.bytes, pool, s);
+		if (ce != cudaSuccess) {
+			(void)cudaGetLastError();
+			return make_diag("x17ai_b200: scratch allocation failed", who, ": scratch allocation of ", plan.bytes, " bytes failed: ",
+							 cudaGetErrorString(ce));
+		}
+	}
+	char *const at = static_cast<char *>(scratch);
+	x17::PagedScratch parts{};
+	parts.o = reinterpret_cast<float *>(at);
+	parts.ms = reinterpret_cast<float4 *>(at + plan.o_bytes);
+	parts.shared_by = reinterpret_cast<uint2 *>(at + plan.o_bytes + plan.ms_bytes);
+	// Rows that a CTA joins: with many parts to a row its eight warps share one row, with few each takes a row of its own.
+	size_t const parts_each = size_t(plan.ctas) * x17::paged_cfg::WARPS / (batch * plan.n_x);
+	uint32_t cta_rows = 1;
+	while (cta_rows < x17::paged_cfg::MERGE_WARPS && cta_rows < plan.chunk_rows && cta_rows * parts_each < 64) cta_rows *= 2;
+	auto go = [&](auto dim, auto tiles, auto low) {
+		constexpr uint32_t D = decltype(dim)::value, RT = decltype(tiles)::value;
+		using K = Kernel<&x17::paged_decode_kernel<D, SCALED, RT, decltype(low)::value>>;
 		constexpr uint32_t ring = x17::paged_cfg::RING_BYTES<D, SCALED>;
-		ce = allow_smem(K{}, scope, ring + x17::paged_cfg::part_bytes<D>(x17::paged_cfg::MAX_SPLITS, x17::paged_cfg::ROWS));
-		if (ce == cudaSuccess) ce = allow_wide_clusters(K{}, scope);
-		if (ce != cudaSuccess) return;
-		(void)launch(K{}, dim3(unsigned(cfg->n_kv_heads * p.chunks), unsigned(batch), unsigned(n_splits)), x17::paged_cfg::THREADS,
-					 ring + x17::paged_cfg::part_bytes<D>(uint32_t(n_splits), p.chunk_rows), s,
-					 n_splits > 1 ? dim3(1, 1, unsigned(n_splits)) : dim3(NO_CLUSTER), p);
+		ce = allow_smem(K{}, scope, ring);
+		if (ce == cudaSuccess) ce = launch(K{}, dim3(plan.ctas), x17::paged_cfg::THREADS, ring, s, dim3(NO_CLUSTER), p, parts);
+		if (ce == cudaSuccess) {
+			ce = launch(Kernel<&x17::paged_merge_kernel<D>>{}, dim3(unsigned(batch * plan.n_x), (plan.chunk_rows + cta_rows - 1) / cta_rows),
+						x17::paged_cfg::MERGE_WARPS * 32, 0, s, dim3(NO_CLUSTER), p, parts, cta_rows);
+		}
 	};
-	if (cfg->head_dim == 128) go(std::integral_constant<uint32_t, 128>{});
-	else if (cfg->head_dim == 64) go(std::integral_constant<uint32_t, 64>{});
-	else go(std::integral_constant<uint32_t, 32>{});
+	auto go_tiles = [&](auto dim, auto tiles) {
+		if constexpr (!SCALED) {
+			if (p.out_i8) return go(dim, tiles, std::true_type{});
+		}
+		go(dim, tiles, std::false_type{});
+	};
+	auto go_dim = [&](auto dim) {
+		if (plan.tiles == 2) go_tiles(dim, std::integral_constant<uint32_t, 2>{});
+		else go_tiles(dim, std::integral_constant<uint32_t, 1>{});
+	};
+	if (cfg->head_dim == 128) go_dim(std::integral_constant<uint32_t, 128>{});
+	else if (cfg->head_dim == 64) go_dim(std::integral_constant<uint32_t, 64>{});
+	else go_dim(std::integral_constant<uint32_t, 32>{});
+	x17ai_DiagnosticBuffer *res = nullptr;
 	if (ce != cudaSuccess) {
 		(void)cudaGetLastError();
-		return make_diag("x17ai_b200: kernel attributes", who, ": kernel attributes: ", cudaGetErrorString(ce));
+		res = make_diag("x17ai_b200: kernel launch failed", who, ": kernel launch failed: ", cudaGetErrorString(ce));
+	} else {
+		res = launch_result(who);
+		if (res == nullptr) g_launches.fetch_add(1, std::memory_order_relaxed);   // (two kernels)
 	}
-	return launch_result(who);
+	if (own) (void)cudaFreeAsync(scratch, s);
+	return res;
 }
 
 // ---- decode without allocation -------------------------------------------------------------------
@@ -1504,6 +1578,17 @@ x17ai_DiagnosticBuffer *x17ai_b200_paged_check_config(x17ai_PagedConfig const *c
 	return check_paged_config(cfg, "x17ai_b200_paged_check_config()");
 }
 
+x17ai_DiagnosticBuffer *x17ai_b200_paged_scratch_bytes(
+	x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, size_t *bytes) {
+	char const *who = "x17ai_b200_paged_scratch_bytes()";
+	if (auto *d = check_paged_decode(cfg, batch, n_tokens, who)) return d;
+	if (bytes == nullptr) return make_diag("x17ai_b200: null argument", who, ": null argument");
+	StreamScope scope(stream, who);
+	if (scope.diag) return scope.diag;
+	*bytes = paged_plan(cfg, batch, n_tokens, scope.state().sm_count).bytes;
+	return nullptr;
+}
+
 x17ai_DiagnosticBuffer *x17ai_b200_paged_append(
 	x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, int8_t const *q, int8_t const *kv, size_t tokens,
 	int32_t const *seqs, int32_t const *positions, int32_t const *page_table, size_t n_seqs, size_t max_pages,
@@ -1524,19 +1609,20 @@ x17ai_DiagnosticBuffer *x17ai_b200_paged_decode(
 	x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, int8_t const *q,
 	int8_t const *pages, size_t n_pages, int32_t const *page_table, size_t max_pages, int32_t const *kv_lens,
 	int8_t const *sink_k, int8_t const *sink_v, float const *attn_temperature, void *out, int32_t out_dtype, float *l,
-	size_t window_size, size_t n_splits) {
+	size_t window_size, void *scratch, size_t scratch_bytes) {
 	return paged_decode<false>("x17ai_b200_paged_decode()", stream, cfg, batch, n_tokens, q, nullptr, pages, nullptr, n_pages, page_table,
-							   max_pages, kv_lens, sink_k, sink_v, attn_temperature, out, out_dtype, l, window_size, n_splits);
+							   max_pages, kv_lens, sink_k, sink_v, attn_temperature, out, out_dtype, l, window_size, scratch,
+							   scratch_bytes);
 }
 
 x17ai_DiagnosticBuffer *x17ai_b200_paged_decode_scaled(
 	x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, int8_t const *q,
 	float const *q_scale, int8_t const *pages, float const *page_scales, size_t n_pages, int32_t const *page_table,
 	size_t max_pages, int32_t const *kv_lens, int8_t const *sink_k, int8_t const *sink_v, float const *attn_temperature,
-	uint16_t *out_bf16, float *l, size_t window_size, size_t n_splits) {
+	uint16_t *out_bf16, float *l, size_t window_size, void *scratch, size_t scratch_bytes) {
 	return paged_decode<true>("x17ai_b200_paged_decode_scaled()", stream, cfg, batch, n_tokens, q, q_scale, pages, page_scales, n_pages,
 							  page_table, max_pages, kv_lens, sink_k, sink_v, attn_temperature, out_bf16, X17AI_DTYPE_BF16, l, window_size,
-							  n_splits);
+							  scratch, scratch_bytes);
 }
 
 x17ai_DiagnosticBuffer *x17ai_b200_gemm_meta(x17ai_GemmConfig const *cfg, x17ai_GemmMeta *meta) {

@@ -24,8 +24,9 @@ struct PagedPool {
 	u32 n_pages, n_seqs, max_pages;
 	u32 page_shift;         // log2(page_size)
 	u32 n_kv_heads;
+	u32 page_rows;          // rows (head, slot) of a page
 	// row of (page, head, slot)
-	X17_DEV u64 row(u32 page, u32 head, u32 slot) const { return ((u64(page) * n_kv_heads + head) << page_shift) + slot; }
+	X17_DEV u64 row(u32 page, u32 head, u32 slot) const { return u64(page) * page_rows + ((head << page_shift) + slot); }
 };
 
 struct PagedAppendParams {
@@ -148,49 +149,54 @@ paged_append_kernel(const PagedAppendParams p) {
 
 // ---- decode ------------------------------------------------------------------------------------
 //
-// A pass over a cache is bound by HBM: the kernel's job is to keep enough bytes in flight and to stay out of their way. One
-// CTA works on the rows (query heads of a group, times new tokens; eight at most) that share a key head, so a key is read
-// once for all of them; up to 16 CTAs (a cluster) share a sequence's keys, four warps a CTA's. A warp takes 16 or 32 keys a
-// step (4 KB) out of a ring of its own in shared memory that it fills itself, three steps ahead, with cp.async: no barrier
-// among warps until the end. A page of a head is one run of memory and a step's page is known long before (32 entries of the page table
-// sit in a warp's lanes), so pages cost no more than a contiguous cache.
+// A pass over a cache is bound by HBM: the kernel's job is to keep enough bytes in flight on every SM, whatever the sequences'
+// lengths, and to stay out of their way. The rows (query heads of a group, times new tokens) that share a key head are taken
+// eight at a time, so a key is read once for all of them. The work of a call is the list of all steps (32 keys) of all (sequence,
+// key head, eight rows), and every warp of a grid that fills the chip once takes an equal run of it: one sequence of 131072
+// keys and 128 ragged ones keep the chip equally busy, and no length has to be known on the host. A warp works alone: it fills a
+// ring of two steps in shared memory (cp.async; page table entries are fetched a step before that), and where its run covers a
+// whole (sequence, head, rows) it writes the output itself; the parts of those that several warps share go through scratch
+// memory and a second kernel.
+// A page of a head is one run of memory, so pages cost no more than a contiguous cache.
 //
 // Scores: mma m16n8k32 (s8 x s8 -> s32, exact), rows as its M, keys as its N; a lane's bytes of a key row are consecutive, the
 // query's are permuted the same way. Values: mma m16n8k16 (f16 x f16 -> f32) with V transposed as its first operand (dims as M)
 // and the weights as the second (rows as N), which is how the scores' fragments lie; accumulators are a lane's 16 dims of two rows.
-// Weights keep 22 bits: e = hi + lo in f16, two products into the same sums. V's codes are exact in f16 (integer added to 1024 as
-// bits). Weights are 2^(x - m + 8) against a maximum m that moves only when a score passes it by 6: between 2^-38 and 2^14 of
+// V's codes are exact in f16 (integer added to 1024 as bits). Weights are rounded to f16's 11 bits for a bf16 output, which
+// has 8: the roundings of many keys average out, a single key's is 2^-12. A FixedI8 output keeps 22 bits (e = hi + lo in f16, two
+// products into the same sums), so that its codes are those of the exact value but for ties. Weights are 2^(x - m + 8) against a maximum m that moves only when a score passes it by 6: between 2^-38 and 2^14 of
 // m's nothing is lost to f16's range. m starts at the sink's score, so no key and no row leaves it undefined.
 
 namespace paged_cfg {
+#ifndef PG_MIN
+#define PG_MIN 1
+#endif
 constexpr u32 WARPS = 4, THREADS = WARPS * 32;
-#ifndef PG_STAGES
-#define PG_STAGES 4
-#endif
-#ifndef PG_CTAS
-#define PG_CTAS 3
-#endif
-#ifndef PG_KEYS
-#define PG_KEYS 16
-#endif
-constexpr u32 STAGES = PG_STAGES;
-constexpr u32 ROWS = 8;          // rows of a CTA
-constexpr u32 MAX_SPLITS = 16;   // CTAs of a cluster
+constexpr u32 KS = 32;           // keys of a step: two runs of 16, each in one page
+constexpr u32 STAGES = 2;
+constexpr u32 ROWS = 8;          // of a tile; a warp has one or two
+constexpr u32 MIN_STEPS = PG_MIN;     // of a warp's run
 constexpr f32 SHIFT = 8.0f, ARG_MAX = 14.0f;   // weights are 2^(x - m + SHIFT), at most 2^ARG_MAX (f16 ends below 2^16)
-template <u32 D>
-constexpr u32 KEYS = D == 128 ? PG_KEYS : 32;       // of a step
+constexpr u32 MERGE_WARPS = 8;   // of a CTA that joins parts
+// CTAs on an SM: 12 warps with a step in work and a step on its way each, 210 KB of rings. With two tiles at width 128 the sums
+// alone are 64 registers: eight warps.
+template <u32 D, u32 RT>
+constexpr u32 CTAS = D == 128 && RT == 2 ? 2 : 3;
 template <u32 D>
 constexpr u32 ROW_BYTES = 2 * D + 16;          // of a key in the ring: rows 16 bytes off each other's banks
 template <u32 D, bool SCALED>
-constexpr u32 STAGE_BYTES = KEYS<D> * (ROW_BYTES<D> + (SCALED ? 8 : 0));
+constexpr u32 STAGE_BYTES = KS * (ROW_BYTES<D> + (SCALED ? 8 : 0));
 template <u32 D, bool SCALED>
 constexpr u32 RING_BYTES = WARPS * STAGES * STAGE_BYTES<D, SCALED>;
-// the parts of a cluster's CTAs, in the first one: [splits][rows][D + 2] f32
-template <u32 D>
-constexpr u32 part_bytes(u32 splits, u32 rows) {
-	return splits > 1 ? splits * rows * (D + 2) * 4 : 0;
-}
 }  // namespace paged_cfg
+
+// Parts of (sequence, x) that several warps share. A warp has at most two: [0] of one that began in an earlier warp's
+// run, [1] of one that begins in its own and goes on behind it.
+struct PagedScratch {
+	uint2 *shared_by;   // [sequences][x]: first warp, number of warps; written on every call
+	float4 *ms;         // [warps][2][rows]: m - SHIFT, sum, the sink's score
+	f32 *o;             // [warps][2][rows][D]
+};
 
 X17_DEV void cp_async_16(u32 dst, void const *src) {
 	asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -205,12 +211,19 @@ template <u32 N>
 X17_DEV void cp_async_wait() {
 	asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-// c[0], c[1]: row lane / 4, columns 2 (lane % 4) and the next one; rows 8-15 of A are zero, their sums are not kept
-X17_DEV void mma_s8(i32 (&c)[2], u32 a0, u32 a2, u32 b0, u32 b1) {
-	i32 unused2, unused3;
-	asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%9, %10, %5, %5};"
-		: "=r"(c[0]), "=r"(c[1]), "=r"(unused2), "=r"(unused3)
-		: "r"(a0), "r"(0), "r"(a2), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]));
+// c[0], c[1]: row lane / 4, columns 2 (lane % 4) and the next one; c[2], c[3]: row lane / 4 + 8. The first product of a sum has
+// no sum before it.
+template <bool FIRST>
+X17_DEV void mma_s8(i32 (&c)[4], u32 const (&a)[4], u32 b0, u32 b1) {
+	if constexpr (FIRST) {
+		asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+			: "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+			: "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
+	} else {
+		asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+			: "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+			: "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+	}
 }
 X17_DEV void mma_f16(f32 (&c)[4], u32 const (&a)[4], u32 b0, u32 b1) {
 	asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -228,9 +241,9 @@ X17_DEV void f16x2_values(u32 h2, f32 &lo, f32 &hi) {
 // byte J of a and of b, signed, as f16x2: the bits 0x6400 + (code + 128) are 1024 + 128 + code
 template <u32 J>
 X17_DEV u32 codes_to_f16x2(u32 a, u32 b) {
-	u32 const t = (__byte_perm(a, b, (J + 4) << 8 | J) & 0x00FF00FFu) ^ 0x64806480u;
 	u32 r;
-	asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(t), "r"(0xE480E480u));
+	asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(r) : "r"(__byte_perm(a, b, (J + 4) << 8 | J)), "r"(0x00FF00FFu), "r"(0x64806480u));
+	asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(r), "r"(0xE480E480u));
 	return r;
 }
 // N words (1, 2, 4 or 8) from shared memory
@@ -269,325 +282,493 @@ X17_DEV void ld_global_words(i8 const *p, u32 (&w)[N]) {
 	}
 }
 
-// One output: the keys' (m, s, v), m being a maximum less SHIFT that is no smaller than the sink's, with the sink token.
-template <u32 D>
-X17_DEV void paged_finish(PagedDecodeParams const &p, u32 b, u32 kvh, u32 row0, u32 r, u32 d, f32 m, f32 s, f32 v, f32 sink) {
-	u32 const group = p.n_heads / p.pool.n_kv_heads;
-	u32 const row = row0 + r, head = kvh * group + row % group;
-	u64 const out_row = u64(b) * p.n_tokens + row / group;
-	f32 const a = ex2_approx(sink - m + paged_cfg::SHIFT);
+// What a sequence's rows see: token i has position n = length(i) and keys [first(n), n).
+struct PagedSpan {
+	u32 len, capacity, window;
+	X17_DEV PagedSpan(PagedDecodeParams const &p, i32 kv_len)
+		: len(u32(max(kv_len, 0))), capacity(p.pool.max_pages << p.pool.page_shift), window(p.window) {}
+	X17_DEV u32 length(u32 token) const { return min(len + token, capacity); }
+	X17_DEV u32 first(u32 n) const { return n - min(n, window); }
+	X17_DEV u32 base() const { return first(length(0)) & ~15u; }   // of the sequence's steps
+	// one at least: a sequence without keys has its sink
+	X17_DEV u32 steps(u32 n_tokens) const { return max(1u, (length(n_tokens - 1) - base() + paged_cfg::KS - 1) / paged_cfg::KS); }
+};
+
+// VD dims from d on of one row, from the keys' (m, s, v), m being a maximum less SHIFT, and the sink token.
+template <u32 D, u32 VD>
+X17_DEV void paged_finish(PagedDecodeParams const &p, u64 out_row, u32 head, u32 d, f32 m, f32 s, f32 (&v)[VD], f32 sink) {
+	f32 const a = ex2_approx(sink - m);
 	s += a;
-	v = __fmaf_rn(f32(p.sink_v[u64(head) * D + d]) * 0.125f, a, v);
-	v = __fdiv_rn(v, s);
+	f32 const inv = __fdiv_rn(1.0f, s);
+	i8 const *sv = p.sink_v + u64(head) * D + d;
 	u64 const at = out_row * p.o_stride + head * D + d;
-	if (p.out_i8) static_cast<i8 *>(p.out)[at] = i8(f32_to_fixedi8(v * 8.0f));
-	else static_cast<u16 *>(p.out)[at] = u16(cvt_bf16x2(v, 0.0f));
+#pragma unroll
+	for (u32 i = 0; i < VD; i += 4) {
+		u32 const w = *reinterpret_cast<u32 const *>(sv + i);
+		f32 x[4];
+#pragma unroll
+		for (u32 j = 0; j < 4; ++j) x[j] = __fmaf_rn(f32(i8(w >> (8 * j))) * 0.125f, a, v[i + j]) * inv;
+		if (p.out_i8) {
+			u32 c[4];
+#pragma unroll
+			for (u32 j = 0; j < 4; ++j) c[j] = u32(f32_to_fixedi8(x[j] * 8.0f));
+			*reinterpret_cast<u32 *>(static_cast<i8 *>(p.out) + at + i) = pack4(c[0], c[1], c[2], c[3]);
+		} else {
+			*reinterpret_cast<uint2 *>(static_cast<u16 *>(p.out) + at + i) = make_uint2(cvt_bf16x2(x[0], x[1]), cvt_bf16x2(x[2], x[3]));
+		}
+	}
 	if (d == 0 && p.l != nullptr) p.l[out_row * p.n_heads + head] = log2f(255.0f * s) + m;
 }
 
-// Grid (key head and chunk of rows, sequence, split); the splits of one (x, y) are a cluster.
+// What the scores of a row are multiplied with.
 template <u32 D, bool SCALED>
-__global__ void __launch_bounds__(paged_cfg::THREADS, PG_CTAS)
-paged_decode_kernel(const PagedDecodeParams p) {
+X17_DEV f32 paged_temperature(PagedDecodeParams const &p, u64 q_row, u32 head, u32 seen) {
+	// D^-1/2 log2(min(W', n) + 4) temp_h, and the scales that are not the key's
+	constexpr f32 ROOT = f32(D == 128 ? 0.08838834764831845 : D == 64 ? 0.125 : 0.17677669529663687);
+	f32 const t = ROOT * log2f(f32(seen + 4)) * p.temperature[head];
+	return SCALED ? t * p.q_scale[q_row * p.n_heads + head] : t * 0.015625f;
+}
+
+// One warp takes units w * per .. of the call's list, in order of sequence, x (key head, chunk of rows), step. RT: tiles of eight
+// rows that a chunk has. LOW: weights with their low parts.
+template <u32 D, bool SCALED, u32 RT, bool LOW>
+__global__ void __launch_bounds__(paged_cfg::THREADS, paged_cfg::CTAS<D, RT>)
+paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 	using namespace paged_cfg;
-	constexpr u32 KS = KEYS<D>, SUBS = KS / 16;      // a step's runs of 16 keys lie in one page each
 	constexpr u32 KW = D / 16;                       // words of a key row that a lane holds
 	constexpr u32 VW = D / 32;                       // words of a value row that a lane holds
-	constexpr u32 RB = ROW_BYTES<D>;
+	constexpr u32 VD = D / 8;                        // dims of a lane
+	constexpr u32 RB = ROW_BYTES<D>, SB = STAGE_BYTES<D, SCALED>;
 	constexpr u32 NEG_INF = 0xFF800000u;
 	extern __shared__ __align__(16) u8 smem[];
-	__shared__ f32 sh_sink[ROWS], sh_m[WARPS][ROWS], sh_s[WARPS][ROWS];
-	u32 const warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+	u32 const lane = threadIdx.x & 31;
 	u32 const g = lane >> 2, t = lane & 3;
-	u32 const splits = gridDim.z;
-
-	if (splits > 1) cluster_arrive();   // "this CTA runs"
-	pdl_wait();
+	u32 const n_warps = gridDim.x * WARPS, w = (threadIdx.x >> 5) * gridDim.x + blockIdx.x;   // a short list reaches every SM
 	u32 const group = p.n_heads / p.pool.n_kv_heads;
-	u32 const kvh = blockIdx.x / p.chunks, chunk = blockIdx.x % p.chunks, b = blockIdx.y;
-	u32 const n_rows_all = group * p.n_tokens;
-	u32 const row0 = chunk * p.chunk_rows;
-	u32 const rows = min(p.chunk_rows, n_rows_all - row0);
-	i32 const len = p.kv_lens[b];
+	u32 const n_x = p.pool.n_kv_heads * p.chunks;
+	u32 const ring = smem_u32(smem) + (threadIdx.x >> 5) * STAGES * SB;
+	pdl_launch_dependents();
+	pdl_wait();
 
-	// this lane's row: a head of the group for one of the new tokens (rows behind the last one repeat it and are not stored)
-	u32 const my_row = row0 + min(g, rows - 1);
-	u32 const tok = my_row / group, head = kvh * group + my_row % group;
-	u64 const q_row = u64(b) * p.n_tokens + tok;
-	u32 qw[KW], skw[KW];
-	ld_global_words(p.q + q_row * p.q_stride + head * D + t * (D / 4), qw);
-	ld_global_words(p.sink_k + u64(head) * D + t * (D / 4), skw);
-	f32 temp = p.temperature[head];
-	if constexpr (SCALED) temp *= p.q_scale[q_row * p.n_heads + head];
+	// ---- the warp's run of units ----
+	u32 total = 0;
+	for (u32 i = lane; i < p.pool.n_seqs; i += 32) total += PagedSpan(p, p.kv_lens[i]).steps(p.n_tokens);
+#pragma unroll
+	for (u32 mask = 16; mask > 0; mask >>= 1) total += __shfl_xor_sync(0xffffffffu, total, mask);
+	total *= n_x;   // (below 2^32: checked on the host for sequences of full length)
+	u32 const per = max((total + n_warps - 1) / n_warps, MIN_STEPS);
+	u32 const start = w * per;
+	if (w > total / per || start >= total) return;
+	u32 const n_units = min(per, total - start);
+	u32 left = n_units;
+	u32 b = 0, before = 0;
+	for (u32 target = start / n_x;; b += 32) {
+		u32 const mine = b + lane < p.pool.n_seqs ? PagedSpan(p, p.kv_lens[b + lane]).steps(p.n_tokens) : 0u;
+		u32 upto = mine;
+#pragma unroll
+		for (u32 d = 1; d < 32; d <<= 1) {
+			u32 const v = __shfl_up_sync(0xffffffffu, upto, d);
+			if (lane >= d) upto += v;
+		}
+		u32 const hit = __ballot_sync(0xffffffffu, before + upto > target);
+		if (hit != 0) {
+			u32 const at = __ffs(hit) - 1;
+			before += __shfl_sync(0xffffffffu, upto - mine, at);
+			b += at;
+			break;
+		}
+		before += __shfl_sync(0xffffffffu, upto, 31);
+	}
 
-	u32 const capacity = p.pool.max_pages << p.pool.page_shift;
-	auto length = [&](u32 tk) { return min(u32(max(len, 0)) + tk, capacity); };
-	auto first = [&](u32 n) { return n - min(n, p.window); };
-	u32 const tok_lo = row0 / group, tok_hi = (row0 + rows - 1) / group;
-	u32 const n = length(tok), lo = first(n);                       // of this lane's row
-	u32 const n_hi = length(tok_hi), lo_all = first(length(tok_lo));   // the union of the rows' keys: [lo_all, n_hi)
-	u32 const n_min = length(tok_lo), lo_max = first(n_hi);            // what every row sees: [lo_max, n_min)
-
-	// the CTA's steps of KS keys from `base` on, dealt out to its warps in turn
-	u32 const base = lo_all & ~15u;
-	u32 const n_steps = n_hi > base ? (n_hi - base + KS - 1) / KS : 0;
-	u32 const per_cta = (n_steps + splits - 1) / splits;
-	u32 const step_lo = min(blockIdx.z * per_cta, n_steps), step_hi = min(step_lo + per_cta, n_steps);
-	u32 const n_own = step_hi - step_lo > warp ? (step_hi - step_lo - warp + WARPS - 1) / WARPS : 0;
-
-	u32 const ring = smem_u32(smem) + warp * STAGES * STAGE_BYTES<D, SCALED>;
-	u32 bad = 0;                       // bit stage * SUBS + sub: that run's page is none
-	u32 page_now = 0, page_next = 0;   // page table entries of the warp's runs, one a lane
-	auto run_key = [&](u32 run) { return base + ((step_lo + warp + run / SUBS * WARPS) * SUBS + run % SUBS) * 16; };
-	auto page_entry = [&](u32 run) -> u32 {
-		u32 const key = run_key(run);
-		return run < n_own * SUBS && key < n_hi ? u32(p.pool.table[u64(b) * p.pool.max_pages + (key >> p.pool.page_shift)]) : 0u;
+	// ---- the (sequence, x) in work, and the one behind it (whose first step is fetched under the last of this one) ----
+	PagedSpan span(p, p.kv_lens[b]);
+	u32 steps = span.steps(p.n_tokens);
+	u32 x = (start - before * n_x) / steps, step = (start - before * n_x) % steps;
+	// page table entries of the 32 runs of 16 keys from `run` on, one a lane
+	auto page_entries = [&](PagedSpan const &sp, u32 seq, u32 run) -> u32 {
+		u32 const key = sp.base() + (run + lane) * 16;
+		return key < sp.length(p.n_tokens - 1) ? u32(p.pool.table[u64(seq) * p.pool.max_pages + (key >> p.pool.page_shift)]) : 0u;
 	};
-	page_next = page_entry(lane);
-	auto issue = [&](u32 i) {
-		if (i < n_own) {
-			u32 const stage = i % STAGES, dst0 = ring + stage * STAGE_BYTES<D, SCALED>;
-			if (i * SUBS % 32 == 0) {
-				page_now = page_next;
-				page_next = page_entry(i * SUBS + 32 + lane);
-			}
+	u32 bad = 0;   // bit 2 stage + run: its page is none
+	// step s of a (sequence, x) into a stage; entries: of the runs from a multiple of 32 on
+	auto issue = [&](PagedSpan const &sp, u32 seq, u32 kvh, u32 s, u32 entries, u32 stage) {
+		u32 const n_hi = sp.length(p.n_tokens - 1);
 #pragma unroll
-			for (u32 j = 0; j < SUBS; ++j) {
-				u32 const page = __shfl_sync(0xffffffffu, page_now, (i * SUBS + j) & 31);
-				u32 const key = run_key(i * SUBS + j);
-				u32 const bit = 1u << (stage * SUBS + j);
-				bool const ok = page < p.pool.n_pages;
-				bad = ok ? bad & ~bit : bad | bit;
-				if (!ok) {
-					if (lane == 0 && key < n_hi) report_status(p.status, ST_BAD_INDEX, b);
-				} else if (key < n_hi) {
-					u64 const row = p.pool.row(page, kvh, key & ((1u << p.pool.page_shift) - 1));
-					i8 const *src = p.pool.pages + row * 2 * D;
-					constexpr u32 CHUNKS = 2 * D / 16;   // of a row
+		for (u32 j = 0; j < 2; ++j) {
+			u32 const page = __shfl_sync(0xffffffffu, entries, (s * 2 + j) & 31);
+			u32 const key = sp.base() + s * KS + j * 16;
+			u32 const bit = 1u << (stage * 2 + j);
+			bad &= ~bit;
+			if (page >= p.pool.n_pages) {
+				bad |= bit;
+				if (lane == 0) report_status(p.status, ST_BAD_INDEX, seq);
+			} else if (key < n_hi) {
+				u64 const row = p.pool.row(page, kvh, key & ((1u << p.pool.page_shift) - 1));
+				i8 const *src = p.pool.pages + row * 2 * D + lane * 16;
+				u32 const dst = ring + stage * SB + j * 16 * RB;
+				constexpr u32 CHUNKS = 2 * D / 16;   // of a row
 #pragma unroll
-					for (u32 c = 0; c < CHUNKS / 2; ++c) {
-						u32 const at = c * 32 + lane;
-						cp_async_16(dst0 + (j * 16 + at / CHUNKS) * RB + at % CHUNKS * 16, src + at * 16);
-					}
-					if constexpr (SCALED) {
-						if (lane < 16) cp_async_8(dst0 + KS * RB + (j * 16 + lane) * 8, p.pool.scales + (row + lane) * 2);
-					}
+				for (u32 c = 0; c < CHUNKS / 2; ++c) {
+					u32 const at = c * 32 + lane;
+					cp_async_16(dst + at / CHUNKS * RB + at % CHUNKS * 16, src + c * 512);
+				}
+				if constexpr (SCALED) {
+					if (lane < 16) cp_async_8(ring + stage * SB + KS * RB + (j * 16 + lane) * 8, p.pool.scales + (row + lane) * 2);
 				}
 			}
 		}
 		cp_async_commit();
 	};
-#pragma unroll
-	for (u32 i = 0; i + 1 < STAGES; ++i) issue(i);
+	u32 entries = page_entries(span, b, step * 2 & ~31u);
+	issue(span, b, x / p.chunks, step, entries, 0);
+	u32 entries_ahead = page_entries(span, b, (step * 2 & ~31u) + 32);
+	u32 stage = 0;
 
-	// temperature D^-1/2 log2(min(W', n) + 4) temp_h, times the scales that are not the key's
-	constexpr f32 ROOT = f32(D == 128 ? 0.08838834764831845 : D == 64 ? 0.125 : 0.17677669529663687);
-	temp *= ROOT * log2f(f32(n - lo + 4)) * (SCALED ? 1.0f : 0.015625f);
-	i32 dot = 0;
-#pragma unroll
-	for (u32 i = 0; i < KW; ++i) dot = __dp4a(i32(qw[i]), i32(skw[i]), dot);
-	dot += __shfl_xor_sync(0xffffffffu, dot, 1);
-	dot += __shfl_xor_sync(0xffffffffu, dot, 2);
-	f32 const sink = f32(dot) * (SCALED ? temp * 0.125f : temp);
-	f32 neg_m = SHIFT - sink, sum = 0.0f;
-	f32 v_unit = 0.0f, v_inv = 0.0f;   // SCALED: weights carry v_scale / v_unit, a power of two no smaller than any seen
 	// tile j: dims g D / 8 + 2 j ([0], [1]) and + 2 j + 1 ([2], [3]) of rows 2 t ([0], [2]) and 2 t + 1 ([1], [3])
-	f32 o[D / 16][4];
+	f32 o[D / 16][RT][4];
+#pragma unroll 1
+	for (;;) {
+		u32 const kvh = x / p.chunks, row0 = (x - kvh * p.chunks) * p.chunk_rows;
+		u32 const rows = min(p.chunk_rows, group * p.n_tokens - row0);
+		u32 const n_here = min(steps - step, left);
+		left -= n_here;
+		// the next one
+		bool const b_ends = x + 1 == n_x;
+		u32 const next_b = b_ends ? b + 1 : b, next_x = b_ends ? 0u : x + 1;
+		PagedSpan next_span = span;
+		u32 entries_next = 0;
+		if (left != 0) {
+			if (b_ends) next_span = PagedSpan(p, p.kv_lens[next_b]);
+			entries_next = page_entries(next_span, next_b, 0);
+		}
+
+		// ---- this lane's rows: heads of the group for one of the new tokens (rows behind the last one repeat it and are not stored) ----
+		u32 qa[KW / 2][4];   // as the products' first operand
+		u32 n[RT], lo[RT];
+		f32 temp[RT], sink[RT], neg_m[RT], sum[RT];
 #pragma unroll
-	for (u32 i = 0; i < D / 16; ++i) {
+		for (u32 r = 0; r < RT; ++r) {
+			u32 const my_row = row0 + min(g + r * ROWS, rows - 1);
+			u32 const tok = my_row / group, head = kvh * group + my_row - tok * group;
+			u64 const q_row = u64(b) * p.n_tokens + tok;
+			u32 qw[KW], skw[KW];
+			ld_global_words(p.q + q_row * p.q_stride + head * D + t * (D / 4), qw);
+			ld_global_words(p.sink_k + u64(head) * D + t * (D / 4), skw);
+			n[r] = span.length(tok);
+			lo[r] = span.first(n[r]);
+			temp[r] = paged_temperature<D, SCALED>(p, q_row, head, n[r] - lo[r]);
+			i32 dot = 0;
 #pragma unroll
-		for (u32 j = 0; j < 4; ++j) o[i][j] = 0.0f;
-	}
+			for (u32 k = 0; k < KW; ++k) {
+				dot = __dp4a(i32(qw[k]), i32(skw[k]), dot);
+				qa[k / 2][k % 2 * 2 + r] = qw[k];
+				if (RT == 1) qa[k / 2][k % 2 * 2 + 1] = 0;
+			}
+			dot += __shfl_xor_sync(0xffffffffu, dot, 1);
+			dot += __shfl_xor_sync(0xffffffffu, dot, 2);
+			sink[r] = f32(dot) * (SCALED ? temp[r] * 0.125f : temp[r]);
+			neg_m[r] = SHIFT - sink[r];
+			sum[r] = 0.0f;
+		}
+		f32 v_unit = 0.0f, v_inv = 0.0f;   // SCALED: weights carry v_scale / v_unit, a power of two no smaller than any seen
+#pragma unroll
+		for (u32 j = 0; j < D / 16; ++j) {
+#pragma unroll
+			for (u32 e = 0; e < 4 * RT; ++e) o[j][e / 4][e % 4] = 0.0f;
+		}
+		u32 const n_min = span.length(row0 / group);                                     // what every row sees: [lo_max, n_min)
+		u32 const lo_max = span.first(span.length((row0 + rows - 1) / group));
+		u32 key0 = span.base() + step * KS;
 
 #pragma unroll 1
-	for (u32 i = 0; i < n_own; ++i) {
-		cp_async_wait<STAGES - 2>();
-		__syncwarp();
-		issue(i + STAGES - 1);
-		u32 const stage = i % STAGES, src = ring + stage * STAGE_BYTES<D, SCALED>;
-		u32 const key0 = base + (step_lo + warp + i * WARPS) * KS;
-		// ---- scores ----
-		f32 arg[KS / 8][2];
-		f32 vs[KS / 8][2];
-#pragma unroll
-		for (u32 n8 = 0; n8 < KS / 8; ++n8) {
-			u32 kw[KW];
-			ld_shared_words(src + (n8 * 8 + g) * RB + t * (D / 4), kw);
-			i32 c[2] = {0, 0};
-#pragma unroll
-			for (u32 k = 0; k < KW; k += 2) mma_s8(c, qw[k], qw[k + 1], kw[k], kw[k + 1]);
-			if constexpr (SCALED) {
-				uint4 const s4 = ld_shared_v4(src + KS * RB + (n8 * 8 + t * 2) * 8);
-				arg[n8][0] = __fmaf_rn(f32(c[0]) * __uint_as_float(s4.x), temp, neg_m);
-				arg[n8][1] = __fmaf_rn(f32(c[1]) * __uint_as_float(s4.z), temp, neg_m);
-				vs[n8][0] = __uint_as_float(s4.y);
-				vs[n8][1] = __uint_as_float(s4.w);
-			} else {
-				arg[n8][0] = __fmaf_rn(f32(c[0]), temp, neg_m);
-				arg[n8][1] = __fmaf_rn(f32(c[1]), temp, neg_m);
+		for (u32 i = 0; i < n_here; ++i) {
+			u32 const src = ring + stage * SB;
+			u32 const bad_now = bad >> (stage * 2) & 3;
+			cp_async_wait<0>();
+			__syncwarp();
+			stage ^= 1;
+			if (i + 1 < n_here) {
+				u32 const s = step + i + 1;
+				if ((s & 15) == 0) {
+					entries = entries_ahead;
+					entries_ahead = page_entries(span, b, s * 2 + 32);
+				}
+				issue(span, b, kvh, s, entries, stage);
+			} else if (left != 0) {
+				issue(next_span, next_b, next_x / p.chunks, 0, entries_next, stage);
 			}
-		}
-		u32 const bad_now = bad >> (stage * SUBS) & ((1u << SUBS) - 1);
-		if (key0 < lo_max || key0 + KS > n_min || bad_now != 0) {
+			// ---- scores ----
+			f32 arg[KS / 8][RT][2];
+			f32 vs[KS / 8][2];
 #pragma unroll
 			for (u32 n8 = 0; n8 < KS / 8; ++n8) {
+				u32 kw[KW];
+				ld_shared_words(src + (n8 * 8 + g) * RB + t * (D / 4), kw);
+				i32 c[4];
+				mma_s8<true>(c, qa[0], kw[0], kw[1]);
 #pragma unroll
-				for (u32 e = 0; e < 2; ++e) {
-					u32 const key = key0 + n8 * 8 + t * 2 + e;
-					if (key < lo || key >= n || (bad_now >> (n8 / 2) & 1)) {
-						arg[n8][e] = __uint_as_float(NEG_INF);
-						vs[n8][e] = 0.0f;   // (what lies there may be anything)
+				for (u32 k = 2; k < KW; k += 2) mma_s8<false>(c, qa[k / 2], kw[k], kw[k + 1]);
+				f32 ks[2] = {1.0f, 1.0f};
+				if constexpr (SCALED) {
+					uint4 const s4 = ld_shared_v4(src + KS * RB + (n8 * 8 + t * 2) * 8);
+					ks[0] = __uint_as_float(s4.x);
+					ks[1] = __uint_as_float(s4.z);
+					vs[n8][0] = __uint_as_float(s4.y);
+					vs[n8][1] = __uint_as_float(s4.w);
+				}
+#pragma unroll
+				for (u32 e = 0; e < 2 * RT; ++e) {
+					f32 const x = SCALED ? f32(c[e]) * ks[e % 2] : f32(c[e]);
+					arg[n8][e / 2][e % 2] = __fmaf_rn(x, temp[e / 2], neg_m[e / 2]);
+				}
+			}
+			if (key0 < lo_max || key0 + KS > n_min || bad_now != 0) {
+#pragma unroll
+				for (u32 n8 = 0; n8 < KS / 8; ++n8) {
+#pragma unroll
+					for (u32 e = 0; e < 2; ++e) {
+						u32 const key = key0 + n8 * 8 + t * 2 + e;
+						bool seen = false;
+#pragma unroll
+						for (u32 r = 0; r < RT; ++r) {
+							bool const off = key < lo[r] || key >= n[r] || (bad_now >> (n8 / 2) & 1);
+							if (off) arg[n8][r][e] = __uint_as_float(NEG_INF);
+							seen |= !off;
+						}
+						if (!seen) vs[n8][e] = 0.0f;   // (what lies there may be anything)
+					}
+				}
+			}
+			key0 += KS;
+			// ---- the maximum, when a score has passed it ----
+			f32 top[RT];
+			bool passed = false;
+#pragma unroll
+			for (u32 r = 0; r < RT; ++r) {
+				top[r] = arg[0][r][0];
+#pragma unroll
+				for (u32 n8 = 0; n8 < KS / 8; ++n8) top[r] = fmaxf(top[r], fmaxf(arg[n8][r][0], arg[n8][r][1]));
+				passed |= top[r] > ARG_MAX;
+			}
+			if (__any_sync(0xffffffffu, passed)) {
+#pragma unroll
+				for (u32 r = 0; r < RT; ++r) {
+					top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+					top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+					f32 const up = fmaxf(top[r] - SHIFT, 0.0f), a = ex2_approx(-up);
+					f32 const a0 = __shfl_sync(0xffffffffu, a, t * 8), a1 = __shfl_sync(0xffffffffu, a, t * 8 + 4);
+					neg_m[r] -= up;
+					sum[r] *= a;
+#pragma unroll
+					for (u32 n8 = 0; n8 < KS / 8; ++n8) {
+						arg[n8][r][0] -= up;
+						arg[n8][r][1] -= up;
+					}
+#pragma unroll
+					for (u32 j = 0; j < D / 16; ++j) {
+						o[j][r][0] *= a0;
+						o[j][r][1] *= a1;
+						o[j][r][2] *= a0;
+						o[j][r][3] *= a1;
+					}
+				}
+			}
+			if constexpr (SCALED) {
+				f32 most = vs[0][0];
+#pragma unroll
+				for (u32 n8 = 0; n8 < KS / 8; ++n8) most = fmaxf(most, fmaxf(vs[n8][0], vs[n8][1]));
+				if (__any_sync(0xffffffffu, most > v_unit)) {
+#pragma unroll
+					for (u32 mask = 16; mask > 0; mask >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, mask));
+					f32 const unit = __uint_as_float(__float_as_uint(fminf(most, 0x1p125f)) & 0x7F800000u) * 2.0f;
+					f32 const a = v_unit * __frcp_rn(unit);   // powers of two
+					v_unit = unit;
+					v_inv = __frcp_rn(unit);
+#pragma unroll
+					for (u32 j = 0; j < D / 16; ++j) {
+#pragma unroll
+						for (u32 e = 0; e < 4 * RT; ++e) o[j][e / 4][e % 4] *= a;
+					}
+				}
+			}
+			// ---- weights and values ----
+#pragma unroll
+			for (u32 j = 0; j < 2; ++j) {
+				u32 hi[RT][2], low[RT][2];
+#pragma unroll
+				for (u32 h = 0; h < 2; ++h) {
+					f32 vw[2] = {1.0f, 1.0f};
+					if constexpr (SCALED) {
+						vw[0] = vs[2 * j + h][0] * v_inv;
+						vw[1] = vs[2 * j + h][1] * v_inv;
+					}
+#pragma unroll
+					for (u32 r = 0; r < RT; ++r) {
+						f32 e0 = ex2_approx(arg[2 * j + h][r][0]), e1 = ex2_approx(arg[2 * j + h][r][1]);
+						sum[r] += e0 + e1;
+						if constexpr (SCALED) {
+							e0 *= vw[0];
+							e1 *= vw[1];
+						}
+						hi[r][h] = f32x2_to_f16x2(e0, e1);
+						if constexpr (LOW) {
+							f32 h0, h1;
+							f16x2_values(hi[r][h], h0, h1);
+							low[r][h] = f32x2_to_f16x2(e0 - h0, e1 - h1);
+						}
+					}
+				}
+				u32 const v0 = src + (j * 16 + t * 2) * RB + D + g * VD;
+				u32 va[VW], vb[VW], vc[VW], vd[VW];
+				ld_shared_words(v0, va);
+				ld_shared_words(v0 + RB, vb);
+				ld_shared_words(v0 + 8 * RB, vc);
+				ld_shared_words(v0 + 9 * RB, vd);
+#pragma unroll
+				for (u32 k = 0; k < VW; ++k) {
+					u32 const v[2][4] = {{codes_to_f16x2<0>(va[k], vb[k]), codes_to_f16x2<1>(va[k], vb[k]), codes_to_f16x2<0>(vc[k], vd[k]),
+										  codes_to_f16x2<1>(vc[k], vd[k])},
+										 {codes_to_f16x2<2>(va[k], vb[k]), codes_to_f16x2<3>(va[k], vb[k]), codes_to_f16x2<2>(vc[k], vd[k]),
+										  codes_to_f16x2<3>(vc[k], vd[k])}};
+#pragma unroll
+					for (u32 r = 0; r < RT; ++r) {
+						mma_f16(o[2 * k][r], v[0], hi[r][0], hi[r][1]);
+						mma_f16(o[2 * k + 1][r], v[1], hi[r][0], hi[r][1]);
+						if constexpr (LOW) {
+							mma_f16(o[2 * k][r], v[0], low[r][0], low[r][1]);
+							mma_f16(o[2 * k + 1][r], v[1], low[r][0], low[r][1]);
+						}
 					}
 				}
 			}
 		}
-		// ---- the maximum, when a score has passed it ----
-		f32 top = arg[0][0];
-#pragma unroll
-		for (u32 n8 = 0; n8 < KS / 8; ++n8) top = fmaxf(top, fmaxf(arg[n8][0], arg[n8][1]));
-		if (__any_sync(0xffffffffu, top > ARG_MAX)) {
-			top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-			top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-			f32 const up = fmaxf(top - SHIFT, 0.0f), a = ex2_approx(-up);
-			f32 const a0 = __shfl_sync(0xffffffffu, a, t * 8), a1 = __shfl_sync(0xffffffffu, a, t * 8 + 4);
-			neg_m -= up;
-			sum *= a;
-#pragma unroll
-			for (u32 n8 = 0; n8 < KS / 8; ++n8) {
-				arg[n8][0] -= up;
-				arg[n8][1] -= up;
-			}
-#pragma unroll
-			for (u32 j = 0; j < D / 16; ++j) {
-				o[j][0] *= a0;
-				o[j][1] *= a1;
-				o[j][2] *= a0;
-				o[j][3] *= a1;
-			}
+		// ---- out, where the run had all steps; else a part ----
+		step += n_here;
+		bool const began = step == n_here, whole = began && step == steps;
+		if (began && lane == 0) {
+			u32 const ends = n_units - left - n_here + steps - 1;   // the last step, counted from this warp's first unit
+			scratch.shared_by[u64(b) * n_x + x] = make_uint2(w, ends / per + 1);
 		}
-		if constexpr (SCALED) {
-			f32 most = vs[0][0];
+		f32 const unit = SCALED ? v_unit : 0.125f;
+		u64 const slot = (u64(w) * 2 + began) * p.chunk_rows;
 #pragma unroll
-			for (u32 n8 = 0; n8 < KS / 8; ++n8) most = fmaxf(most, fmaxf(vs[n8][0], vs[n8][1]));
-			if (__any_sync(0xffffffffu, most > v_unit)) {
+		for (u32 r = 0; r < RT; ++r) {
+			sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+			sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
 #pragma unroll
-				for (u32 mask = 16; mask > 0; mask >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, mask));
-				f32 const unit = __uint_as_float(__float_as_uint(fminf(most, 0x1p125f)) & 0x7F800000u) * 2.0f;
-				f32 const a = v_unit * __frcp_rn(unit);   // powers of two
-				v_unit = unit;
-				v_inv = __frcp_rn(unit);
+			for (u32 e = 0; e < 2; ++e) {
+				u32 const from = (2 * t + e) * 4, at = r * ROWS + 2 * t + e;
+				f32 const m_r = -__shfl_sync(0xffffffffu, neg_m[r], from), s_r = __shfl_sync(0xffffffffu, sum[r], from);
+				f32 const sink_r = __shfl_sync(0xffffffffu, sink[r], from);
+				if (at < rows) {
+					f32 v[VD];
 #pragma unroll
-				for (u32 j = 0; j < D / 16; ++j) {
+					for (u32 j = 0; j < D / 16; ++j) {
+						v[2 * j] = o[j][r][e] * unit;
+						v[2 * j + 1] = o[j][r][e + 2] * unit;
+					}
+					if (whole) {
+						u32 const row = row0 + at, tok = row / group;
+						paged_finish<D, VD>(p, u64(b) * p.n_tokens + tok, kvh * group + row - tok * group, g * VD, m_r, s_r, v, sink_r);
+					} else {
+						float4 *dst = reinterpret_cast<float4 *>(scratch.o + (slot + at) * D + g * VD);
 #pragma unroll
-					for (u32 e = 0; e < 4; ++e) o[j][e] *= a;
+						for (u32 j = 0; j < VD; j += 4) dst[j / 4] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+						if (g == 0) scratch.ms[slot + at] = make_float4(m_r, s_r, sink_r, 0.0f);
+					}
 				}
 			}
 		}
-		// ---- weights and values ----
-#pragma unroll
-		for (u32 j = 0; j < SUBS; ++j) {
-			u32 hi[2], low[2];
-#pragma unroll
-			for (u32 h = 0; h < 2; ++h) {
-				f32 e0 = ex2_approx(arg[2 * j + h][0]), e1 = ex2_approx(arg[2 * j + h][1]);
-				sum += e0 + e1;
-				if constexpr (SCALED) {
-					e0 *= vs[2 * j + h][0] * v_inv;
-					e1 *= vs[2 * j + h][1] * v_inv;
-				}
-				hi[h] = f32x2_to_f16x2(e0, e1);
-				f32 h0, h1;
-				f16x2_values(hi[h], h0, h1);
-				low[h] = f32x2_to_f16x2(e0 - h0, e1 - h1);
-			}
-			u32 const v0 = src + (j * 16 + t * 2) * RB + D + g * (D / 8);
-			u32 va[VW], vb[VW], vc[VW], vd[VW];
-			ld_shared_words(v0, va);
-			ld_shared_words(v0 + RB, vb);
-			ld_shared_words(v0 + 8 * RB, vc);
-			ld_shared_words(v0 + 9 * RB, vd);
-#pragma unroll
-			for (u32 w = 0; w < VW; ++w) {
-				u32 const x[4] = {codes_to_f16x2<0>(va[w], vb[w]), codes_to_f16x2<1>(va[w], vb[w]), codes_to_f16x2<0>(vc[w], vd[w]),
-								  codes_to_f16x2<1>(vc[w], vd[w])};
-				u32 const y[4] = {codes_to_f16x2<2>(va[w], vb[w]), codes_to_f16x2<3>(va[w], vb[w]), codes_to_f16x2<2>(vc[w], vd[w]),
-								  codes_to_f16x2<3>(vc[w], vd[w])};
-				mma_f16(o[2 * w], x, hi[0], hi[1]);
-				mma_f16(o[2 * w + 1], y, hi[0], hi[1]);
-				mma_f16(o[2 * w], x, low[0], low[1]);
-				mma_f16(o[2 * w + 1], y, low[0], low[1]);
-			}
-		}
+		if (left == 0) return;
+		step = 0;
+		b = next_b;
+		x = next_x;
+		span = next_span;
+		steps = span.steps(p.n_tokens);
+		entries = entries_next;
+		entries_ahead = page_entries(span, b, 32);
 	}
-	cp_async_wait<0>();
-	sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-	sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+}
 
-	// ---- merge the warps: [warp][row][D] in the ring's place ----
+// Joins the parts of a (sequence, x): `cta_rows` of its rows to a CTA (1, 2, 4 or 8), as many warps to a row as that leaves, each
+// every so manyth part; a lane D / 32 dims.
+template <u32 D>
+__global__ void __launch_bounds__(paged_cfg::MERGE_WARPS * 32)
+paged_merge_kernel(const PagedDecodeParams p, const PagedScratch scratch, const u32 cta_rows) {
+	using namespace paged_cfg;
+	constexpr u32 V = D / 32, W = MERGE_WARPS;
+	__shared__ f32 sh_o[W][D], sh_m[W], sh_s[W];
+	u32 const warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+	u32 const n_x = p.pool.n_kv_heads * p.chunks;
+	u32 const b = blockIdx.x / n_x, x = blockIdx.x - b * n_x;
+	u32 const group = p.n_heads / p.pool.n_kv_heads;
+	u32 const kvh = x / p.chunks, row0 = (x - kvh * p.chunks) * p.chunk_rows;
+	u32 const r = blockIdx.y * cta_rows + warp % cta_rows, row = row0 + r;
+	u32 const mine = warp / cta_rows, shares = W / cta_rows;
+	pdl_launch_dependents();
+	pdl_wait();
+	uint2 const by = scratch.shared_by[blockIdx.x];
+	if (by.y < 2) return;
+	bool const live = r < p.chunk_rows && row < group * p.n_tokens;
+	// part k is slot [1] of the first warp, slot [0] of the others
+	auto slot = [&](u32 k) { return (u64(by.x + k) * 2 + (k == 0)) * p.chunk_rows + r; };
+	f32 m = -3.0e38f, s = 0.0f;
+	__align__(16) f32 v[V] = {};
+	constexpr u32 AHEAD = 8;
+	for (u32 k0 = mine; live && k0 < by.y; k0 += shares * AHEAD) {
+		float2 ms[AHEAD];
+		__align__(16) f32 part[AHEAD][V];
+#pragma unroll
+		for (u32 i = 0; i < AHEAD; ++i) {
+			u32 const k = k0 + i * shares;
+			ms[i] = make_float2(-3.0e38f, 0.0f);
+			if (k < by.y) {
+				u64 const at = slot(k);
+				ms[i] = *reinterpret_cast<float2 const *>(scratch.ms + at);
+				f32 const *src = scratch.o + at * D + lane * V;
+				if constexpr (V == 4) *reinterpret_cast<float4 *>(part[i]) = *reinterpret_cast<float4 const *>(src);
+				else if constexpr (V == 2) *reinterpret_cast<float2 *>(part[i]) = *reinterpret_cast<float2 const *>(src);
+				else part[i][0] = *src;
+			} else {
+#pragma unroll
+				for (u32 j = 0; j < V; ++j) part[i][j] = 0.0f;
+			}
+		}
+		f32 up = m;
+#pragma unroll
+		for (u32 i = 0; i < AHEAD; ++i) up = fmaxf(up, ms[i].x);
+		f32 const a = ex2_approx(m - up);
+		s *= a;
+#pragma unroll
+		for (u32 j = 0; j < V; ++j) v[j] *= a;
+		m = up;
+#pragma unroll
+		for (u32 i = 0; i < AHEAD; ++i) {
+			f32 const e = ex2_approx(ms[i].x - m);
+			s = __fmaf_rn(ms[i].y, e, s);
+#pragma unroll
+			for (u32 j = 0; j < V; ++j) v[j] = __fmaf_rn(part[i][j], e, v[j]);
+		}
+	}
+#pragma unroll
+	for (u32 j = 0; j < V; ++j) sh_o[warp][lane * V + j] = v[j];
+	if (lane == 0) {
+		sh_m[warp] = m;
+		sh_s[warp] = s;
+	}
 	__syncthreads();
-	f32 *parts = reinterpret_cast<f32 *>(smem);
-	f32 const unit = SCALED ? v_unit : 0.125f;
+	if (!live || mine != 0 || lane >= D / 4) return;
+	f32 out[4] = {};
+	s = 0.0f;
+	for (u32 k = warp; k < W; k += cta_rows) m = fmaxf(m, sh_m[k]);
+	for (u32 k = warp; k < W; k += cta_rows) {
+		f32 const a = ex2_approx(sh_m[k] - m);
+		s = __fmaf_rn(sh_s[k], a, s);
 #pragma unroll
-	for (u32 e = 0; e < 2; ++e) {
-		if (2 * t + e < rows) {
-			f32 *dst = parts + (warp * ROWS + 2 * t + e) * D + g * (D / 8);
-#pragma unroll
-			for (u32 j = 0; j < D / 16; j += 2) {
-				*reinterpret_cast<float4 *>(dst + 2 * j) =
-					make_float4(o[j][e] * unit, o[j][e + 2] * unit, o[j + 1][e] * unit, o[j + 1][e + 2] * unit);
-			}
-		}
+		for (u32 j = 0; j < 4; ++j) out[j] = __fmaf_rn(sh_o[k][lane * 4 + j], a, out[j]);
 	}
-	if (t == 0) {
-		sh_m[warp][g] = -neg_m;   // m - SHIFT
-		sh_s[warp][g] = sum;
-		if (warp == 0) sh_sink[g] = sink - SHIFT;
-	}
-	__syncthreads();
-	if (splits > 1) cluster_wait();   // the first CTA runs (asked for at entry): its shared memory can be written
-	f32 *recv = reinterpret_cast<f32 *>(smem + RING_BYTES<D, SCALED>);
-	for (u32 at = threadIdx.x; at < rows * D; at += THREADS) {
-		u32 const r = at / D, d = at % D;
-		f32 m = sh_m[0][r];
-#pragma unroll
-		for (u32 w = 1; w < WARPS; ++w) m = fmaxf(m, sh_m[w][r]);
-		f32 s = 0.0f, v = 0.0f;
-#pragma unroll
-		for (u32 w = 0; w < WARPS; ++w) {
-			f32 const a = ex2_approx(sh_m[w][r] - m);
-			s = __fmaf_rn(sh_s[w][r], a, s);
-			v = __fmaf_rn(parts[(w * ROWS + r) * D + d], a, v);
-		}
-		if (splits > 1) {
-			u32 const dst = map_to_cta(smem_u32(recv + (blockIdx.z * rows + r) * (D + 2)), 0);
-			st_cluster_f32(dst + d * 4, v);
-			if (d == 0) {
-				st_cluster_f32(dst + D * 4, m);
-				st_cluster_f32(dst + D * 4 + 4, s);
-			}
-		} else {
-			paged_finish<D>(p, b, kvh, row0, r, d, m, s, v, sh_sink[r]);
-		}
-	}
-	pdl_launch_dependents();   // not earlier: a next call's clusters would be packed onto the few SMs with room
-	if (splits > 1) {
-		__syncwarp();
-		cluster_arrive();              // this CTA's part is stored
-		if (blockIdx.z != 0) return;
-		cluster_wait();
-		for (u32 at = threadIdx.x; at < rows * D; at += THREADS) {
-			u32 const r = at / D, d = at % D;
-			f32 m = sh_sink[r], s = 0.0f, v = 0.0f;
-			for (u32 z = 0; z < splits; ++z) m = fmaxf(m, recv[(z * rows + r) * (D + 2) + D]);
-			for (u32 z = 0; z < splits; ++z) {
-				f32 const *part = recv + (z * rows + r) * (D + 2);
-				f32 const a = ex2_approx(part[D] - m);
-				s = __fmaf_rn(part[D + 1], a, s);
-				v = __fmaf_rn(part[d], a, v);
-			}
-			paged_finish<D>(p, b, kvh, row0, r, d, m, s, v, sh_sink[r]);
-		}
-	}
+	u32 const tok = row / group;
+	paged_finish<D, 4>(p, u64(b) * p.n_tokens + tok, kvh * group + row - tok * group, lane * 4, m, s, out, scratch.ms[slot(0)].z);
 }
 
 }  // namespace x17

@@ -396,8 +396,8 @@ class PagedAttnKernel(_Configured):
       page_table   int32 [n_seqs, max_pages]: a sequence's pages in order of position; entries behind its last page are not read
 
     Sequences, positions and pages are checked on the device: what is out of range is left out and recorded in the status words
-    (read_status: code 16). Nothing is allocated, so the calls can be captured into graphs, and two of them can run at once as
-    far as they do not write the same rows."""
+    (read_status: code 16). The calls can be captured into graphs, and two of them can run at once as far as they do not write
+    the same rows."""
 
     def __init__(self, config: PagedConfig):
         self.config = config
@@ -479,10 +479,25 @@ class PagedAttnKernel(_Configured):
             max_pages, _ptr(rope), 0 if rope is None else rope.shape[0], _ptr(pages), _ptr(page_scales), n_pages, _ptr(q_out),
             _ptr(q_scale)))
 
+    def scratch(self, stream, sequences: int, n_tokens: int = 1, device="cuda") -> torch.Tensor:
+        """Memory for the parts of a decode call of this shape, for hosts that allocate nothing while
+        they serve. Calls that may run at the same time need one each."""
+        out, cfg = ctypes.c_size_t(), self.config._c()
+        check(self._lib.x17ai_b200_paged_scratch_bytes(stream.handle, ctypes.byref(cfg), sequences, n_tokens, ctypes.byref(out)))
+        return torch.empty(out.value, dtype=torch.uint8, device=device)
+
+    @staticmethod
+    def _scratch_bytes(scratch):
+        if scratch is None:
+            return 0
+        if scratch.dtype != torch.uint8 or scratch.dim() != 1 or not scratch.is_cuda or not scratch.is_contiguous():
+            raise X17Error("paged decode scratch must be a contiguous uint8 vector on device cuda")
+        return scratch.numel()
+
     def _decode_shapes(self, q, pages, page_scales, page_table, kv_lens, sink_k, sink_v, attn_temperature, out, l, out_dtype):
         c, op = self.config, "paged decode"
         batch = kv_lens.shape[0] if kv_lens.dim() == 1 else 0
-        if batch == 0 or kv_lens.dtype not in (torch.int32, torch.uint32) or not kv_lens.is_cuda or not kv_lens.is_contiguous():
+        if batch == 0 or kv_lens.dtype != torch.int32 or not kv_lens.is_cuda or not kv_lens.is_contiguous():
             raise X17Error(f"{op} input kv_lens must be a contiguous int32 [sequences] on device cuda, got {kv_lens.dtype} {list(kv_lens.shape)}")
         rows, _ = matrix_shape(op, "q", q, (None, c.q_stride), DTYPE_INT8)
         if rows % batch != 0:
@@ -497,22 +512,23 @@ class PagedAttnKernel(_Configured):
         return batch, rows // batch, n_pages, max_pages
 
     def decode(self, stream, q, pages, page_table, kv_lens, sink_k, sink_v, attn_temperature, out, l=None, window_size=0,
-               n_splits=0):
+               scratch=None):
         """New tokens over the cache: `q` [sequences * n, q_stride] holds n (1 to 64) new tokens of each sequence, token i of
         sequence b at position kv_lens[b] + i, which attends the keys in front of that position (the last `window_size` of them,
         0 = all) and the sink, as AttnKernel.decode does. `out` [rows, o_stride] int8 (FixedI8) or bf16; `l` [rows, n_heads].
-        A sequence of length 0 sees the sink alone (a row of padding costs no more). `n_splits`: CTAs that share a sequence's
-        keys, 1 to 16, 0 = chosen."""
+        A sequence of length 0 sees the sink alone (a row of padding costs no more). `scratch`: memory from scratch() for this
+        call's shape, used by one call at a time; without it the call takes its own from the library's pool, in stream order."""
         out_dtype = DTYPE_BF16 if out.dtype == torch.bfloat16 else DTYPE_INT8
         batch, n, n_pages, max_pages = self._decode_shapes(
             q, pages, None, page_table, kv_lens, sink_k, sink_v, attn_temperature, out, l, out_dtype)
         cfg = self.config._c()
         check(self._lib.x17ai_b200_paged_decode(
             stream.handle, ctypes.byref(cfg), batch, n, _ptr(q), _ptr(pages), n_pages, _ptr(page_table), max_pages, _ptr(kv_lens),
-            _ptr(sink_k), _ptr(sink_v), _ptr(attn_temperature), _ptr(out), out_dtype, _ptr(l), window_size, n_splits))
+            _ptr(sink_k), _ptr(sink_v), _ptr(attn_temperature), _ptr(out), out_dtype, _ptr(l), window_size,
+            _ptr(scratch), self._scratch_bytes(scratch)))
 
     def decode_scaled(self, stream, q, q_scale, pages, page_scales, page_table, kv_lens, sink_k, sink_v, attn_temperature, out,
-                      l=None, window_size=0, n_splits=0):
+                      l=None, window_size=0, scratch=None):
         """The same over a cache with scales: `q_scale` f32 [rows, n_heads], `out` bf16."""
         batch, n, n_pages, max_pages = self._decode_shapes(
             q, pages, page_scales, page_table, kv_lens, sink_k, sink_v, attn_temperature, out, l, DTYPE_BF16)
@@ -521,7 +537,7 @@ class PagedAttnKernel(_Configured):
         check(self._lib.x17ai_b200_paged_decode_scaled(
             stream.handle, ctypes.byref(cfg), batch, n, _ptr(q), _ptr(q_scale), _ptr(pages), _ptr(page_scales), n_pages,
             _ptr(page_table), max_pages, _ptr(kv_lens), _ptr(sink_k), _ptr(sink_v), _ptr(attn_temperature), _ptr(out), _ptr(l),
-            window_size, n_splits))
+            window_size, _ptr(scratch), self._scratch_bytes(scratch)))
 
 
 @dataclass(frozen=True)
