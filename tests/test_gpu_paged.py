@@ -23,11 +23,11 @@ def _gpu(a):
     return (a if isinstance(a, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(a))).cuda()
 
 
-def _table(rng, page, ends, spare=2):
-    """Pages in no order; -1 behind a sequence's last page."""
+def _table(rng, page, ends, spare=2, room=0):
+    """Pages in no order; -1 behind a sequence's last page, room for `room` tokens at least."""
     need = [-(-e // page) for e in ends]
     order = rng.permutation(sum(need) + spare).astype(np.int32)
-    table = np.full((len(ends), max(max(need), 1)), -1, dtype=np.int32)
+    table = np.full((len(ends), max(max(need), 1, room // page)), -1, dtype=np.int32)
     at = 0
     for i, n in enumerate(need):
         table[i, :n] = order[at:at + n]
@@ -225,10 +225,10 @@ def _check_decode(got, got_l, want, want_l, bound, bound_l, fixed):
         assert (np.abs(got_l - want_l) <= bound_l).all(), (np.abs(got_l - want_l) / bound_l).max()
 
 
-def _run_decode(stream, H, Hk, D, page, lens, new, window, scaled, fixed, own_scratch=False, extra=0, seed=0, with_l=True, cap=None):
+def _run_decode(stream, H, Hk, D, page, lens, new, window, scaled, fixed, own_scratch=False, extra=0, seed=0, with_l=True, room=0):
     rng = np.random.default_rng([seed, H, D, page, new, len(lens)])
     ends = [n + new - 1 for n in lens]
-    table, n_pages = _table(rng, page, [max(e, cap or 0) for e in ends])
+    table, n_pages = _table(rng, page, ends, room=room)
     pages, scales, seqs = _cache(rng, table, n_pages, Hk, page, D, scaled, ends)
     B = len(lens)
     q = _codes(rng, B * new, H * D + extra)
@@ -284,8 +284,11 @@ DECODES = [
 
 @pytest.mark.parametrize("H,Hk,D,page,lens,new,window", DECODES)
 @pytest.mark.parametrize("kind", ["bf16", "fixed", "scaled"])
-def test_decode(stream, kind, H, Hk, D, page, lens, new, window):
-    _run_decode(stream, H, Hk, D, page, lens, new, window, kind == "scaled", kind == "fixed")
+@pytest.mark.parametrize("room", [0, 80000])
+def test_decode(stream, kind, H, Hk, D, page, lens, new, window, room):
+    """With room for few keys a sequence has CTAs of its own, with room for many all sequences share the chip's (a window
+    counts as room)."""
+    _run_decode(stream, H, Hk, D, page, lens, new, window, kind == "scaled", kind == "fixed", room=room)
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fixed", "scaled"])
@@ -304,17 +307,12 @@ def test_decode_many_sequences(stream, kind):
     _run_decode(stream, 24, 8, 32, 32, [(91 * i) % 777 for i in range(70)], 3, 64, kind == "scaled", kind == "fixed", seed=1)
 
 
-def test_decode_with_room_behind_the_lengths(stream):
-    """A page table with room for far more keys than the sequences have."""
-    _run_decode(stream, 4, 1, 64, 16, [3, 40], 1, 0, False, False, cap=4000)
-
-
 def test_scratch_that_is_too_small(stream):
     from x17ai_b200 import X17Error
     H, D, page = 4, 64, 16
     kern = _kernel(H, H, D, page)
     z = lambda dtype, *shape: torch.zeros(shape, dtype=dtype, device="cuda")
-    args = (z(torch.int8, 2, H * D), kern.pages(4), z(torch.int32, 2, 2), z(torch.int32, 2), z(torch.int8, H, D), z(torch.int8, H, D),
+    args = (z(torch.int8, 2, H * D), kern.pages(4), z(torch.int32, 2, 5000), z(torch.int32, 2), z(torch.int8, H, D), z(torch.int8, H, D),
             z(torch.float32, H), z(torch.bfloat16, 2, H * D))
     scratch = kern.scratch(stream, 2)
     torch.cuda.synchronize()
@@ -374,13 +372,14 @@ def test_decode_lengths_beyond_the_table(stream):
 
 
 @pytest.mark.parametrize("scaled", [False, True])
-def test_decode_leaves_out_bad_pages(scaled):
+@pytest.mark.parametrize("room", [0, 80000])
+def test_decode_leaves_out_bad_pages(scaled, room):
     """A key on a page outside the pool is not attended to; the status words say so."""
     from x17ai_b200 import device
     stream = device.CudaStream(0)
     H, Hk, D, page, n = 4, 2, 64, 16, 100
     rng = np.random.default_rng(6)
-    table, n_pages = _table(rng, page, [n, n])
+    table, n_pages = _table(rng, page, [n, n], room=room)
     pages, scales, seqs = _cache(rng, table, n_pages, Hk, page, D, scaled, [n, n])
     table[0, 2], table[0, 6], table[1, 0] = n_pages, -1, 2 ** 31 - 1
     keep = [np.r_[0:32, 48:96], np.r_[16:100]]
@@ -530,13 +529,14 @@ def test_drafted_tokens_equal_single_steps(stream):
             assert (l[i::new] - one_l).abs().max() <= 1e-4
 
 
-def test_captured_and_replayed():
+@pytest.mark.parametrize("room,kernels", [(0, 2), (80000, 3)])
+def test_captured_and_replayed(room, kernels):
     """A step recorded once and replayed with other positions, lengths and rows in the same buffers; two graphs at once on two
     streams, which share the pool and write different pages."""
     from x17ai_b200 import device, kernels as K
     H, Hk, D, page, B = 8, 2, 64, 16, 4
     rng = np.random.default_rng(31)
-    table, n_pages = _table(rng, page, [200] * (2 * B))
+    table, n_pages = _table(rng, page, [200] * (2 * B), room=room)
     pages, _, _ = _cache(rng, table, n_pages, Hk, page, D, False, [200] * (2 * B))
     t_pages, rope = _gpu(pages), K.rope_table(256, D)
     kern = _kernel(H, Hk, D, page, rotary=D)
@@ -557,7 +557,7 @@ def test_captured_and_replayed():
         s.synchronize()
         with device.CudaGraph(s) as g:
             step()
-        assert g.kernel_nodes == 3
+        assert g.kernel_nodes == kernels
         sides.append((s, x, step, g))
     for turn in range(3):
         fresh = [(_gpu(_codes(rng, B, H * D)), _gpu(_codes(rng, B, 2 * Hk * D)), _gpu(rng.integers(0, 199, B).astype(np.int32))) for _ in sides]
@@ -583,12 +583,13 @@ def test_captured_and_replayed():
         s.close()
 
 
-def test_reads_what_torch_wrote_in_front():
+@pytest.mark.parametrize("room", [0, 80000])
+def test_reads_what_torch_wrote_in_front(room):
     """Inputs written by torch on the same stream right in front of the calls, changing from pass to pass, nothing waited for."""
     from x17ai_b200 import device, kernels as K
     H, Hk, D, page, B, n = 8, 2, 128, 32, 5, 24
     rng = np.random.default_rng(41)
-    table, n_pages = _table(rng, page, [400] * B)
+    table, n_pages = _table(rng, page, [400] * B, room=room)
     kern, rope = _kernel(H, Hk, D, page, rotary=D), K.rope_table(512, D)
     sk, sv, temp = _gpu(_codes(rng, H, D)), _gpu(_codes(rng, H, D)), _gpu(np.ones(H, dtype=np.float32))
     src = [(_gpu(_codes(rng, n_pages, Hk, page, 2 * D)), _gpu(_codes(rng, B, H * D)), _gpu(_codes(rng, B, 2 * Hk * D)),

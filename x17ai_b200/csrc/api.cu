@@ -831,8 +831,8 @@ x17ai_DiagnosticBuffer *check_paged_config(x17ai_PagedConfig const *cfg, char co
 	char const *const bad = "x17ai_b200: bad paged cache config";
 	if (cfg == nullptr) return make_diag("x17ai_b200: null config", who, ": null config");
 	size_t const h = cfg->n_heads, hk = cfg->n_kv_heads, d = cfg->head_dim;
-	if (h == 0 || hk == 0 || h > 65535 || h % hk != 0) {
-		return make_diag(bad, who, ": paged cache config requires n_heads > 0 and a multiple of n_kv_heads, got ", h, " and ", hk);
+	if (h == 0 || hk == 0 || h > 4096 || h % hk != 0) {
+		return make_diag(bad, who, ": paged cache config requires n_heads > 0, at most 4096 and a multiple of n_kv_heads, got ", h, " and ", hk);
 	}
 	if (d != 32 && d != 64 && d != 128) {
 		return make_diag(bad, who, ": paged cache config requires head_dim 32, 64 or 128, got ", d);
@@ -961,7 +961,7 @@ cudaError_t scratch_pool(StreamScope const &on, cudaMemPool_t *pool) {
 
 // How a call's rows are dealt out, and what its parts need.
 struct PagedPlan {
-	uint32_t chunk_rows, chunks, tiles, ctas;
+	uint32_t chunk_rows, chunks, tiles, sm_warps, ctas;
 	size_t n_x, ms_bytes, o_bytes, bytes;   // bytes: [o][ms][shared_by]
 };
 PagedPlan paged_plan(x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, int sm_count) {
@@ -974,13 +974,35 @@ PagedPlan paged_plan(x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens
 	plan.chunks = uint32_t((rows + plan.chunk_rows - 1) / plan.chunk_rows);
 	plan.tiles = plan.chunk_rows > ROWS ? 2 : 1;
 	plan.n_x = cfg->n_kv_heads * plan.chunks;
-	plan.ctas = uint32_t(sm_count) * (cfg->head_dim == 128 && plan.tiles == 2 ? CTAS<128, 2> : CTAS<128, 1>);
-	static_assert(CTAS<64, 1> == CTAS<128, 1> && CTAS<64, 2> == CTAS<128, 1> && CTAS<32, 1> == CTAS<128, 1> && CTAS<32, 2> == CTAS<128, 1>);
-	size_t const slots = size_t(plan.ctas) * WARPS * 2 * plan.chunk_rows;
+	static_assert(SM_WARPS<64, 2> == SM_WARPS<128, 1> && SM_WARPS<32, 2> == SM_WARPS<128, 1>);
+	plan.sm_warps = cfg->head_dim == 128 && plan.tiles == 2 ? SM_WARPS<128, 2> : SM_WARPS<128, 1>;
+	plan.ctas = uint32_t(sm_count) * (plan.sm_warps / WARPS);
+	size_t const slots = size_t(plan.ctas) * (WARPS + 2) * plan.chunk_rows;
 	plan.ms_bytes = slots * sizeof(float4);
 	plan.o_bytes = slots * cfg->head_dim * sizeof(float);
 	plan.bytes = plan.o_bytes + plan.ms_bytes + batch * plan.n_x * sizeof(uint2);
 	return plan;
+}
+
+// CTAs for every (sequence, x), and warps of each, where the whole call finds place on the chip at once and none of its warps
+// gets more than a few steps; splits 0: the list.
+struct PagedPlaces {
+	uint32_t splits, warps;
+};
+PagedPlaces paged_places(PagedPlan const &plan, size_t pairs, size_t keys, int sm_count) {
+	using namespace x17::paged_cfg;
+	size_t const steps = (keys + KS - 1) / KS;
+	size_t const each = (pairs + sm_count - 1) / sm_count;   // CTAs on an SM
+	if (each * WARPS > plan.sm_warps) return {0, WARPS};
+	size_t warps = plan.sm_warps / each, splits = 1;
+	if (each == 1) splits = size_t(sm_count) / pairs;
+	if (splits > MAX_SPLITS) splits = MAX_SPLITS;
+	// no more of either than there are steps
+	if (splits * warps > steps) splits = (steps + warps - 1) / warps;
+	if (splits * warps > steps + warps) warps = steps / splits + 1;
+	if (warps < WARPS) warps = WARPS;
+	if (splits == 0) splits = 1;
+	return {steps <= 9 * splits * warps ? uint32_t(splits) : 0, uint32_t(warps)};
 }
 
 x17ai_DiagnosticBuffer *check_paged_decode(x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, char const *who) {
@@ -1040,9 +1062,14 @@ x17ai_DiagnosticBuffer *paged_decode(char const *who, x17ai_CudaStreamHandle *st
 						 " keys in each of ", batch, " sequences)");
 	}
 	p.chunk_rows = plan.chunk_rows;
-	p.chunks = plan.chunks;
-	bool const own = scratch == nullptr;
-	if (!own && (scratch_bytes < plan.bytes || !aligned16(scratch))) {
+	auto const fast = [](uint32_t d) { return x17::FastDiv{d, uint32_t(((uint64_t(1) << 32) + d - 1) / d)}; };
+	p.chunks = fast(plan.chunks);
+	p.group = fast(uint32_t(cfg->n_heads / cfg->n_kv_heads));
+	p.n_x = uint32_t(plan.n_x);
+	PagedPlaces places = paged_places(plan, batch * plan.n_x, keys, scope.state().sm_count);
+	p.splits = places.splits;
+	bool const own = scratch == nullptr && p.splits == 0;
+	if (scratch != nullptr && (scratch_bytes < plan.bytes || !aligned16(scratch))) {
 		return make_diag("x17ai_b200: scratch too small", who, ": scratch must be 16-byte aligned and have ", plan.bytes, " bytes, got ",
 						 scratch_bytes);
 	}
@@ -1063,18 +1090,23 @@ x17ai_DiagnosticBuffer *paged_decode(char const *who, x17ai_CudaStreamHandle *st
 	parts.ms = reinterpret_cast<float4 *>(at + plan.o_bytes);
 	parts.shared_by = reinterpret_cast<uint2 *>(at + plan.o_bytes + plan.ms_bytes);
 	// Rows that a CTA joins: with many parts to a row its eight warps share one row, with few each takes a row of its own.
-	size_t const parts_each = size_t(plan.ctas) * x17::paged_cfg::WARPS / (batch * plan.n_x);
+	size_t const parts_each = size_t(plan.ctas) / (batch * plan.n_x);
 	uint32_t cta_rows = 1;
 	while (cta_rows < x17::paged_cfg::MERGE_WARPS && cta_rows < plan.chunk_rows && cta_rows * parts_each < 64) cta_rows *= 2;
 	auto go = [&](auto dim, auto tiles, auto low) {
 		constexpr uint32_t D = decltype(dim)::value, RT = decltype(tiles)::value;
 		using K = Kernel<&x17::paged_decode_kernel<D, SCALED, RT, decltype(low)::value>>;
-		constexpr uint32_t ring = x17::paged_cfg::RING_BYTES<D, SCALED>;
-		ce = allow_smem(K{}, scope, ring);
-		if (ce == cudaSuccess) ce = launch(K{}, dim3(plan.ctas), x17::paged_cfg::THREADS, ring, s, dim3(NO_CLUSTER), p, parts);
-		if (ce == cudaSuccess) {
-			ce = launch(Kernel<&x17::paged_merge_kernel<D>>{}, dim3(unsigned(batch * plan.n_x), (plan.chunk_rows + cta_rows - 1) / cta_rows),
-						x17::paged_cfg::MERGE_WARPS * 32, 0, s, dim3(NO_CLUSTER), p, parts, cta_rows);
+		constexpr uint32_t ring = x17::paged_cfg::RING_BYTES<D, SCALED>, most = x17::paged_cfg::SM_WARPS<D, RT>;
+		ce = allow_smem(K{}, scope, ring * most);
+		if (ce == cudaSuccess && p.splits != 0) {
+			ce = launch(K{}, dim3(unsigned(plan.n_x), unsigned(batch), p.splits), places.warps * 32, ring * places.warps, s,
+						p.splits > 1 ? dim3(1, 1, p.splits) : dim3(NO_CLUSTER), p, parts);
+		} else if (ce == cudaSuccess) {
+			ce = launch(K{}, dim3(plan.ctas), x17::paged_cfg::WARPS * 32, ring * x17::paged_cfg::WARPS, s, dim3(NO_CLUSTER), p, parts);
+			if (ce == cudaSuccess) {
+				ce = launch(Kernel<&x17::paged_merge_kernel<D>>{}, dim3(unsigned(batch * plan.n_x), (plan.chunk_rows + cta_rows - 1) / cta_rows),
+							x17::paged_cfg::MERGE_WARPS * 32, 0, s, dim3(NO_CLUSTER), p, parts, plan.ctas * x17::paged_cfg::WARPS, cta_rows);
+			}
 		}
 	};
 	auto go_tiles = [&](auto dim, auto tiles) {
@@ -1096,7 +1128,7 @@ x17ai_DiagnosticBuffer *paged_decode(char const *who, x17ai_CudaStreamHandle *st
 		res = make_diag("x17ai_b200: kernel launch failed", who, ": kernel launch failed: ", cudaGetErrorString(ce));
 	} else {
 		res = launch_result(who);
-		if (res == nullptr) g_launches.fetch_add(1, std::memory_order_relaxed);   // (two kernels)
+		if (res == nullptr && p.splits == 0) g_launches.fetch_add(1, std::memory_order_relaxed);   // (two kernels)
 	}
 	if (own) (void)cudaFreeAsync(scratch, s);
 	return res;

@@ -29,6 +29,12 @@ struct PagedPool {
 	X17_DEV u64 row(u32 page, u32 head, u32 slot) const { return u64(page) * page_rows + ((head << page_shift) + slot); }
 };
 
+// Division by a number that the host knows, for n * d up to 2^32.
+struct FastDiv {
+	u32 d, m;   // m: 2^32 / d, rounded up
+	X17_DEV u32 operator()(u32 n) const { return d == 1 ? n : __umulhi(n, m); }
+};
+
 struct PagedAppendParams {
 	PagedPool pool;
 	void const *q, *kv;     // i8 or bf16, [tokens][stride]; q may be null
@@ -53,7 +59,10 @@ struct PagedDecodeParams {
 	f32 *l;                 // [batch * n_tokens][n_heads] or null
 	u64 q_stride, o_stride;
 	u32 n_heads, n_tokens;
-	u32 chunk_rows, chunks; // rows (query heads of a group x new tokens) of a CTA, CTAs that a key head's rows take
+	u32 chunk_rows;         // rows (query heads of a group x new tokens) of a chunk
+	FastDiv chunks, group;  // chunks that a key head's rows take; query heads that share a key head
+	u32 n_x;                // key heads x chunks
+	u32 splits;             // 0: the list; else CTAs (a cluster) for every (sequence, x)
 	u32 window;             // 0xFFFFFFFF = unbounded
 	bool out_i8;
 	u32 *status;
@@ -154,9 +163,9 @@ paged_append_kernel(const PagedAppendParams p) {
 // eight at a time, so a key is read once for all of them. The work of a call is the list of all steps (32 keys) of all (sequence,
 // key head, eight rows), and every warp of a grid that fills the chip once takes an equal run of it: one sequence of 131072
 // keys and 128 ragged ones keep the chip equally busy, and no length has to be known on the host. A warp works alone: it fills a
-// ring of two steps in shared memory (cp.async; page table entries are fetched a step before that), and where its run covers a
-// whole (sequence, head, rows) it writes the output itself; the parts of those that several warps share go through scratch
-// memory and a second kernel.
+// ring of two steps in shared memory (cp.async; page table entries are fetched 32 runs of keys at once), and where its run covers
+// a whole (sequence, head, rows) it writes the output itself. What the four warps of a CTA share they join at their end; the
+// parts of what several CTAs share go through scratch memory and a second kernel.
 // A page of a head is one run of memory, so pages cost no more than a contiguous cache.
 //
 // Scores: mma m16n8k32 (s8 x s8 -> s32, exact), rows as its M, keys as its N; a lane's bytes of a key row are consecutive, the
@@ -171,31 +180,36 @@ namespace paged_cfg {
 #ifndef PG_MIN
 #define PG_MIN 1
 #endif
-constexpr u32 WARPS = 4, THREADS = WARPS * 32;
+constexpr u32 WARPS = 4;         // of a CTA that takes a run of the list
+constexpr u32 MAX_WARPS = 12;    // of any CTA
 constexpr u32 KS = 32;           // keys of a step: two runs of 16, each in one page
 constexpr u32 STAGES = 2;
 constexpr u32 ROWS = 8;          // of a tile; a warp has one or two
 constexpr u32 MIN_STEPS = PG_MIN;     // of a warp's run
 constexpr f32 SHIFT = 8.0f, ARG_MAX = 14.0f;   // weights are 2^(x - m + SHIFT), at most 2^ARG_MAX (f16 ends below 2^16)
+constexpr u32 MAX_SPLITS = 8;    // CTAs of a cluster
 constexpr u32 MERGE_WARPS = 8;   // of a CTA that joins parts
-// CTAs on an SM: 12 warps with a step in work and a step on its way each, 210 KB of rings. With two tiles at width 128 the sums
-// alone are 64 registers: eight warps.
+// Warps on an SM: 12 with a step in work and a step on its way each, 210 KB of rings. With two tiles at width 128 the sums
+// alone are 64 registers: eight.
 template <u32 D, u32 RT>
-constexpr u32 CTAS = D == 128 && RT == 2 ? 2 : 3;
+constexpr u32 SM_WARPS = D == 128 && RT == 2 ? 8 : 12;
+template <u32 D, u32 RT>
+constexpr u32 REGS = 65536 / (SM_WARPS<D, RT> * 32) / 8 * 8 - (SM_WARPS<D, RT> == 8 ? 8 : 0);
 template <u32 D>
 constexpr u32 ROW_BYTES = 2 * D + 16;          // of a key in the ring: rows 16 bytes off each other's banks
 template <u32 D, bool SCALED>
 constexpr u32 STAGE_BYTES = KS * (ROW_BYTES<D> + (SCALED ? 8 : 0));
 template <u32 D, bool SCALED>
-constexpr u32 RING_BYTES = WARPS * STAGES * STAGE_BYTES<D, SCALED>;
+constexpr u32 RING_BYTES = STAGES * STAGE_BYTES<D, SCALED>;   // of a warp
 }  // namespace paged_cfg
 
-// Parts of (sequence, x) that several warps share. A warp has at most two: [0] of one that began in an earlier warp's
-// run, [1] of one that begins in its own and goes on behind it.
+// Slots for parts of a (sequence, x), each [rows]. One for every warp: of what began in an earlier warp's run and ended in its
+// own, before the run did. Behind these two for every CTA: [0] of what began in an earlier CTA's run, [1] of what begins in its
+// own and goes on behind it.
 struct PagedScratch {
-	uint2 *shared_by;   // [sequences][x]: first warp, number of warps; written on every call
-	float4 *ms;         // [warps][2][rows]: m - SHIFT, sum, the sink's score
-	f32 *o;             // [warps][2][rows][D]
+	uint2 *shared_by;   // [sequences][x]: first CTA, number of CTAs; written on every call
+	float4 *ms;         // [slots][rows]: m - SHIFT, sum, the sink's score
+	f32 *o;             // [slots][rows][D]
 };
 
 X17_DEV void cp_async_16(u32 dst, void const *src) {
@@ -296,15 +310,15 @@ struct PagedSpan {
 
 // VD dims from d on of one row, from the keys' (m, s, v), m being a maximum less SHIFT, and the sink token.
 template <u32 D, u32 VD>
-X17_DEV void paged_finish(PagedDecodeParams const &p, u64 out_row, u32 head, u32 d, f32 m, f32 s, f32 (&v)[VD], f32 sink) {
+X17_DEV void paged_finish(PagedDecodeParams const &p, u64 out_row, u32 head, u32 d, f32 m, f32 s, f32 (&v)[VD], f32 sink,
+						   u32 const (&sink_v)[VD / 4]) {
 	f32 const a = ex2_approx(sink - m);
 	s += a;
-	f32 const inv = __fdiv_rn(1.0f, s);
-	i8 const *sv = p.sink_v + u64(head) * D + d;
+	f32 const inv = rcp_approx(s);   // (one step)
 	u64 const at = out_row * p.o_stride + head * D + d;
 #pragma unroll
 	for (u32 i = 0; i < VD; i += 4) {
-		u32 const w = *reinterpret_cast<u32 const *>(sv + i);
+		u32 const w = sink_v[i / 4];
 		f32 x[4];
 #pragma unroll
 		for (u32 j = 0; j < 4; ++j) x[j] = __fmaf_rn(f32(i8(w >> (8 * j))) * 0.125f, a, v[i + j]) * inv;
@@ -320,19 +334,48 @@ X17_DEV void paged_finish(PagedDecodeParams const &p, u64 out_row, u32 head, u32
 	if (d == 0 && p.l != nullptr) p.l[out_row * p.n_heads + head] = log2f(255.0f * s) + m;
 }
 
-// What the scores of a row are multiplied with.
-template <u32 D, bool SCALED>
-X17_DEV f32 paged_temperature(PagedDecodeParams const &p, u64 q_row, u32 head, u32 seen) {
-	// D^-1/2 log2(min(W', n) + 4) temp_h, and the scales that are not the key's
-	constexpr f32 ROOT = f32(D == 128 ? 0.08838834764831845 : D == 64 ? 0.125 : 0.17677669529663687);
-	f32 const t = ROOT * log2f(f32(seen + 4)) * p.temperature[head];
-	return SCALED ? t * p.q_scale[q_row * p.n_heads + head] : t * 0.015625f;
+template <u32 D, u32 VD>
+X17_DEV void paged_finish(PagedDecodeParams const &p, u64 out_row, u32 head, u32 d, f32 m, f32 s, f32 (&v)[VD], f32 sink) {
+	u32 sink_v[VD / 4];
+#pragma unroll
+	for (u32 i = 0; i < VD / 4; ++i) sink_v[i] = reinterpret_cast<u32 const *>(p.sink_v + u64(head) * D + d)[i];
+	paged_finish<D, VD>(p, out_row, head, d, m, s, v, sink, sink_v);
+}
+
+constexpr f32 NO_PART = -3.0e38f;   // m of what has no keys
+// Joins n parts of four dims of a row, first their maxima, so that no part waits for the one before. ms: m - SHIFT, sum, the
+// sink's score; get(k, true) is a part's, get(k, false) its values.
+template <typename Get>
+X17_DEV void paged_join(float4 &ms, float4 &v, u32 n, Get get) {
+	f32 up = ms.x;
+#pragma unroll 4
+	for (u32 k = 0; k < n; ++k) up = fmaxf(up, get(k, true).x);
+	f32 const a = ex2_approx(ms.x - up);
+	ms.x = up;
+	ms.y *= a;
+	v = make_float4(v.x * a, v.y * a, v.z * a, v.w * a);
+#pragma unroll 4
+	for (u32 k = 0; k < n; ++k) {
+		float4 const m = get(k, true);
+		if (m.x == NO_PART) continue;   // (where its values would lie may be anything)
+		float4 const part = get(k, false);
+		f32 const e = ex2_approx(m.x - up);
+		v.x = __fmaf_rn(part.x, e, v.x);
+		v.y = __fmaf_rn(part.y, e, v.y);
+		v.z = __fmaf_rn(part.z, e, v.z);
+		v.w = __fmaf_rn(part.w, e, v.w);
+		ms.y = __fmaf_rn(m.y, e, ms.y);
+		ms.z = m.z;   // (the same in every part)
+	}
+}
+X17_DEV void st_cluster_f32x4(u32 addr_cluster, float4 v) {
+	st_cluster_v4(addr_cluster, __float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w));
 }
 
 // One warp takes units w * per .. of the call's list, in order of sequence, x (key head, chunk of rows), step. RT: tiles of eight
 // rows that a chunk has. LOW: weights with their low parts.
 template <u32 D, bool SCALED, u32 RT, bool LOW>
-__global__ void __launch_bounds__(paged_cfg::THREADS, paged_cfg::CTAS<D, RT>)
+__global__ void __maxnreg__((paged_cfg::REGS<D, RT>))
 paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 	using namespace paged_cfg;
 	constexpr u32 KW = D / 16;                       // words of a key row that a lane holds
@@ -340,50 +383,73 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 	constexpr u32 VD = D / 8;                        // dims of a lane
 	constexpr u32 RB = ROW_BYTES<D>, SB = STAGE_BYTES<D, SCALED>;
 	constexpr u32 NEG_INF = 0xFF800000u;
+	constexpr f32 ROOT = f32(D == 128 ? 0.08838834764831845 : D == 64 ? 0.125 : 0.17677669529663687);   // D^-1/2
 	extern __shared__ __align__(16) u8 smem[];
-	u32 const lane = threadIdx.x & 31;
+	// what the warps leave for the end: [warp][of the run's beginning, of its end]; those of the end lie in the warps' rings
+	enum : u32 { THERE = 1, BEGAN = 2, ENDED = 4 };
+	__shared__ uint2 items[MAX_WARPS * 2];   // (sequence, x), flags
+	__shared__ float4 item_ms[MAX_WARPS][RT * ROWS];
+	u32 const warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
 	u32 const g = lane >> 2, t = lane & 3;
-	u32 const n_warps = gridDim.x * WARPS, w = (threadIdx.x >> 5) * gridDim.x + blockIdx.x;   // a short list reaches every SM
-	u32 const group = p.n_heads / p.pool.n_kv_heads;
-	u32 const n_x = p.pool.n_kv_heads * p.chunks;
-	u32 const ring = smem_u32(smem) + (threadIdx.x >> 5) * STAGES * SB;
-	pdl_launch_dependents();
+	u32 const n_warps = gridDim.x * warps, w = blockIdx.x * warps + warp;
+	u32 const group = p.group.d;
+	u32 const n_x = p.n_x;
+	u32 const ring = smem_u32(smem) + warp * STAGES * SB;
 	pdl_wait();
 
 	// ---- the warp's run of units ----
-	u32 total = 0;
-	for (u32 i = lane; i < p.pool.n_seqs; i += 32) total += PagedSpan(p, p.kv_lens[i]).steps(p.n_tokens);
+	u32 start, n_units, b, x, step, per = 0;
+	if (p.splits == 0) {
+		pdl_launch_dependents();
+		u32 total = 0;
+		for (u32 i = lane; i < p.pool.n_seqs; i += 32) total += PagedSpan(p, p.kv_lens[i]).steps(p.n_tokens);
 #pragma unroll
-	for (u32 mask = 16; mask > 0; mask >>= 1) total += __shfl_xor_sync(0xffffffffu, total, mask);
-	total *= n_x;   // (below 2^32: checked on the host for sequences of full length)
-	u32 const per = max((total + n_warps - 1) / n_warps, MIN_STEPS);
-	u32 const start = w * per;
-	if (w > total / per || start >= total) return;
-	u32 const n_units = min(per, total - start);
-	u32 left = n_units;
-	u32 b = 0, before = 0;
-	for (u32 target = start / n_x;; b += 32) {
-		u32 const mine = b + lane < p.pool.n_seqs ? PagedSpan(p, p.kv_lens[b + lane]).steps(p.n_tokens) : 0u;
-		u32 upto = mine;
+		for (u32 mask = 16; mask > 0; mask >>= 1) total += __shfl_xor_sync(0xffffffffu, total, mask);
+		total *= n_x;   // (below 2^32: checked on the host for sequences of full length)
+		per = max((total + n_warps - 1) / n_warps, MIN_STEPS);
+		if (blockIdx.x > total / (per * warps) || blockIdx.x * warps * per >= total) return;
+		start = w * per;
+		n_units = start < total ? min(per, total - start) : 0;
+		u32 before = 0;
+		b = 0;
+		for (u32 target = start / n_x; n_units != 0; b += 32) {
+			u32 const mine = b + lane < p.pool.n_seqs ? PagedSpan(p, p.kv_lens[b + lane]).steps(p.n_tokens) : 0u;
+			u32 upto = mine;
 #pragma unroll
-		for (u32 d = 1; d < 32; d <<= 1) {
-			u32 const v = __shfl_up_sync(0xffffffffu, upto, d);
-			if (lane >= d) upto += v;
+			for (u32 d = 1; d < 32; d <<= 1) {
+				u32 const v = __shfl_up_sync(0xffffffffu, upto, d);
+				if (lane >= d) upto += v;
+			}
+			u32 const hit = __ballot_sync(0xffffffffu, before + upto > target);
+			if (hit != 0) {
+				u32 const at = __ffs(hit) - 1;
+				before += __shfl_sync(0xffffffffu, upto - mine, at);
+				b += at;
+				break;
+			}
+			before += __shfl_sync(0xffffffffu, upto, 31);
 		}
-		u32 const hit = __ballot_sync(0xffffffffu, before + upto > target);
-		if (hit != 0) {
-			u32 const at = __ffs(hit) - 1;
-			before += __shfl_sync(0xffffffffu, upto - mine, at);
-			b += at;
-			break;
-		}
-		before += __shfl_sync(0xffffffffu, upto, 31);
+		u32 const steps_of = PagedSpan(p, n_units != 0 ? p.kv_lens[b] : 0).steps(p.n_tokens);
+		x = (start - before * n_x) / steps_of;
+		step = start - before * n_x - x * steps_of;
+	} else {
+		b = blockIdx.y;
+		x = blockIdx.x;
+		// the first pages' entries are brought closer while the length is on its way
+		i32 touch = 0;
+		if (lane * 8 < p.pool.max_pages) asm volatile("ld.global.b32 %0, [%1];" : "=r"(touch) : "l"(p.pool.table + u64(b) * p.pool.max_pages + lane * 8));
+		u32 const all = PagedSpan(p, p.kv_lens[b]).steps(p.n_tokens), each = (all + p.splits - 1) / p.splits;
+		u32 const from = min(blockIdx.z * each, all), to = min(from + each, all), mine = (to - from + warps - 1) / warps;
+		start = step = min(from + warp * mine, to);
+		n_units = min(start + mine, to) - start;
 	}
+	u32 left = n_units;
 
 	// ---- the (sequence, x) in work, and the one behind it (whose first step is fetched under the last of this one) ----
-	PagedSpan span(p, p.kv_lens[b]);
+	PagedSpan span(p, n_units != 0 ? p.kv_lens[b] : 0);
 	u32 steps = span.steps(p.n_tokens);
-	u32 x = (start - before * n_x) / steps, step = (start - before * n_x) % steps;
+	if (lane < 2) items[warp * 2 + lane] = make_uint2(0, 0);
+	if (lane < RT * ROWS) item_ms[warp][lane] = make_float4(NO_PART, 0.0f, 0.0f, 0.0f);
 	// page table entries of the 32 runs of 16 keys from `run` on, one a lane
 	auto page_entries = [&](PagedSpan const &sp, u32 seq, u32 run) -> u32 {
 		u32 const key = sp.base() + (run + lane) * 16;
@@ -419,16 +485,19 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 		}
 		cp_async_commit();
 	};
-	u32 entries = page_entries(span, b, step * 2 & ~31u);
-	issue(span, b, x / p.chunks, step, entries, 0);
-	u32 entries_ahead = page_entries(span, b, (step * 2 & ~31u) + 32);
+	u32 entries = 0, entries_ahead = 0;
+	if (n_units != 0) {
+		entries = page_entries(span, b, step * 2 & ~31u);
+		entries_ahead = page_entries(span, b, (step * 2 & ~31u) + 32);
+	}
 	u32 stage = 0;
+	bool asked = false;   // for the first step
 
 	// tile j: dims g D / 8 + 2 j ([0], [1]) and + 2 j + 1 ([2], [3]) of rows 2 t ([0], [2]) and 2 t + 1 ([1], [3])
 	f32 o[D / 16][RT][4];
 #pragma unroll 1
-	for (;;) {
-		u32 const kvh = x / p.chunks, row0 = (x - kvh * p.chunks) * p.chunk_rows;
+	while (left != 0) {
+		u32 const kvh = p.chunks(x), row0 = (x - kvh * p.chunks.d) * p.chunk_rows;
 		u32 const rows = min(p.chunk_rows, group * p.n_tokens - row0);
 		u32 const n_here = min(steps - step, left);
 		left -= n_here;
@@ -446,22 +515,30 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 		u32 qa[KW / 2][4];   // as the products' first operand
 		u32 n[RT], lo[RT];
 		f32 temp[RT], sink[RT], neg_m[RT], sum[RT];
+		u32 qw[RT][KW], skw[RT][KW];
 #pragma unroll
 		for (u32 r = 0; r < RT; ++r) {
 			u32 const my_row = row0 + min(g + r * ROWS, rows - 1);
-			u32 const tok = my_row / group, head = kvh * group + my_row - tok * group;
+			u32 const tok = p.group(my_row), head = kvh * group + my_row - tok * group;
 			u64 const q_row = u64(b) * p.n_tokens + tok;
-			u32 qw[KW], skw[KW];
-			ld_global_words(p.q + q_row * p.q_stride + head * D + t * (D / 4), qw);
-			ld_global_words(p.sink_k + u64(head) * D + t * (D / 4), skw);
+			ld_global_words(p.q + q_row * p.q_stride + head * D + t * (D / 4), qw[r]);
+			ld_global_words(p.sink_k + u64(head) * D + t * (D / 4), skw[r]);
+			temp[r] = p.temperature[head];
+			if constexpr (SCALED) temp[r] *= p.q_scale[q_row * p.n_heads + head];
 			n[r] = span.length(tok);
 			lo[r] = span.first(n[r]);
-			temp[r] = paged_temperature<D, SCALED>(p, q_row, head, n[r] - lo[r]);
+		}
+		if (!asked) issue(span, b, kvh, step, entries, 0);   // (under the loads above)
+		asked = true;
+#pragma unroll
+		for (u32 r = 0; r < RT; ++r) {
+			// D^-1/2 log2(min(W', n) + 4) temp_h, and the scales that are not the key's
+			temp[r] *= ROOT * log2f(f32(n[r] - lo[r] + 4)) * (SCALED ? 1.0f : 0.015625f);
 			i32 dot = 0;
 #pragma unroll
 			for (u32 k = 0; k < KW; ++k) {
-				dot = __dp4a(i32(qw[k]), i32(skw[k]), dot);
-				qa[k / 2][k % 2 * 2 + r] = qw[k];
+				dot = __dp4a(i32(qw[r][k]), i32(skw[r][k]), dot);
+				qa[k / 2][k % 2 * 2 + r] = qw[r][k];
 				if (RT == 1) qa[k / 2][k % 2 * 2 + 1] = 0;
 			}
 			dot += __shfl_xor_sync(0xffffffffu, dot, 1);
@@ -470,14 +547,17 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 			neg_m[r] = SHIFT - sink[r];
 			sum[r] = 0.0f;
 		}
+		// (zeros that the compiler does not know, or it would move them in front of every product)
+#pragma unroll
+		for (u32 k = 0; k < KW / 2; ++k) asm volatile("" : "+r"(qa[k][0]), "+r"(qa[k][1]), "+r"(qa[k][2]), "+r"(qa[k][3]));
 		f32 v_unit = 0.0f, v_inv = 0.0f;   // SCALED: weights carry v_scale / v_unit, a power of two no smaller than any seen
 #pragma unroll
 		for (u32 j = 0; j < D / 16; ++j) {
 #pragma unroll
 			for (u32 e = 0; e < 4 * RT; ++e) o[j][e / 4][e % 4] = 0.0f;
 		}
-		u32 const n_min = span.length(row0 / group);                                     // what every row sees: [lo_max, n_min)
-		u32 const lo_max = span.first(span.length((row0 + rows - 1) / group));
+		u32 const n_min = span.length(p.group(row0));                                     // what every row sees: [lo_max, n_min)
+		u32 const lo_max = span.first(span.length(p.group(row0 + rows - 1)));
 		u32 key0 = span.base() + step * KS;
 
 #pragma unroll 1
@@ -495,7 +575,7 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 				}
 				issue(span, b, kvh, s, entries, stage);
 			} else if (left != 0) {
-				issue(next_span, next_b, next_x / p.chunks, 0, entries_next, stage);
+				issue(next_span, next_b, p.chunks(next_x), 0, entries_next, stage);
 			}
 			// ---- scores ----
 			f32 arg[KS / 8][RT][2];
@@ -642,24 +722,27 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 				}
 			}
 		}
-		// ---- out, where the run had all steps; else a part ----
+		// ---- out, where the run had all steps; else a part: of the run's beginning to scratch memory, of its end to the ring ----
 		step += n_here;
-		bool const began = step == n_here, whole = began && step == steps;
-		if (began && lane == 0) {
-			u32 const ends = n_units - left - n_here + steps - 1;   // the last step, counted from this warp's first unit
-			scratch.shared_by[u64(b) * n_x + x] = make_uint2(w, ends / per + 1);
+		bool const began = step == n_here, ended = step == steps, whole = p.splits == 0 && began && ended, at_end = left == 0;
+		__syncwarp();
+		if (lane == 0) {
+			if (began && p.splits == 0) {
+				u32 const last = start + n_units - left - n_here + steps - 1;
+				scratch.shared_by[u64(b) * n_x + x] = make_uint2(blockIdx.x, last / (per * warps) - blockIdx.x + 1);
+			}
+			if (!whole) items[warp * 2 + at_end] = make_uint2(b * n_x + x, THERE | (began ? BEGAN : 0u) | (ended ? ENDED : 0u));
 		}
 		f32 const unit = SCALED ? v_unit : 0.125f;
-		u64 const slot = (u64(w) * 2 + began) * p.chunk_rows;
 #pragma unroll
 		for (u32 r = 0; r < RT; ++r) {
 			sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
 			sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
 #pragma unroll
 			for (u32 e = 0; e < 2; ++e) {
-				u32 const from = (2 * t + e) * 4, at = r * ROWS + 2 * t + e;
-				f32 const m_r = -__shfl_sync(0xffffffffu, neg_m[r], from), s_r = __shfl_sync(0xffffffffu, sum[r], from);
-				f32 const sink_r = __shfl_sync(0xffffffffu, sink[r], from);
+				u32 const lane_of = (2 * t + e) * 4, at = r * ROWS + 2 * t + e;
+				f32 const m_r = -__shfl_sync(0xffffffffu, neg_m[r], lane_of), s_r = __shfl_sync(0xffffffffu, sum[r], lane_of);
+				f32 const sink_r = __shfl_sync(0xffffffffu, sink[r], lane_of);
 				if (at < rows) {
 					f32 v[VD];
 #pragma unroll
@@ -668,25 +751,129 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 						v[2 * j + 1] = o[j][r][e + 2] * unit;
 					}
 					if (whole) {
-						u32 const row = row0 + at, tok = row / group;
+						u32 const row = row0 + at, tok = p.group(row);
 						paged_finish<D, VD>(p, u64(b) * p.n_tokens + tok, kvh * group + row - tok * group, g * VD, m_r, s_r, v, sink_r);
 					} else {
-						float4 *dst = reinterpret_cast<float4 *>(scratch.o + (slot + at) * D + g * VD);
+						u64 const slot = u64(w) * p.chunk_rows + at;
+						f32 *dst = at_end ? reinterpret_cast<f32 *>(smem + warp * STAGES * SB) + at * D : scratch.o + slot * D;
 #pragma unroll
-						for (u32 j = 0; j < VD; j += 4) dst[j / 4] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-						if (g == 0) scratch.ms[slot + at] = make_float4(m_r, s_r, sink_r, 0.0f);
+						for (u32 j = 0; j < VD; j += 4) *reinterpret_cast<float4 *>(dst + g * VD + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+						if (g == 0) *(at_end ? item_ms[warp] + at : scratch.ms + slot) = make_float4(m_r, s_r, sink_r, 0.0f);
 					}
 				}
 			}
 		}
-		if (left == 0) return;
 		step = 0;
 		b = next_b;
 		x = next_x;
 		span = next_span;
 		steps = span.steps(p.n_tokens);
 		entries = entries_next;
-		entries_ahead = page_entries(span, b, 32);
+		if (left != 0) entries_ahead = page_entries(span, b, 32);
+	}
+
+	// ---- what the CTA's warps share ----
+	__syncthreads();
+	if (p.splits != 0) {
+		// ... and the CTAs of a cluster: their parts go to the first one's shared memory, [splits][rows][D + 4], in place of its ring
+		static_assert(MAX_SPLITS * RT * ROWS * (D + 4) * 4 <= WARPS * RING_BYTES<D, SCALED>);
+		constexpr u32 MINE = (RT * ROWS * (D / 4) + WARPS * 32 - 1) / (WARPS * 32);   // (rows of four dims that a thread has at most)
+		u32 const kvh = p.chunks(blockIdx.x), row0 = (blockIdx.x - kvh * p.chunks.d) * p.chunk_rows;
+		u32 const rows = min(p.chunk_rows, group * p.n_tokens - row0);
+		float4 ms[MINE], v[MINE];
+		u32 sink_v[MINE];
+		auto place = [&](u32 c, u32 &r, u32 &d, u64 &out_row, u32 &head) {
+			u32 const at = threadIdx.x + c * blockDim.x;
+			r = at / (D / 4);
+			d = at % (D / 4) * 4;
+			u32 const row = row0 + r, tok = p.group(row);
+			out_row = u64(blockIdx.y) * p.n_tokens + tok;
+			head = kvh * group + row - tok * group;
+			return r < rows;
+		};
+#pragma unroll
+		for (u32 c = 0; c < MINE; ++c) {
+			u32 r, d, head;
+			u64 out_row;
+			ms[c] = make_float4(NO_PART, 0.0f, 0.0f, 0.0f);
+			v[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+			if (place(c, r, d, out_row, head)) {
+				sink_v[c] = *reinterpret_cast<u32 const *>(p.sink_v + u64(head) * D + d);
+				paged_join(ms[c], v[c], warps, [&](u32 k, bool of_ms) {
+					return of_ms ? item_ms[k][r] : *reinterpret_cast<float4 const *>(reinterpret_cast<f32 const *>(smem + k * STAGES * SB) + r * D + d);
+				});
+			}
+		}
+		pdl_launch_dependents();   // not earlier: a next call's clusters would be packed onto the few SMs with room
+		if (p.splits > 1) {
+			cluster_arrive();
+			cluster_wait();        // every CTA runs, and has read its ring
+			u32 const to = map_to_cta(smem_u32(smem) + blockIdx.z * rows * (D + 4) * 4, 0);
+#pragma unroll
+			for (u32 c = 0; c < MINE; ++c) {
+				u32 r, d, head;
+				u64 out_row;
+				if (place(c, r, d, out_row, head)) {
+					st_cluster_f32x4(to + (r * (D + 4) + d) * 4, v[c]);
+					if (d == 0) st_cluster_f32x4(to + (r * (D + 4) + D) * 4, ms[c]);
+				}
+			}
+			__syncwarp();
+			cluster_arrive();      // this CTA's part is stored
+			if (blockIdx.z != 0) return;
+			cluster_wait();
+		}
+#pragma unroll
+		for (u32 c = 0; c < MINE; ++c) {
+			u32 r, d, head;
+			u64 out_row;
+			if (place(c, r, d, out_row, head)) {
+				paged_join(ms[c], v[c], p.splits - 1, [&](u32 z, bool of_ms) {
+					return *reinterpret_cast<float4 const *>(reinterpret_cast<f32 const *>(smem) + ((z + 1) * rows + r) * (D + 4) + (of_ms ? D : d));
+				});
+				f32 out[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+				u32 const sv[1] = {sink_v[c]};
+				paged_finish<D, 4>(p, out_row, head, d, ms[c].x, ms[c].y, out, ms[c].z, sv);
+			}
+		}
+		return;
+	}
+#pragma unroll 1
+	for (u32 i = 0; i < warps * 2;) {
+		uint2 const first = items[i];
+		if (!(first.y & THERE)) {
+			++i;
+			continue;
+		}
+		u32 end = i + 1, last = i;
+		for (; end < warps * 2 && (!(items[end].y & THERE) || items[end].x == first.x); ++end) {
+			if (items[end].y & THERE) last = end;
+		}
+		bool const began = first.y & BEGAN, whole = began && (items[last].y & ENDED);
+		u32 const seq = first.x / n_x, x_of = first.x - seq * n_x, kvh = p.chunks(x_of), row0 = (x_of - kvh * p.chunks.d) * p.chunk_rows;
+		u32 const rows = min(p.chunk_rows, group * p.n_tokens - row0);
+		for (u32 at = threadIdx.x; at < rows * (D / 4); at += blockDim.x) {
+			u32 const r = at / (D / 4), d = at % (D / 4) * 4;
+			float4 ms = make_float4(NO_PART, 0.0f, 0.0f, 0.0f), v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+			paged_join(ms, v, last + 1 - i, [&](u32 from_i, bool of_ms) {
+				u32 const k = i + from_i;
+				if (!(items[k].y & THERE)) return make_float4(NO_PART, 0.0f, 0.0f, 0.0f);
+				u64 const slot = u64(blockIdx.x * warps + k / 2) * p.chunk_rows + r;
+				if (of_ms) return k & 1 ? item_ms[k / 2][r] : scratch.ms[slot];
+				f32 const *part = k & 1 ? reinterpret_cast<f32 const *>(smem + k / 2 * STAGES * SB) + r * D : scratch.o + slot * D;
+				return *reinterpret_cast<float4 const *>(part + d);
+			});
+			if (whole) {
+				u32 const row = row0 + r, tok = p.group(row);
+				f32 out[4] = {v.x, v.y, v.z, v.w};
+				paged_finish<D, 4>(p, u64(seq) * p.n_tokens + tok, kvh * group + row - tok * group, d, ms.x, ms.y, out, ms.z);
+			} else {
+				u64 const slot = (u64(n_warps) + blockIdx.x * 2 + began) * p.chunk_rows + r;
+				*reinterpret_cast<float4 *>(scratch.o + slot * D + d) = v;
+				if (d == 0) scratch.ms[slot] = ms;
+			}
+		}
+		i = last + 1;
 	}
 }
 
@@ -694,15 +881,15 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 // every so manyth part; a lane D / 32 dims.
 template <u32 D>
 __global__ void __launch_bounds__(paged_cfg::MERGE_WARPS * 32)
-paged_merge_kernel(const PagedDecodeParams p, const PagedScratch scratch, const u32 cta_rows) {
+paged_merge_kernel(const PagedDecodeParams p, const PagedScratch scratch, const u32 first_slot, const u32 cta_rows) {
 	using namespace paged_cfg;
 	constexpr u32 V = D / 32, W = MERGE_WARPS;
 	__shared__ f32 sh_o[W][D], sh_m[W], sh_s[W];
 	u32 const warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-	u32 const n_x = p.pool.n_kv_heads * p.chunks;
+	u32 const n_x = p.n_x;
 	u32 const b = blockIdx.x / n_x, x = blockIdx.x - b * n_x;
-	u32 const group = p.n_heads / p.pool.n_kv_heads;
-	u32 const kvh = x / p.chunks, row0 = (x - kvh * p.chunks) * p.chunk_rows;
+	u32 const group = p.group.d;
+	u32 const kvh = p.chunks(x), row0 = (x - kvh * p.chunks.d) * p.chunk_rows;
 	u32 const r = blockIdx.y * cta_rows + warp % cta_rows, row = row0 + r;
 	u32 const mine = warp / cta_rows, shares = W / cta_rows;
 	pdl_launch_dependents();
@@ -710,8 +897,15 @@ paged_merge_kernel(const PagedDecodeParams p, const PagedScratch scratch, const 
 	uint2 const by = scratch.shared_by[blockIdx.x];
 	if (by.y < 2) return;
 	bool const live = r < p.chunk_rows && row < group * p.n_tokens;
-	// part k is slot [1] of the first warp, slot [0] of the others
-	auto slot = [&](u32 k) { return (u64(by.x + k) * 2 + (k == 0)) * p.chunk_rows + r; };
+	// part k is slot [1] of the first CTA, slot [0] of the others
+	auto slot = [&](u32 k) { return (u64(first_slot) + (by.x + k) * 2 + (k == 0)) * p.chunk_rows + r; };
+	u32 const tok = p.group(row), head = kvh * group + row - tok * group;
+	f32 sink = 0.0f;
+	u32 sink_v[1] = {};
+	if (live && mine == 0 && lane < D / 4) {
+		sink = scratch.ms[slot(0)].z;
+		sink_v[0] = reinterpret_cast<u32 const *>(p.sink_v + u64(head) * D)[lane];
+	}
 	f32 m = -3.0e38f, s = 0.0f;
 	__align__(16) f32 v[V] = {};
 	constexpr u32 AHEAD = 8;
@@ -767,8 +961,7 @@ paged_merge_kernel(const PagedDecodeParams p, const PagedScratch scratch, const 
 #pragma unroll
 		for (u32 j = 0; j < 4; ++j) out[j] = __fmaf_rn(sh_o[k][lane * 4 + j], a, out[j]);
 	}
-	u32 const tok = row / group;
-	paged_finish<D, 4>(p, u64(b) * p.n_tokens + tok, kvh * group + row - tok * group, lane * 4, m, s, out, scratch.ms[slot(0)].z);
+	paged_finish<D, 4>(p, u64(b) * p.n_tokens + tok, head, lane * 4, m, s, out, sink, sink_v);
 }
 
 }  // namespace x17
