@@ -959,12 +959,13 @@ cudaError_t scratch_pool(StreamScope const &on, cudaMemPool_t *pool) {
 	return cudaSuccess;
 }
 
+constexpr size_t ANY_KEYS = size_t(1) << 31;   // of a sequence: what scratch memory has to suffice for
 // How a call's rows are dealt out, and what its parts need.
 struct PagedPlan {
-	uint32_t chunk_rows, chunks, tiles, sm_warps, ctas;
+	uint32_t chunk_rows, chunks, tiles, sm_warps, first_ctas, ctas;   // ctas: of the list
 	size_t n_x, ms_bytes, o_bytes, bytes;   // bytes: [o][ms][shared_by]
 };
-PagedPlan paged_plan(x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, int sm_count) {
+PagedPlan paged_plan(x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, size_t keys, int sm_count) {
 	using namespace x17::paged_cfg;
 	PagedPlan plan{};
 	// the rows of a key head in as few chunks of at most two tiles as they need, evenly
@@ -976,7 +977,8 @@ PagedPlan paged_plan(x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens
 	plan.n_x = cfg->n_kv_heads * plan.chunks;
 	static_assert(SM_WARPS<64, 2> == SM_WARPS<128, 1> && SM_WARPS<32, 2> == SM_WARPS<128, 1>);
 	plan.sm_warps = cfg->head_dim == 128 && plan.tiles == 2 ? SM_WARPS<128, 2> : SM_WARPS<128, 1>;
-	plan.ctas = uint32_t(sm_count) * (plan.sm_warps / WARPS);
+	plan.first_ctas = uint32_t(sm_count) * (plan.sm_warps / WARPS);
+	plan.ctas = batch * plan.n_x * (keys / KS + 1) / (plan.first_ctas * WARPS) >= LONG_RUN ? plan.first_ctas * MORE_CTAS : plan.first_ctas;
 	size_t const slots = size_t(plan.ctas) * (WARPS + 2) * plan.chunk_rows;
 	plan.ms_bytes = slots * sizeof(float4);
 	plan.o_bytes = slots * cfg->head_dim * sizeof(float);
@@ -1054,10 +1056,10 @@ x17ai_DiagnosticBuffer *paged_decode(char const *who, x17ai_CudaStreamHandle *st
 	p.out_i8 = out_dtype == X17AI_DTYPE_INT8;
 	p.status = scope.state().status;
 	cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-	PagedPlan const plan = paged_plan(cfg, batch, n_tokens, scope.state().sm_count);
 	size_t const capacity = max_pages * cfg->page_size;
-	size_t const keys = p.window < capacity ? p.window + n_tokens + 15 : capacity;
-	if (batch * plan.n_x * (keys / x17::paged_cfg::KS + 2) >= (size_t(1) << 32)) {
+	size_t const keys = p.window < capacity ? p.window + n_tokens + 15 : capacity;   // at most, of a sequence
+	PagedPlan const plan = paged_plan(cfg, batch, n_tokens, keys, scope.state().sm_count);
+	if (batch * plan.n_x * (keys / x17::paged_cfg::KS + 2) >= (size_t(1) << 31)) {
 		return make_diag("x17ai_b200: decode shape out of range", who, ": sequences x key heads x keys out of range (room for ", capacity,
 						 " keys in each of ", batch, " sequences)");
 	}
@@ -1066,12 +1068,16 @@ x17ai_DiagnosticBuffer *paged_decode(char const *who, x17ai_CudaStreamHandle *st
 	p.chunks = fast(plan.chunks);
 	p.group = fast(uint32_t(cfg->n_heads / cfg->n_kv_heads));
 	p.n_x = uint32_t(plan.n_x);
+	p.first_ctas = plan.first_ctas;
 	PagedPlaces places = paged_places(plan, batch * plan.n_x, keys, scope.state().sm_count);
 	p.splits = places.splits;
 	bool const own = scratch == nullptr && p.splits == 0;
-	if (scratch != nullptr && (scratch_bytes < plan.bytes || !aligned16(scratch))) {
-		return make_diag("x17ai_b200: scratch too small", who, ": scratch must be 16-byte aligned and have ", plan.bytes, " bytes, got ",
-						 scratch_bytes);
+	if (scratch != nullptr) {
+		size_t const need = paged_plan(cfg, batch, n_tokens, ANY_KEYS, scope.state().sm_count).bytes;
+		if (scratch_bytes < need || !aligned16(scratch)) {
+			return make_diag("x17ai_b200: scratch too small", who, ": scratch must be 16-byte aligned and have ", need, " bytes, got ",
+							 scratch_bytes);
+		}
 	}
 	cudaError_t ce = cudaSuccess;
 	if (own) {
@@ -1617,7 +1623,7 @@ x17ai_DiagnosticBuffer *x17ai_b200_paged_scratch_bytes(
 	if (bytes == nullptr) return make_diag("x17ai_b200: null argument", who, ": null argument");
 	StreamScope scope(stream, who);
 	if (scope.diag) return scope.diag;
-	*bytes = paged_plan(cfg, batch, n_tokens, scope.state().sm_count).bytes;
+	*bytes = paged_plan(cfg, batch, n_tokens, ANY_KEYS, scope.state().sm_count).bytes;
 	return nullptr;
 }
 

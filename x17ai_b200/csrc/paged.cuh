@@ -63,6 +63,7 @@ struct PagedDecodeParams {
 	FastDiv chunks, group;  // chunks that a key head's rows take; query heads that share a key head
 	u32 n_x;                // key heads x chunks
 	u32 splits;             // 0: the list; else CTAs (a cluster) for every (sequence, x)
+	u32 first_ctas;         // of the list: CTAs that the chip holds at once
 	u32 window;             // 0xFFFFFFFF = unbounded
 	bool out_i8;
 	u32 *status;
@@ -177,15 +178,13 @@ paged_append_kernel(const PagedAppendParams p) {
 // m's nothing is lost to f16's range. m starts at the sink's score, so no key and no row leaves it undefined.
 
 namespace paged_cfg {
-#ifndef PG_MIN
-#define PG_MIN 1
-#endif
-constexpr u32 WARPS = 4;         // of a CTA that takes a run of the list
+constexpr u32 WARPS = 4;         // of a CTA at least
 constexpr u32 MAX_WARPS = 12;    // of any CTA
 constexpr u32 KS = 32;           // keys of a step: two runs of 16, each in one page
 constexpr u32 STAGES = 2;
 constexpr u32 ROWS = 8;          // of a tile; a warp has one or two
-constexpr u32 MIN_STEPS = PG_MIN;     // of a warp's run
+constexpr u32 LONG_RUN = 100;    // steps of a warp, from which the list is not dealt out equally
+constexpr u32 MORE_CTAS = 3;     // CTAs of the list then, as a multiple of what the chip holds at once
 constexpr f32 SHIFT = 8.0f, ARG_MAX = 14.0f;   // weights are 2^(x - m + SHIFT), at most 2^ARG_MAX (f16 ends below 2^16)
 constexpr u32 MAX_SPLITS = 8;    // CTAs of a cluster
 constexpr u32 MERGE_WARPS = 8;   // of a CTA that joins parts
@@ -334,6 +333,24 @@ X17_DEV void paged_finish(PagedDecodeParams const &p, u64 out_row, u32 head, u32
 	if (d == 0 && p.l != nullptr) p.l[out_row * p.n_heads + head] = log2f(255.0f * s) + m;
 }
 
+// The list dealt out to CTAs in order. SMs do not read equally fast: with equal runs of 350 us the first are done 60 to 90 us before
+// the last. Where the runs are long, the CTAs that are there from the beginning get four fifths of the work, and twice as many smaller
+// ones the rest, each where one has ended (64 x 4096 keys x 32 heads: 362 -> 342 us). A CTA more costs an SM about as long as
+// 6 us of its reading: with runs of 100 us (128 ragged sequences, 543 MB) that is what the balance gains, below it is a loss
+// (131072 keys of one sequence: 59 -> 78 us).
+struct PagedRuns {
+	u32 total, first, large, small;
+	X17_DEV PagedRuns() = default;
+	X17_DEV PagedRuns(u32 total, u32 first, u32 ctas) : total(total), first(first) {
+		bool const equal = ctas == first || total / (first * paged_cfg::WARPS) < paged_cfg::LONG_RUN;
+		large = (equal ? total : total / 5 * 4) / first + 1;
+		u32 const rest = total - min(total, large * first);
+		small = equal ? 1 : rest / (ctas - first) + 1;
+	}
+	X17_DEV u32 start(u32 cta) const { return min(total, cta <= first ? cta * large : first * large + (cta - first) * small); }
+	X17_DEV u32 cta(u32 unit) const { return unit < first * large ? unit / large : first + (unit - first * large) / small; }
+};
+
 template <u32 D, u32 VD>
 X17_DEV void paged_finish(PagedDecodeParams const &p, u64 out_row, u32 head, u32 d, f32 m, f32 s, f32 (&v)[VD], f32 sink) {
 	u32 sink_v[VD / 4];
@@ -398,7 +415,8 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 	pdl_wait();
 
 	// ---- the warp's run of units ----
-	u32 start, n_units, b, x, step, per = 0;
+	u32 start, n_units, b, x, step;
+	PagedRuns runs{};
 	if (p.splits == 0) {
 		pdl_launch_dependents();
 		u32 total = 0;
@@ -406,10 +424,11 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 #pragma unroll
 		for (u32 mask = 16; mask > 0; mask >>= 1) total += __shfl_xor_sync(0xffffffffu, total, mask);
 		total *= n_x;   // (below 2^32: checked on the host for sequences of full length)
-		per = max((total + n_warps - 1) / n_warps, MIN_STEPS);
-		if (blockIdx.x > total / (per * warps) || blockIdx.x * warps * per >= total) return;
-		start = w * per;
-		n_units = start < total ? min(per, total - start) : 0;
+		runs = PagedRuns(total, p.first_ctas, gridDim.x);
+		u32 const from = runs.start(blockIdx.x), to = runs.start(blockIdx.x + 1), each = (to - from + warps - 1) / warps;
+		if (from == to) return;
+		start = min(from + warp * each, to);
+		n_units = min(start + each, to) - start;
 		u32 before = 0;
 		b = 0;
 		for (u32 target = start / n_x; n_units != 0; b += 32) {
@@ -729,7 +748,7 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 		if (lane == 0) {
 			if (began && p.splits == 0) {
 				u32 const last = start + n_units - left - n_here + steps - 1;
-				scratch.shared_by[u64(b) * n_x + x] = make_uint2(blockIdx.x, last / (per * warps) - blockIdx.x + 1);
+				scratch.shared_by[u64(b) * n_x + x] = make_uint2(blockIdx.x, runs.cta(last) - blockIdx.x + 1);
 			}
 			if (!whole) items[warp * 2 + at_end] = make_uint2(b * n_x + x, THERE | (began ? BEGAN : 0u) | (ended ? ENDED : 0u));
 		}
