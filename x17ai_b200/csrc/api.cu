@@ -889,8 +889,7 @@ x17ai_DiagnosticBuffer *paged_append(char const *who, x17ai_CudaStreamHandle *st
 									 int32_t const *table, size_t n_seqs, size_t max_pages, int16_t const *rope, size_t rope_rows,
 									 int8_t *pages, float *scales, size_t n_pages, int8_t *q_out, float *q_scale, int8_t *kv_out) {
 	if (auto *d = check_paged_config(cfg, who)) return d;
-	// (the grid has one warp per token and head, four to a CTA)
-	if (tokens == 0 || tokens >= (size_t(1) << 31) || tokens * (cfg->n_heads + 2 * cfg->n_kv_heads) >= (size_t(1) << 33)) {
+	if (tokens == 0 || tokens >= (size_t(1) << 31)) {
 		return make_diag("x17ai_b200: bad token count", who, ": input kv has zero size or too many rows");
 	}
 	x17::PagedAppendParams p{};
@@ -920,13 +919,21 @@ x17ai_DiagnosticBuffer *paged_append(char const *who, x17ai_CudaStreamHandle *st
 	p.n_heads = uint32_t(cfg->n_heads);
 	p.rope_rows = uint32_t(rope_rows < (size_t(1) << 31) ? rope_rows : (size_t(1) << 31));
 	p.rotary = uint32_t(cfg->rotary_dim);
-	p.adjacent = cfg->adjacent_pairs != 0;
 	p.status = scope.state().status;
 	cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-	size_t const items = tokens * ((q != nullptr ? cfg->n_heads : 0) + 2 * cfg->n_kv_heads);
+	// a warp a token; where that leaves the chip empty, several share its heads
+	size_t const rounds = ((q != nullptr ? cfg->n_heads : 0) + 2 * cfg->n_kv_heads + 1024 / cfg->head_dim - 1) / (1024 / cfg->head_dim);
+	size_t const want = size_t(scope.state().sm_count) * 16;
+	size_t const parts = tokens >= want ? 1 : (want + tokens - 1) / tokens;
+	p.parts = uint32_t(parts < rounds ? parts : rounds);
 	auto go = [&](auto dim) {
 		constexpr uint32_t D = decltype(dim)::value;
-		(void)launch(Kernel<&x17::paged_append_kernel<D, SCALED>>{}, dim3(unsigned((items + 3) / 4)), 128, 0, s, dim3(NO_CLUSTER), p);
+		dim3 const grid(unsigned((tokens * p.parts + x17::append_cfg::WARPS - 1) / x17::append_cfg::WARPS));
+		if (cfg->adjacent_pairs) {
+			(void)launch(Kernel<&x17::paged_append_kernel<D, SCALED, true>>{}, grid, x17::append_cfg::THREADS, 0, s, dim3(NO_CLUSTER), p);
+		} else {
+			(void)launch(Kernel<&x17::paged_append_kernel<D, SCALED, false>>{}, grid, x17::append_cfg::THREADS, 0, s, dim3(NO_CLUSTER), p);
+		}
 	};
 	if (cfg->head_dim == 128) go(std::integral_constant<uint32_t, 128>{});
 	else if (cfg->head_dim == 64) go(std::integral_constant<uint32_t, 64>{});

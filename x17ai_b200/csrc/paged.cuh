@@ -44,7 +44,7 @@ struct PagedAppendParams {
 	f32 *q_scale;           // [tokens][n_heads], scaled form
 	u64 q_stride, kv_stride;
 	u32 tokens, n_heads, rope_rows, rotary;
-	bool adjacent;          // pairs (2 i, 2 i + 1); otherwise (i, i + rotary / 2)
+	u32 parts;              // warps that share a token's heads
 	u32 *status;
 };
 
@@ -78,81 +78,194 @@ X17_DEV bool paged_slot(PagedPool const &pool, i32 seq, i32 pos, u32 &page, u32 
 	return page < pool.n_pages;
 }
 
-// One warp per token and head (query heads, then key and value heads). FixedI8: x' = (x cos - y sin + 2^13) >> 14 in integers.
-// Scaled: x' in f32 (bf16 times a 15-bit table value is exact), code = rint(x' * (127 / absmax)).
-template <u32 D, bool SCALED>
-__global__ void __launch_bounds__(128)
+// ---- append ------------------------------------------------------------------------------------
+//
+// Reads and writes every row once: HBM-bound for prompts, one chain of four loads (position, page, row of the rope table) for a
+// decode step. A warp takes a token, or where there are few tokens a part of its heads. A lane holds 32 dims of a head, in two runs
+// of 16: both halves of 16 pairs, whose cosines and sines it loads once and keeps for all heads of the token. Lanes of one head
+// lie side by side, so loads and stores are whole sectors. Rows of the next heads are on their way under the arithmetic.
+//
+// FixedI8: x' = (x cos - y sin + 2^13) >> 14 is one dp2a (two products of 16 by 8 bits and a sum) and a shift, exact in 32 bits.
+// Scaled: x' in f32; bf16 times a 15-bit table value is exact, so x' has one rounding and is the same however it is fused;
+// absmax over the lanes of a head; code = rint(x' * (127 / absmax)) by adding 1.5 * 2^23 (|code| <= 127, so its low byte is it).
+
+namespace append_cfg {
+constexpr u32 THREADS = 128, WARPS = THREADS / 32;
+}
+
+// a: two signed 16-bit values, pair PAIR of b's signed bytes
+template <u32 PAIR>
+X17_DEV i32 dp2a_s16_s8(u32 a, u32 b, i32 c) {
+	return PAIR == 0 ? __dp2a_lo(i32(a), i32(b), c) : __dp2a_hi(i32(a), i32(b), c);
+}
+// four sums in units of 2^-14 -> codes
+X17_DEV u32 pack4_turned(i32 a, i32 b, i32 c, i32 d) {
+	constexpr i32 LEAST = -127 * 16384;   // the pack saturates at -128
+	a = max(a, LEAST) >> 14;
+	b = max(b, LEAST) >> 14;
+	c = max(c, LEAST) >> 14;
+	d = max(d, LEAST) >> 14;
+	u32 hi, packed;
+	asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, 0;" : "=r"(hi) : "r"(d), "r"(c));
+	asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(packed) : "r"(b), "r"(a), "r"(hi));
+	return packed;
+}
+
+// One head's 32 dims of a lane: FixedI8 bytes, or bf16 pairs.
+template <bool SCALED>
+struct AppendRow {
+	uint4 lo[SCALED ? 2 : 1], hi[SCALED ? 2 : 1];
+};
+
+template <u32 D, bool SCALED, bool ADJACENT>
+__global__ void __launch_bounds__(append_cfg::THREADS)
 paged_append_kernel(const PagedAppendParams p) {
+	constexpr u32 C = D / 32;        // lanes of a head
+	constexpr u32 HEADS = 32 / C;    // heads of a warp at once
+	constexpr u32 SIZE = SCALED ? 2 : 1;
 	pdl_launch_dependents();
 	pdl_wait();
-	constexpr u32 V = D / 32;
-	u32 const lane = threadIdx.x & 31;
-	u32 const n_q = p.q == nullptr ? 0u : p.n_heads;
-	u32 const per_token = n_q + 2 * p.pool.n_kv_heads;
-	u64 const item = u64(blockIdx.x) * 4 + (threadIdx.x >> 5);
-	if (item >= u64(p.tokens) * per_token) return;
-	u32 const token = u32(item / per_token), head = u32(item % per_token);
+	u32 const lane = threadIdx.x & 31, chunk = lane % C;
+	u32 const n_q = p.q == nullptr ? 0u : p.n_heads, n_kv = p.pool.n_kv_heads;
+	u32 const per_token = n_q + 2 * n_kv;   // heads: queries, keys, values
+	u32 const unit = blockIdx.x * append_cfg::WARPS + (threadIdx.x >> 5);
+	u32 const token = unit / p.parts, part = unit - token * p.parts;
+	if (token >= p.tokens) return;
 	i32 const seq = p.seqs[token], pos = p.positions[token];
-	if (seq < 0) return;
+	// the lane's two runs of 16 dims
+	bool const turns = chunk < p.rotary / 32;
+	u32 const off0 = turns && !ADJACENT ? chunk * 16 : chunk * 32;
+	u32 const off1 = turns && !ADJACENT ? p.rotary / 2 + chunk * 16 : chunk * 32 + 16;
+
+	u32 const rounds = (per_token + HEADS - 1) / HEADS, each = (rounds + p.parts - 1) / p.parts;
+	u32 const from = part * each, to = min(from + each, rounds);
+	u8 const *const q_row = static_cast<u8 const *>(p.q) + u64(token) * p.q_stride * SIZE;
+	u8 const *const kv_row = static_cast<u8 const *>(p.kv) + u64(token) * p.kv_stride * SIZE;
+	auto load = [&](u32 round, AppendRow<SCALED> &row) {
+		u32 const h = round * HEADS + lane / C;
+		if (round >= to || h >= per_token) return;
+		u32 const kv = h - n_q;   // keys, then values
+		u8 const *src = h < n_q ? q_row + h * D * SIZE : kv < n_kv ? kv_row + kv * 2 * D * SIZE : kv_row + ((kv - n_kv) * 2 + 1) * D * SIZE;
+#pragma unroll
+		for (u32 i = 0; i < SIZE; ++i) {
+			row.lo[i] = reinterpret_cast<uint4 const *>(src + off0 * SIZE)[i];
+			row.hi[i] = reinterpret_cast<uint4 const *>(src + off1 * SIZE)[i];
+		}
+	};
+	AppendRow<SCALED> row, next;
+	load(from, row);
+	load(from + 1, next);
+	if (seq < 0) return;   // padding
 	u32 page = 0, slot = 0;
 	if (!paged_slot(p.pool, seq, pos, page, slot) || (p.rotary != 0 && u32(pos) >= p.rope_rows)) {
-		if (lane == 0) report_status(p.status, ST_BAD_INDEX, token);
+		if (lane == 0 && part == 0) report_status(p.status, ST_BAD_INDEX, token);
 		return;
 	}
-	bool const is_q = head < n_q;
-	u32 const kvh = is_q ? 0u : (head - n_q) / 2;
-	bool const is_v = !is_q && ((head - n_q) & 1);
-	u64 const src = is_q ? token * p.q_stride + head * D : token * p.kv_stride + (u64(kvh) * 2 + is_v) * D;
-	auto load = [&](u32 d) -> f32 {
-		void const *base = is_q ? p.q : p.kv;
-		if constexpr (SCALED) return __uint_as_float(u32(static_cast<u16 const *>(base)[src + d]) << 16);
-		else return f32(static_cast<i8 const *>(base)[src + d]);
-	};
-	u32 const half = p.rotary / 2;
-	f32 val[V];
-	f32 top = 0.0f;
+	// cos | sin of the lane's 16 pairs
+	__align__(16) u32 cs[16];
+	if (turns) {
+		uint4 const *src = reinterpret_cast<uint4 const *>(p.rope + (u64(u32(pos)) * (p.rotary / 2) + chunk * 16) * 2);
 #pragma unroll
-	for (u32 j = 0; j < V; ++j) {
-		u32 const d = j * 32 + lane;
-		val[j] = load(d);
-		if (!is_v && d < p.rotary) {
-			u32 const pair = p.adjacent ? d / 2 : d % half;
-			bool const second = p.adjacent ? d & 1 : d >= half;
-			f32 const other = load(p.adjacent ? d ^ 1u : second ? d - half : d + half);
-			int16_t const *cs = p.rope + (u64(u32(pos)) * half + pair) * 2;
-			if constexpr (SCALED) {
-				f32 const c = f32(cs[0]) * 0x1p-14f, s = f32(cs[1]) * 0x1p-14f;
-				val[j] = second ? __fmaf_rn(other, s, __fmul_rn(val[j], c)) : __fmaf_rn(val[j], c, -__fmul_rn(other, s));
-			} else {
-				i32 const x = i32(val[j]), y = i32(other);
-				i32 const acc = second ? y * cs[1] + x * cs[0] : x * cs[0] - y * cs[1];
-				val[j] = f32(max(-127, min(127, (acc + 8192) >> 14)));
+		for (u32 i = 0; i < 4; ++i) *reinterpret_cast<uint4 *>(cs + 4 * i) = src[i];
+	}
+	u64 const slot_row = p.pool.row(page, 0, slot);
+
+	for (u32 round = from; round < to; ++round) {
+		AppendRow<SCALED> const now = row;
+		row = next;
+		load(round + 2, next);
+		u32 const h = round * HEADS + lane / C;
+		bool const live = h < per_token, is_q = h < n_q, is_v = !is_q && h - n_q >= n_kv;
+		u32 const kv_head = is_q ? 0u : is_v ? h - n_q - n_kv : h - n_q;
+		bool const turn = turns && !is_v;
+		__align__(16) u32 lo[4], hi[4];
+		if constexpr (!SCALED) {
+			*reinterpret_cast<uint4 *>(lo) = now.lo[0];
+			*reinterpret_cast<uint4 *>(hi) = now.hi[0];
+			if (turn) {
+				// word w of eight: pairs 2 w, 2 w + 1 as bytes x y x y
+				auto pairs = [&](u32 w) -> u32 {
+					if constexpr (ADJACENT) return w < 4 ? lo[w] : hi[w - 4];
+					return __byte_perm(lo[w / 2], hi[w / 2], w % 2 == 0 ? 0x5140 : 0x7362);
+				};
+				i32 x[16], y[16];
+#pragma unroll
+				for (u32 w = 0; w < 8; ++w) {
+					u32 const b = pairs(w);
+#pragma unroll
+					for (u32 e = 0; e < 2; ++e) {
+						u32 const c = cs[2 * w + e];
+						u32 const minus = (c & 0xFFFFu) | (0u - (c & 0xFFFF0000u)), swapped = __byte_perm(c, c, 0x1032);   // (cos, -sin), (sin, cos)
+						x[2 * w + e] = e == 0 ? dp2a_s16_s8<0>(minus, b, 8192) : dp2a_s16_s8<1>(minus, b, 8192);
+						y[2 * w + e] = e == 0 ? dp2a_s16_s8<0>(swapped, b, 8192) : dp2a_s16_s8<1>(swapped, b, 8192);
+					}
+				}
+#pragma unroll
+				for (u32 w = 0; w < 4; ++w) {
+					if constexpr (ADJACENT) {
+						lo[w] = pack4_turned(x[2 * w], y[2 * w], x[2 * w + 1], y[2 * w + 1]);
+						hi[w] = pack4_turned(x[2 * w + 8], y[2 * w + 8], x[2 * w + 9], y[2 * w + 9]);
+					} else {
+						lo[w] = pack4_turned(x[4 * w], x[4 * w + 1], x[4 * w + 2], x[4 * w + 3]);
+						hi[w] = pack4_turned(y[4 * w], y[4 * w + 1], y[4 * w + 2], y[4 * w + 3]);
+					}
+				}
+			}
+		} else {
+			f32 v[32];
+#pragma unroll
+			for (u32 i = 0; i < 2; ++i) {
+				u32 const a[4] = {now.lo[i].x, now.lo[i].y, now.lo[i].z, now.lo[i].w}, c[4] = {now.hi[i].x, now.hi[i].y, now.hi[i].z, now.hi[i].w};
+#pragma unroll
+				for (u32 w = 0; w < 4; ++w) {
+					v[8 * i + 2 * w] = __uint_as_float(a[w] << 16);
+					v[8 * i + 2 * w + 1] = __uint_as_float(a[w] & 0xFFFF0000u);
+					v[16 + 8 * i + 2 * w] = __uint_as_float(c[w] << 16);
+					v[16 + 8 * i + 2 * w + 1] = __uint_as_float(c[w] & 0xFFFF0000u);
+				}
+			}
+			if (turn) {
+#pragma unroll
+				for (u32 j = 0; j < 16; ++j) {
+					u32 const at_x = ADJACENT ? 2 * j : j, at_y = ADJACENT ? 2 * j + 1 : 16 + j;
+					f32 const c = f32(i32(cs[j] << 16) >> 16) * 0x1p-14f, sn = f32(i32(cs[j]) >> 16) * 0x1p-14f;
+					f32 const x = v[at_x], y = v[at_y];
+					v[at_x] = __fmaf_rn(x, c, -__fmul_rn(y, sn));
+					v[at_y] = __fmaf_rn(x, sn, __fmul_rn(y, c));
+				}
+			}
+			f32 top = 0.0f;
+#pragma unroll
+			for (u32 j = 0; j < 32; ++j) top = fmaxf(top, fabsf(v[j]));
+#pragma unroll
+			for (u32 mask = 1; mask < C; mask <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, mask));
+			bool const some = top > PAGED_TINY;
+			f32 const inv = some ? __fdiv_rn(127.0f, top) : 0.0f;
+			if (chunk == 0 && live) {
+				f32 const scale = some ? __fmul_rn(top, 1.0f / 127.0f) : 0.0f;
+				if (is_q) p.q_scale[u64(token) * p.n_heads + h] = scale;
+				else p.pool.scales[(slot_row + (u64(kv_head) << p.pool.page_shift)) * 2 + is_v] = scale;
+			}
+			// (not the packed forms: product and sum of those become one operation, and a value on a tie another code)
+			auto code = [&](f32 x) { return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.0f)); };
+#pragma unroll
+			for (u32 w = 0; w < 8; ++w) {
+				u32 const word = __byte_perm(__byte_perm(code(v[4 * w]), code(v[4 * w + 1]), 0x0040),
+											 __byte_perm(code(v[4 * w + 2]), code(v[4 * w + 3]), 0x0040), 0x5410);
+				if (w < 4) lo[w] = word;
+				else hi[w - 4] = word;
 			}
 		}
-		top = fmaxf(top, fabsf(val[j]));
-	}
-	f32 inv = 1.0f;
-	f32 scale = 0.0f;
-	if constexpr (SCALED) {
-#pragma unroll
-		for (u32 mask = 16; mask > 0; mask >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, mask));
-		bool const live = top > PAGED_TINY;
-		inv = live ? __fdiv_rn(127.0f, top) : 0.0f;
-		scale = live ? __fmul_rn(top, 1.0f / 127.0f) : 0.0f;
-		if (lane == 0) {
-			if (is_q) p.q_scale[u64(token) * p.n_heads + head] = scale;
-			else p.pool.scales[p.pool.row(page, kvh, slot) * 2 + is_v] = scale;
-		}
-	}
-#pragma unroll
-	for (u32 j = 0; j < V; ++j) {
-		u32 const d = j * 32 + lane;
-		i8 const code = SCALED ? i8(f32_to_fixedi8(__fmul_rn(val[j], inv))) : i8(i32(val[j]));
+		if (!live) continue;
+		auto store = [&](i8 *dst) {
+			*reinterpret_cast<uint4 *>(dst + off0) = *reinterpret_cast<uint4 const *>(lo);
+			*reinterpret_cast<uint4 *>(dst + off1) = *reinterpret_cast<uint4 const *>(hi);
+		};
 		if (is_q) {
-			p.q_out[token * p.q_stride + head * D + d] = code;
+			store(p.q_out + u64(token) * p.q_stride + h * D);
 		} else {
-			p.pool.pages[p.pool.row(page, kvh, slot) * 2 * D + is_v * D + d] = code;
-			if (p.kv_out != nullptr) p.kv_out[src + d] = code;
+			store(p.pool.pages + (slot_row + (u64(kv_head) << p.pool.page_shift)) * 2 * D + is_v * D);
+			if (p.kv_out != nullptr) store(p.kv_out + u64(token) * p.kv_stride + (kv_head * 2 + is_v) * D);
 		}
 	}
 }
