@@ -145,6 +145,18 @@ def test_decode_scaled_refuses(lib, kw, text):
         K.PagedAttnKernel(_config()).decode_scaled(_Stream(), **{**args, **kw})
 
 
+def test_tensors_without_storage_raise(lib):
+    """Regular arguments whose memory cannot be read: the native launch path gives them back, the Python path raises."""
+    from x17ai_b200 import kernels as K
+    kern = K.PagedAttnKernel(_config())
+    scales, bf16 = dict(page_scales=_c(F32, 9, 2, 16, 2)), dict(q=_c(BF16, 5, 512), kv=_c(BF16, 5, 256), q_scale=_c(F32, 5, 8))
+    for call in (lambda: kern.append(_Stream(), **_append_args()), lambda: kern.append_scaled(_Stream(), **_append_args(**scales, **bf16)),
+                 lambda: kern.decode(_Stream(), **_decode_args()),
+                 lambda: kern.decode_scaled(_Stream(), **_decode_args(**scales, q_scale=_c(F32, 6, 8)))):
+        with pytest.raises(RuntimeError):
+            call()
+
+
 def _entry(lib, name, **kw):
     """A C entry point with plausible addresses (never read: every refusal comes before the device is entered)."""
     from x17ai_b200 import _lib

@@ -26,7 +26,11 @@ namespace {
 	X(x17ai_b200_attn_decode_i8_noalloc) \
 	X(x17ai_b200_gemm_fwd)           \
 	X(x17ai_b200_qkvg_fwd_i8)        \
-	X(x17ai_b200_rms_norm)
+	X(x17ai_b200_rms_norm)           \
+	X(x17ai_b200_paged_append)       \
+	X(x17ai_b200_paged_append_scaled) \
+	X(x17ai_b200_paged_decode)       \
+	X(x17ai_b200_paged_decode_scaled)
 
 #define X17_DECL(name) decltype(&name) p_##name = nullptr;
 X17_ENTRIES(X17_DECL)
@@ -36,7 +40,7 @@ using at::Tensor;
 
 constexpr int64_t ANY = -1;
 
-enum Kind { I8, E4M3, BF16, F32, I32_OUT, U32_IN };
+enum Kind { I8, E4M3, BF16, F32, I32_OUT, U32_IN, I16 };
 
 bool dtype_is(Tensor const &t, Kind k) {
 	switch (t.scalar_type()) {
@@ -46,6 +50,7 @@ bool dtype_is(Tensor const &t, Kind k) {
 	case at::kBFloat16: return k == BF16;
 	case at::kFloat: return k == F32;
 	case at::kInt: return k == I32_OUT || k == U32_IN;
+	case at::kShort: return k == I16;
 	case at::kUInt32: return k == U32_IN;
 	default: return false;
 	}
@@ -290,6 +295,109 @@ PyObject *rms_norm(PyObject *, PyObject *const *v, Py_ssize_t n) {
 	});
 }
 
+// The pages, their scales and the page table of a paged cache; false where one is irregular.
+struct PagedArgs {
+	x17ai_PagedConfig const *c = nullptr;
+	x17ai_CudaStreamHandle *stream = nullptr;
+	size_t n_pages = 0, n_seqs = 0, max_pages = 0;
+	bool read(PyObject *cfg, PyObject *st, Arg const &pages, Arg const *scales, Arg const &table) {
+		c = to_config<x17ai_PagedConfig>(cfg);
+		stream = to_stream(st);
+		if (c == nullptr || stream == nullptr || !pages.ok || pages.t->dim() != 4 || !dtype_is(*pages.t, I8)) return false;
+		int64_t const heads = int64_t(c->n_kv_heads), size = int64_t(c->page_size), n = pages.t->size(0);
+		if (pages.t->size(1) != heads || pages.t->size(2) != size || pages.t->size(3) != int64_t(2 * c->head_dim)) return false;
+		if (scales != nullptr) {
+			if (!scales->ok || scales->t->dim() != 4 || !dtype_is(*scales->t, F32)) return false;
+			if (scales->t->size(0) != n || scales->t->size(1) != heads || scales->t->size(2) != size || scales->t->size(3) != 2) return false;
+		}
+		if (!table.is2(ANY, ANY, I32_OUT)) return false;
+		n_pages = size_t(n);
+		n_seqs = size_t(table.t->size(0));
+		max_pages = size_t(table.t->size(1));
+		return true;
+	}
+};
+
+// paged_append(config, stream, q, kv, seqs, positions, page_table, pages, q_out, rope, kv_out)
+// paged_append_scaled(config, stream, q, kv, seqs, positions, page_table, pages, page_scales, q_out, q_scale, rope)
+template <bool SCALED>
+PyObject *paged_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
+	if (n != (SCALED ? 12 : 11)) Py_RETURN_FALSE;
+	Arg q(a[2], true), kv(a[3]), seqs(a[4]), pos(a[5]), table(a[6]), pages(a[7]), scales(a[8], !SCALED), q_out(a[SCALED ? 9 : 8], true),
+		q_scale(a[10], true), rope(a[SCALED ? 11 : 9], true), kv_out(a[10], true);
+	PagedArgs s;
+	constexpr Kind in = SCALED ? BF16 : I8;
+	if (!s.read(a[0], a[1], pages, SCALED ? &scales : nullptr, table) || !q.ok || !q_out.ok || !rope.ok || !(SCALED ? q_scale : kv_out).ok
+		|| !kv.is2(ANY, int64_t(s.c->kv_stride), in)) {
+		Py_RETURN_FALSE;
+	}
+	int64_t const tokens = kv.t->size(0);
+	if (!seqs.is_vec(tokens, I32_OUT) || !pos.is_vec(tokens, I32_OUT) || q.none() != q_out.none()) Py_RETURN_FALSE;
+	if (!q.none() && (!q.is2(tokens, int64_t(s.c->q_stride), in) || !q_out.is2(tokens, int64_t(s.c->q_stride), I8))) Py_RETURN_FALSE;
+	if (SCALED ? q_scale.none() != q.none() || (!q_scale.none() && !q_scale.is2(tokens, int64_t(s.c->n_heads), F32))
+			   : !kv_out.none() && !kv_out.is2(tokens, int64_t(s.c->kv_stride), I8)) {
+		Py_RETURN_FALSE;
+	}
+	if (rope.none() != (s.c->rotary_dim == 0)) Py_RETURN_FALSE;
+	if (!rope.none() && !(rope.t->dim() == 3 && rope.t->size(1) == int64_t(s.c->rotary_dim / 2) && rope.t->size(2) == 2 && dtype_is(*rope.t, I16))) {
+		Py_RETURN_FALSE;
+	}
+	size_t const rope_rows = rope.none() ? 0 : size_t(rope.t->size(0));
+	return launch([&] {
+		if constexpr (SCALED) {
+			return p_x17ai_b200_paged_append_scaled(s.stream, s.c, (uint16_t const *)q.ptr(), (uint16_t const *)kv.ptr(), size_t(tokens),
+													(int32_t const *)seqs.ptr(), (int32_t const *)pos.ptr(), (int32_t const *)table.ptr(), s.n_seqs,
+													s.max_pages, (int16_t const *)rope.ptr(), rope_rows, (int8_t *)pages.ptr(), (float *)scales.ptr(),
+													s.n_pages, (int8_t *)q_out.ptr(), (float *)q_scale.ptr());
+		} else {
+			return p_x17ai_b200_paged_append(s.stream, s.c, (int8_t const *)q.ptr(), (int8_t const *)kv.ptr(), size_t(tokens),
+											 (int32_t const *)seqs.ptr(), (int32_t const *)pos.ptr(), (int32_t const *)table.ptr(), s.n_seqs,
+											 s.max_pages, (int16_t const *)rope.ptr(), rope_rows, (int8_t *)pages.ptr(), s.n_pages,
+											 (int8_t *)q_out.ptr(), (int8_t *)kv_out.ptr());
+		}
+	});
+}
+
+// paged_decode(config, stream, q, pages, page_table, kv_lens, sink_k, sink_v, temperature, out, l, window, scratch)
+// paged_decode_scaled(config, stream, q, q_scale, pages, page_scales, page_table, kv_lens, ... the same)
+template <bool SCALED>
+PyObject *paged_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
+	if (n != (SCALED ? 15 : 13)) Py_RETURN_FALSE;
+	PyObject *const *r = a + (SCALED ? 6 : 4);   // from the page table on
+	Arg q(a[2]), q_scale(a[3], !SCALED), pages(a[SCALED ? 4 : 3]), scales(a[5], !SCALED), table(r[0]), lens(r[1]), sk(r[2]), sv(r[3]), temp(r[4]),
+		out(r[5]), l(r[6], true), scratch(r[8], true);
+	PagedArgs s;
+	size_t window;
+	if (!s.read(a[0], a[1], pages, SCALED ? &scales : nullptr, table) || !lens.ok || !l.ok || !scratch.ok || !to_size(r[7], window)
+		|| !q.is2(ANY, int64_t(s.c->q_stride), I8) || !out.ok) {
+		Py_RETURN_FALSE;
+	}
+	int64_t const rows = q.t->size(0), batch = int64_t(s.n_seqs), heads = int64_t(s.c->n_heads), hd = int64_t(s.c->head_dim);
+	bool const bf16 = dtype_is(*out.t, BF16);
+	if (rows % batch != 0 || lens.t->dim() != 1 || lens.t->size(0) != batch || !dtype_is(*lens.t, I32_OUT) || !sk.is2(heads, hd, I8)
+		|| !sv.is2(heads, hd, I8) || !temp.is_vec(heads, F32) || !out.is2(rows, int64_t(s.c->o_stride), SCALED || bf16 ? BF16 : I8)
+		|| (!l.none() && !l.is2(rows, heads, F32)) || (SCALED && !q_scale.is2(rows, heads, F32))
+		|| (!scratch.none() && !(scratch.t->dim() == 1 && scratch.t->scalar_type() == at::kByte))) {
+		Py_RETURN_FALSE;
+	}
+	size_t const scratch_bytes = scratch.none() ? 0 : size_t(scratch.t->numel());
+	return launch([&] {
+		if constexpr (SCALED) {
+			return p_x17ai_b200_paged_decode_scaled(s.stream, s.c, size_t(batch), size_t(rows / batch), (int8_t const *)q.ptr(),
+													(float const *)q_scale.ptr(), (int8_t const *)pages.ptr(), (float const *)scales.ptr(), s.n_pages,
+													(int32_t const *)table.ptr(), s.max_pages, (int32_t const *)lens.ptr(), (int8_t const *)sk.ptr(),
+													(int8_t const *)sv.ptr(), (float const *)temp.ptr(), (uint16_t *)out.ptr(), (float *)l.ptr(), window,
+													scratch.ptr(), scratch_bytes);
+		} else {
+			return p_x17ai_b200_paged_decode(s.stream, s.c, size_t(batch), size_t(rows / batch), (int8_t const *)q.ptr(),
+											 (int8_t const *)pages.ptr(), s.n_pages, (int32_t const *)table.ptr(), s.max_pages,
+											 (int32_t const *)lens.ptr(), (int8_t const *)sk.ptr(), (int8_t const *)sv.ptr(), (float const *)temp.ptr(),
+											 out.ptr(), bf16 ? X17AI_DTYPE_BF16 : X17AI_DTYPE_INT8, (float *)l.ptr(), window, scratch.ptr(),
+											 scratch_bytes);
+		}
+	});
+}
+
 // init({name: address}): the entry points of the loaded library
 PyObject *init(PyObject *, PyObject *addresses) {
 	if (!PyDict_Check(addresses)) {
@@ -323,7 +431,8 @@ PyObject *guarded(PyObject *self, PyObject *const *a, Py_ssize_t n) noexcept {
 	Py_RETURN_FALSE;
 }
 
-#define X17_FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<name>)), METH_FASTCALL, nullptr}
+#define X17_FAST_AS(name, ...) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<__VA_ARGS__>)), METH_FASTCALL, nullptr}
+#define X17_FAST(name) X17_FAST_AS(#name, name)
 PyMethodDef methods[] = {
 	{"init", init, METH_O, nullptr},
 	{"entries", [](PyObject *, PyObject *) -> PyObject * {
@@ -341,6 +450,10 @@ PyMethodDef methods[] = {
 	X17_FAST(gemm),
 	X17_FAST(qkvg),
 	X17_FAST(rms_norm),
+	X17_FAST_AS("paged_append", paged_append<false>),
+	X17_FAST_AS("paged_append_scaled", paged_append<true>),
+	X17_FAST_AS("paged_decode", paged_decode<false>),
+	X17_FAST_AS("paged_decode_scaled", paged_decode<true>),
 	{nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_hostcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -402,6 +402,7 @@ class PagedAttnKernel(_Configured):
     def __init__(self, config: PagedConfig):
         self.config = config
         self._lib = _lib.load()
+        self._native = _lib.hostcall()
         cfg = self._c_config[1]
         check(self._lib.x17ai_b200_paged_check_config(ctypes.byref(cfg)))
 
@@ -456,6 +457,9 @@ class PagedAttnKernel(_Configured):
         to position positions[t] of sequence seqs[t], keys rotated; the queries `q` [tokens, q_stride] are rotated into `q_out`
         (both None: keys and values alone). `kv_out`: the rows as stored, for the prefill attention of the same tokens. A
         negative sequence marks a row of padding. Two tokens of a call must not share a place; outputs must not overlap inputs."""
+        held = self._c_config   # the C form lives as long as the call
+        if _launched(self._native.paged_append(held[2], stream.handle, q, kv, seqs, positions, page_table, pages, q_out, rope, kv_out)):
+            return
         tokens, n_seqs, max_pages, n_pages = self._append_shapes(
             "paged append", q, kv, seqs, positions, page_table, pages, None, q_out, None, rope, kv_out, DTYPE_INT8)
         cfg = self.config._c()
@@ -466,6 +470,10 @@ class PagedAttnKernel(_Configured):
     def append_scaled(self, stream, q, kv, seqs, positions, page_table, pages, page_scales, q_out, q_scale, rope=None):
         """The same from bf16 rows, rotated in f32 and quantised with one scale per token and head (absmax / 127): codes into
         `pages`, scales into `page_scales`, queries into `q_out` int8 and `q_scale` f32 [tokens, n_heads]."""
+        held = self._c_config   # the C form lives as long as the call
+        if _launched(self._native.paged_append_scaled(held[2], stream.handle, q, kv, seqs, positions, page_table, pages, page_scales, q_out,
+                                                      q_scale, rope)):
+            return
         op = "paged append"
         tokens, n_seqs, max_pages, n_pages = self._append_shapes(
             op, q, kv, seqs, positions, page_table, pages, page_scales, q_out, q_scale, rope, None, DTYPE_BF16)
@@ -518,6 +526,10 @@ class PagedAttnKernel(_Configured):
         0 = all) and the sink, as AttnKernel.decode does. `out` [rows, o_stride] int8 (FixedI8) or bf16; `l` [rows, n_heads].
         A sequence of length 0 sees the sink alone (a row of padding costs no more). `scratch`: memory from scratch() for this
         call's shape, used by one call at a time; without it the call takes its own from the library's pool, in stream order."""
+        held = self._c_config   # the C form lives as long as the call
+        if _launched(self._native.paged_decode(held[2], stream.handle, q, pages, page_table, kv_lens, sink_k, sink_v, attn_temperature, out, l,
+                                               window_size, scratch)):
+            return
         out_dtype = DTYPE_BF16 if out.dtype == torch.bfloat16 else DTYPE_INT8
         batch, n, n_pages, max_pages = self._decode_shapes(
             q, pages, None, page_table, kv_lens, sink_k, sink_v, attn_temperature, out, l, out_dtype)
@@ -530,6 +542,10 @@ class PagedAttnKernel(_Configured):
     def decode_scaled(self, stream, q, q_scale, pages, page_scales, page_table, kv_lens, sink_k, sink_v, attn_temperature, out,
                       l=None, window_size=0, scratch=None):
         """The same over a cache with scales: `q_scale` f32 [rows, n_heads], `out` bf16."""
+        held = self._c_config   # the C form lives as long as the call
+        if _launched(self._native.paged_decode_scaled(held[2], stream.handle, q, q_scale, pages, page_scales, page_table, kv_lens, sink_k,
+                                                      sink_v, attn_temperature, out, l, window_size, scratch)):
+            return
         batch, n, n_pages, max_pages = self._decode_shapes(
             q, pages, page_scales, page_table, kv_lens, sink_k, sink_v, attn_temperature, out, l, DTYPE_BF16)
         matrix_shape("paged decode", "q_scale", q_scale, (batch * n, self.config.n_heads), DTYPE_F32)
