@@ -284,7 +284,7 @@ DECODES = [
 
 @pytest.mark.parametrize("H,Hk,D,page,lens,new,window", DECODES)
 @pytest.mark.parametrize("kind", ["bf16", "fixed", "scaled"])
-@pytest.mark.parametrize("room", [0, 80000])
+@pytest.mark.parametrize("room", [0, 300000])
 def test_decode(stream, kind, H, Hk, D, page, lens, new, window, room):
     """With room for few keys a sequence has CTAs of its own, with room for many all sequences share the chip's (a window
     counts as room)."""
@@ -312,7 +312,7 @@ def test_scratch_that_is_too_small(stream):
     H, D, page = 4, 64, 16
     kern = _kernel(H, H, D, page)
     z = lambda dtype, *shape: torch.zeros(shape, dtype=dtype, device="cuda")
-    args = (z(torch.int8, 2, H * D), kern.pages(4), z(torch.int32, 2, 5000), z(torch.int32, 2), z(torch.int8, H, D), z(torch.int8, H, D),
+    args = (z(torch.int8, 2, H * D), kern.pages(4), z(torch.int32, 2, 20000), z(torch.int32, 2), z(torch.int8, H, D), z(torch.int8, H, D),
             z(torch.float32, H), z(torch.bfloat16, 2, H * D))
     scratch = kern.scratch(stream, 2)
     torch.cuda.synchronize()
@@ -372,7 +372,7 @@ def test_decode_lengths_beyond_the_table(stream):
 
 
 @pytest.mark.parametrize("scaled", [False, True])
-@pytest.mark.parametrize("room", [0, 80000])
+@pytest.mark.parametrize("room", [0, 300000])
 def test_decode_leaves_out_bad_pages(scaled, room):
     """A key on a page outside the pool is not attended to; the status words say so."""
     from x17ai_b200 import device
@@ -529,7 +529,7 @@ def test_drafted_tokens_equal_single_steps(stream):
             assert (l[i::new] - one_l).abs().max() <= 1e-4
 
 
-@pytest.mark.parametrize("room,kernels", [(0, 2), (80000, 3)])
+@pytest.mark.parametrize("room,kernels", [(0, 2), (300000, 3)])
 def test_captured_and_replayed(room, kernels):
     """A step recorded once and replayed with other positions, lengths and rows in the same buffers; two graphs at once on two
     streams, which share the pool and write different pages."""
@@ -583,7 +583,7 @@ def test_captured_and_replayed(room, kernels):
         s.close()
 
 
-@pytest.mark.parametrize("room", [0, 80000])
+@pytest.mark.parametrize("room", [0, 300000])
 def test_reads_what_torch_wrote_in_front(room):
     """Inputs written by torch on the same stream right in front of the calls, changing from pass to pass, nothing waited for."""
     from x17ai_b200 import device, kernels as K

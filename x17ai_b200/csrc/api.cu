@@ -969,7 +969,7 @@ cudaError_t scratch_pool(StreamScope const &on, cudaMemPool_t *pool) {
 constexpr size_t ANY_KEYS = size_t(1) << 31;   // of a sequence: what scratch memory has to suffice for
 // How a call's rows are dealt out, and what its parts need.
 struct PagedPlan {
-	uint32_t chunk_rows, chunks, tiles, sm_warps, first_ctas, ctas;   // ctas: of the list
+	uint32_t chunk_rows, chunks, tiles, step, sm_warps, first_ctas, ctas;   // step: its keys; ctas: of the list
 	size_t n_x, ms_bytes, o_bytes, bytes;   // bytes: [o][ms][shared_by]
 };
 PagedPlan paged_plan(x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, size_t keys, int sm_count) {
@@ -981,11 +981,12 @@ PagedPlan paged_plan(x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens
 	plan.chunk_rows = uint32_t((rows + most - 1) / most);
 	plan.chunks = uint32_t((rows + plan.chunk_rows - 1) / plan.chunk_rows);
 	plan.tiles = plan.chunk_rows > ROWS ? 2 : 1;
+	plan.step = uint32_t(KS * (128 / cfg->head_dim));
 	plan.n_x = cfg->n_kv_heads * plan.chunks;
 	static_assert(SM_WARPS<64, 2> == SM_WARPS<128, 1> && SM_WARPS<32, 2> == SM_WARPS<128, 1>);
 	plan.sm_warps = cfg->head_dim == 128 && plan.tiles == 2 ? SM_WARPS<128, 2> : SM_WARPS<128, 1>;
 	plan.first_ctas = uint32_t(sm_count) * (plan.sm_warps / WARPS);
-	plan.ctas = batch * plan.n_x * (keys / KS + 1) / (plan.first_ctas * WARPS) >= LONG_RUN ? plan.first_ctas * MORE_CTAS : plan.first_ctas;
+	plan.ctas = batch * plan.n_x * (keys / plan.step + 1) / (plan.first_ctas * WARPS) >= LONG_RUN ? plan.first_ctas * MORE_CTAS : plan.first_ctas;
 	size_t const slots = size_t(plan.ctas) * (WARPS + 2) * plan.chunk_rows;
 	plan.ms_bytes = slots * sizeof(float4);
 	plan.o_bytes = slots * cfg->head_dim * sizeof(float);
@@ -1000,18 +1001,19 @@ struct PagedPlaces {
 };
 PagedPlaces paged_places(PagedPlan const &plan, size_t pairs, size_t keys, int sm_count) {
 	using namespace x17::paged_cfg;
-	size_t const steps = (keys + KS - 1) / KS;
+	size_t const steps = (keys + plan.step - 1) / plan.step;
 	size_t const each = (pairs + sm_count - 1) / sm_count;   // CTAs on an SM
-	if (each * WARPS > plan.sm_warps) return {0, WARPS};
+	if (each > plan.sm_warps) return {0, WARPS};
 	size_t warps = plan.sm_warps / each, splits = 1;
-	if (each == 1) splits = size_t(sm_count) / pairs;
-	if (splits > MAX_SPLITS) splits = MAX_SPLITS;
-	// no more of either than there are steps
-	if (splits * warps > steps) splits = (steps + warps - 1) / warps;
-	if (splits * warps > steps + warps) warps = steps / splits + 1;
-	if (warps < WARPS) warps = WARPS;
-	if (splits == 0) splits = 1;
-	return {steps <= 9 * splits * warps ? uint32_t(splits) : 0, uint32_t(warps)};
+	if (each == 1) {
+		splits = size_t(sm_count) / pairs;
+		if (splits > MAX_SPLITS) splits = MAX_SPLITS;
+		if (splits * warps > steps) splits = (steps + warps - 1) / warps;   // (no more than there are steps)
+		if (splits == 0) splits = 1;
+	}
+	// a warp's steps, against those that the list would give it
+	size_t const mine = (steps + splits * warps - 1) / (splits * warps), shared = pairs * steps / (size_t(sm_count) * plan.sm_warps);
+	return {mine <= MOST_STEPS && mine <= shared + 5 ? uint32_t(splits) : 0, uint32_t(warps)};
 }
 
 x17ai_DiagnosticBuffer *check_paged_decode(x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, char const *who) {
@@ -1066,7 +1068,7 @@ x17ai_DiagnosticBuffer *paged_decode(char const *who, x17ai_CudaStreamHandle *st
 	size_t const capacity = max_pages * cfg->page_size;
 	size_t const keys = p.window < capacity ? p.window + n_tokens + 15 : capacity;   // at most, of a sequence
 	PagedPlan const plan = paged_plan(cfg, batch, n_tokens, keys, scope.state().sm_count);
-	if (batch * plan.n_x * (keys / x17::paged_cfg::KS + 2) >= (size_t(1) << 31)) {
+	if (batch * plan.n_x * (keys / plan.step + 2) >= (size_t(1) << 31)) {
 		return make_diag("x17ai_b200: decode shape out of range", who, ": sequences x key heads x keys out of range (room for ", capacity,
 						 " keys in each of ", batch, " sequences)");
 	}

@@ -293,13 +293,19 @@ paged_append_kernel(const PagedAppendParams p) {
 namespace paged_cfg {
 constexpr u32 WARPS = 4;         // of a CTA at least
 constexpr u32 MAX_WARPS = 12;    // of any CTA
-constexpr u32 KS = 32;           // keys of a step: two runs of 16, each in one page
+constexpr u32 KS = 32;           // keys that the products take at once
+// Keys of a step, which is what a warp asks for at once: 8 KB at every width, in runs of 16 keys, each in one page.
+template <u32 D>
+constexpr u32 STEP = KS * (128 / D);
+template <u32 D>
+constexpr u32 RUNS = STEP<D> / 16;
 constexpr u32 STAGES = 2;
 constexpr u32 ROWS = 8;          // of a tile; a warp has one or two
 constexpr u32 LONG_RUN = 100;    // steps of a warp, from which the list is not dealt out equally
 constexpr u32 MORE_CTAS = 3;     // CTAs of the list then, as a multiple of what the chip holds at once
 constexpr f32 SHIFT = 8.0f, ARG_MAX = 14.0f;   // weights are 2^(x - m + SHIFT), at most 2^ARG_MAX (f16 ends below 2^16)
 constexpr u32 MAX_SPLITS = 8;    // CTAs of a cluster
+constexpr u32 MOST_STEPS = 23;   // of a warp, where every (sequence, x) has CTAs of its own
 constexpr u32 MERGE_WARPS = 8;   // of a CTA that joins parts
 // Warps on an SM: 12 with a step in work and a step on its way each, 210 KB of rings. With two tiles at width 128 the sums
 // alone are 64 registers: eight.
@@ -307,10 +313,14 @@ template <u32 D, u32 RT>
 constexpr u32 SM_WARPS = D == 128 && RT == 2 ? 8 : 12;
 template <u32 D, u32 RT>
 constexpr u32 REGS = 65536 / (SM_WARPS<D, RT> * 32) / 8 * 8 - (SM_WARPS<D, RT> == 8 ? 8 : 0);
+// In the ring a key's row [K | V] keeps its 2 D bytes, its 16-byte pieces in places i ^ ring_swap(row): without bank conflicts for the
+// fragments' loads (keys: eight rows, four lanes a row; values: every other row, eight lanes a row; at width 32 values have two).
 template <u32 D>
-constexpr u32 ROW_BYTES = 2 * D + 16;          // of a key in the ring: rows 16 bytes off each other's banks
+__host__ __device__ constexpr u32 ring_swap(u32 row) {
+	return D == 128 ? row & 7 : D == 64 ? ((row ^ row >> 1) & 1) << 2 | (row >> 2 & 1) << 1 : (row >> 1 & 1) << 1;
+}
 template <u32 D, bool SCALED>
-constexpr u32 STAGE_BYTES = KS * (ROW_BYTES<D> + (SCALED ? 8 : 0));
+constexpr u32 STAGE_BYTES = STEP<D> * (2 * D + (SCALED ? 8 : 0));
 template <u32 D, bool SCALED>
 constexpr u32 RING_BYTES = STAGES * STAGE_BYTES<D, SCALED>;   // of a warp
 }  // namespace paged_cfg
@@ -409,6 +419,7 @@ X17_DEV void ld_global_words(i8 const *p, u32 (&w)[N]) {
 }
 
 // What a sequence's rows see: token i has position n = length(i) and keys [first(n), n).
+template <u32 STEP>
 struct PagedSpan {
 	u32 len, capacity, window;
 	X17_DEV PagedSpan(PagedDecodeParams const &p, i32 kv_len)
@@ -417,7 +428,7 @@ struct PagedSpan {
 	X17_DEV u32 first(u32 n) const { return n - min(n, window); }
 	X17_DEV u32 base() const { return first(length(0)) & ~15u; }   // of the sequence's steps
 	// one at least: a sequence without keys has its sink
-	X17_DEV u32 steps(u32 n_tokens) const { return max(1u, (length(n_tokens - 1) - base() + paged_cfg::KS - 1) / paged_cfg::KS); }
+	X17_DEV u32 steps(u32 n_tokens) const { return max(1u, (length(n_tokens - 1) - base() + STEP - 1) / STEP); }
 };
 
 // VD dims from d on of one row, from the keys' (m, s, v), m being a maximum less SHIFT, and the sink token.
@@ -511,7 +522,8 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 	constexpr u32 KW = D / 16;                       // words of a key row that a lane holds
 	constexpr u32 VW = D / 32;                       // words of a value row that a lane holds
 	constexpr u32 VD = D / 8;                        // dims of a lane
-	constexpr u32 RB = ROW_BYTES<D>, SB = STAGE_BYTES<D, SCALED>;
+	constexpr u32 RB = 2 * D, SB = STAGE_BYTES<D, SCALED>, S_AT = STEP<D> * RB;   // pitch of a row, of a stage; its scales
+	using Span = PagedSpan<STEP<D>>;
 	constexpr u32 NEG_INF = 0xFF800000u;
 	constexpr f32 ROOT = f32(D == 128 ? 0.08838834764831845 : D == 64 ? 0.125 : 0.17677669529663687);   // D^-1/2
 	extern __shared__ __align__(16) u8 smem[];
@@ -533,7 +545,7 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 	if (p.splits == 0) {
 		pdl_launch_dependents();
 		u32 total = 0;
-		for (u32 i = lane; i < p.pool.n_seqs; i += 32) total += PagedSpan(p, p.kv_lens[i]).steps(p.n_tokens);
+		for (u32 i = lane; i < p.pool.n_seqs; i += 32) total += Span(p, p.kv_lens[i]).steps(p.n_tokens);
 #pragma unroll
 		for (u32 mask = 16; mask > 0; mask >>= 1) total += __shfl_xor_sync(0xffffffffu, total, mask);
 		total *= n_x;   // (below 2^32: checked on the host for sequences of full length)
@@ -545,7 +557,7 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 		u32 before = 0;
 		b = 0;
 		for (u32 target = start / n_x; n_units != 0; b += 32) {
-			u32 const mine = b + lane < p.pool.n_seqs ? PagedSpan(p, p.kv_lens[b + lane]).steps(p.n_tokens) : 0u;
+			u32 const mine = b + lane < p.pool.n_seqs ? Span(p, p.kv_lens[b + lane]).steps(p.n_tokens) : 0u;
 			u32 upto = mine;
 #pragma unroll
 			for (u32 d = 1; d < 32; d <<= 1) {
@@ -561,7 +573,7 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 			}
 			before += __shfl_sync(0xffffffffu, upto, 31);
 		}
-		u32 const steps_of = PagedSpan(p, n_units != 0 ? p.kv_lens[b] : 0).steps(p.n_tokens);
+		u32 const steps_of = Span(p, n_units != 0 ? p.kv_lens[b] : 0).steps(p.n_tokens);
 		x = (start - before * n_x) / steps_of;
 		step = start - before * n_x - x * steps_of;
 	} else {
@@ -570,7 +582,7 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 		// the first pages' entries are brought closer while the length is on its way
 		i32 touch = 0;
 		if (lane * 8 < p.pool.max_pages) asm volatile("ld.global.b32 %0, [%1];" : "=r"(touch) : "l"(p.pool.table + u64(b) * p.pool.max_pages + lane * 8));
-		u32 const all = PagedSpan(p, p.kv_lens[b]).steps(p.n_tokens), each = (all + p.splits - 1) / p.splits;
+		u32 const all = Span(p, p.kv_lens[b]).steps(p.n_tokens), each = (all + p.splits - 1) / p.splits;
 		u32 const from = min(blockIdx.z * each, all), to = min(from + each, all), mine = (to - from + warps - 1) / warps;
 		start = step = min(from + warp * mine, to);
 		n_units = min(start + mine, to) - start;
@@ -578,24 +590,30 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 	u32 left = n_units;
 
 	// ---- the (sequence, x) in work, and the one behind it (whose first step is fetched under the last of this one) ----
-	PagedSpan span(p, n_units != 0 ? p.kv_lens[b] : 0);
+	Span span(p, n_units != 0 ? p.kv_lens[b] : 0);
 	u32 steps = span.steps(p.n_tokens);
 	if (lane < 2) items[warp * 2 + lane] = make_uint2(0, 0);
 	if (lane < RT * ROWS) item_ms[warp][lane] = make_float4(NO_PART, 0.0f, 0.0f, 0.0f);
 	// page table entries of the 32 runs of 16 keys from `run` on, one a lane
-	auto page_entries = [&](PagedSpan const &sp, u32 seq, u32 run) -> u32 {
+	auto page_entries = [&](Span const &sp, u32 seq, u32 run) -> u32 {
 		u32 const key = sp.base() + (run + lane) * 16;
 		return key < sp.length(p.n_tokens - 1) ? u32(p.pool.table[u64(seq) * p.pool.max_pages + (key >> p.pool.page_shift)]) : 0u;
 	};
-	u32 bad = 0;   // bit 2 stage + run: its page is none
+	constexpr u32 PIECES = 2 * D / 16;   // of a row; a warp asks for 32
+	u32 const piece = lane / PIECES * RB + (lane % PIECES ^ ring_swap<D>(lane / PIECES)) * 16;
+	// this lane's bytes of key row g, and of value rows 2 t and 2 t + 1
+	u32 const k_at = g * RB + (t * (D / 4) / 16 ^ ring_swap<D>(g)) * 16 + t * (D / 4) % 16;
+	u32 const v_at[2] = {2 * t * RB + ((D + g * VD) / 16 ^ ring_swap<D>(2 * t)) * 16 + g * VD % 16,
+						 (2 * t + 1) * RB + ((D + g * VD) / 16 ^ ring_swap<D>(2 * t + 1)) * 16 + g * VD % 16};
+	u32 bad = 0;   // bit RUNS stage + run: its page is none
 	// step s of a (sequence, x) into a stage; entries: of the runs from a multiple of 32 on
-	auto issue = [&](PagedSpan const &sp, u32 seq, u32 kvh, u32 s, u32 entries, u32 stage) {
+	auto issue = [&](Span const &sp, u32 seq, u32 kvh, u32 s, u32 entries, u32 stage) {
 		u32 const n_hi = sp.length(p.n_tokens - 1);
 #pragma unroll
-		for (u32 j = 0; j < 2; ++j) {
-			u32 const page = __shfl_sync(0xffffffffu, entries, (s * 2 + j) & 31);
-			u32 const key = sp.base() + s * KS + j * 16;
-			u32 const bit = 1u << (stage * 2 + j);
+		for (u32 j = 0; j < RUNS<D>; ++j) {
+			u32 const page = __shfl_sync(0xffffffffu, entries, (s * RUNS<D> + j) & 31);
+			u32 const key = sp.base() + s * STEP<D> + j * 16;
+			u32 const bit = 1u << (stage * RUNS<D> + j);
 			bad &= ~bit;
 			if (page >= p.pool.n_pages) {
 				bad |= bit;
@@ -604,14 +622,10 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 				u64 const row = p.pool.row(page, kvh, key & ((1u << p.pool.page_shift) - 1));
 				i8 const *src = p.pool.pages + row * 2 * D + lane * 16;
 				u32 const dst = ring + stage * SB + j * 16 * RB;
-				constexpr u32 CHUNKS = 2 * D / 16;   // of a row
 #pragma unroll
-				for (u32 c = 0; c < CHUNKS / 2; ++c) {
-					u32 const at = c * 32 + lane;
-					cp_async_16(dst + at / CHUNKS * RB + at % CHUNKS * 16, src + c * 512);
-				}
+				for (u32 c = 0; c < PIECES / 2; ++c) cp_async_16(dst + c * 512 + (piece ^ ring_swap<D>(c * 32 / PIECES) * 16), src + c * 512);
 				if constexpr (SCALED) {
-					if (lane < 16) cp_async_8(ring + stage * SB + KS * RB + (j * 16 + lane) * 8, p.pool.scales + (row + lane) * 2);
+					if (lane < 16) cp_async_8(ring + stage * SB + S_AT + (j * 16 + lane) * 8, p.pool.scales + (row + lane) * 2);
 				}
 			}
 		}
@@ -619,8 +633,8 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 	};
 	u32 entries = 0, entries_ahead = 0;
 	if (n_units != 0) {
-		entries = page_entries(span, b, step * 2 & ~31u);
-		entries_ahead = page_entries(span, b, (step * 2 & ~31u) + 32);
+		entries = page_entries(span, b, step * RUNS<D> & ~31u);
+		entries_ahead = page_entries(span, b, (step * RUNS<D> & ~31u) + 32);
 	}
 	u32 stage = 0;
 	bool asked = false;   // for the first step
@@ -636,10 +650,10 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 		// the next one
 		bool const b_ends = x + 1 == n_x;
 		u32 const next_b = b_ends ? b + 1 : b, next_x = b_ends ? 0u : x + 1;
-		PagedSpan next_span = span;
+		Span next_span = span;
 		u32 entries_next = 0;
 		if (left != 0) {
-			if (b_ends) next_span = PagedSpan(p, p.kv_lens[next_b]);
+			if (b_ends) next_span = Span(p, p.kv_lens[next_b]);
 			entries_next = page_entries(next_span, next_b, 0);
 		}
 
@@ -690,169 +704,179 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 		}
 		u32 const n_min = span.length(p.group(row0));                                     // what every row sees: [lo_max, n_min)
 		u32 const lo_max = span.first(span.length(p.group(row0 + rows - 1)));
-		u32 key0 = span.base() + step * KS;
+		u32 key0 = span.base() + step * STEP<D>;
+		u32 const n_hi = span.length(p.n_tokens - 1);
 
 #pragma unroll 1
 		for (u32 i = 0; i < n_here; ++i) {
-			u32 const src = ring + stage * SB;
-			u32 const bad_now = bad >> (stage * 2) & 3;
+			u32 src = ring + stage * SB, src_scales = src + S_AT;
+			u32 bad_now = bad >> (stage * RUNS<D>) & ((1u << RUNS<D>) - 1);
 			cp_async_wait<0>();
 			__syncwarp();
 			stage ^= 1;
 			if (i + 1 < n_here) {
 				u32 const s = step + i + 1;
-				if ((s & 15) == 0) {
+				if (s * RUNS<D> % 32 == 0) {
 					entries = entries_ahead;
-					entries_ahead = page_entries(span, b, s * 2 + 32);
+					entries_ahead = page_entries(span, b, s * RUNS<D> + 32);
 				}
 				issue(span, b, kvh, s, entries, stage);
 			} else if (left != 0) {
 				issue(next_span, next_b, p.chunks(next_x), 0, entries_next, stage);
 			}
-			// ---- scores ----
-			f32 arg[KS / 8][RT][2];
-			f32 vs[KS / 8][2];
-#pragma unroll
-			for (u32 n8 = 0; n8 < KS / 8; ++n8) {
-				u32 kw[KW];
-				ld_shared_words(src + (n8 * 8 + g) * RB + t * (D / 4), kw);
-				i32 c[4];
-				mma_s8<true>(c, qa[0], kw[0], kw[1]);
-#pragma unroll
-				for (u32 k = 2; k < KW; k += 2) mma_s8<false>(c, qa[k / 2], kw[k], kw[k + 1]);
-				f32 ks[2] = {1.0f, 1.0f};
-				if constexpr (SCALED) {
-					uint4 const s4 = ld_shared_v4(src + KS * RB + (n8 * 8 + t * 2) * 8);
-					ks[0] = __uint_as_float(s4.x);
-					ks[1] = __uint_as_float(s4.z);
-					vs[n8][0] = __uint_as_float(s4.y);
-					vs[n8][1] = __uint_as_float(s4.w);
-				}
-#pragma unroll
-				for (u32 e = 0; e < 2 * RT; ++e) {
-					f32 const x = SCALED ? f32(c[e]) * ks[e % 2] : f32(c[e]);
-					arg[n8][e / 2][e % 2] = __fmaf_rn(x, temp[e / 2], neg_m[e / 2]);
-				}
-			}
-			if (key0 < lo_max || key0 + KS > n_min || bad_now != 0) {
+			u32 const key_end = key0 + STEP<D>;
+#pragma unroll 1
+			for (u32 part = 0; part < STEP<D> / KS && (part == 0 || key0 < n_hi); ++part, key0 += KS, src += KS * RB, src_scales += KS * 8, bad_now >>= 2) {
+				// ---- scores ----
+				f32 arg[KS / 8][RT][2];
+				f32 vs[KS / 8][2];
 #pragma unroll
 				for (u32 n8 = 0; n8 < KS / 8; ++n8) {
+					u32 kw[KW];
+					if constexpr (D == 128) {
+						ld_shared_words(src + n8 * 8 * RB + k_at, *reinterpret_cast<u32 (*)[4]>(kw));
+						ld_shared_words(src + n8 * 8 * RB + (k_at ^ 16), *reinterpret_cast<u32 (*)[4]>(kw + 4));
+					} else {
+						ld_shared_words(src + n8 * 8 * RB + k_at, kw);
+					}
+					i32 c[4];
+					mma_s8<true>(c, qa[0], kw[0], kw[1]);
 #pragma unroll
-					for (u32 e = 0; e < 2; ++e) {
-						u32 const key = key0 + n8 * 8 + t * 2 + e;
-						bool seen = false;
+					for (u32 k = 2; k < KW; k += 2) mma_s8<false>(c, qa[k / 2], kw[k], kw[k + 1]);
+					f32 ks[2] = {1.0f, 1.0f};
+					if constexpr (SCALED) {
+						uint4 const s4 = ld_shared_v4(src_scales + (n8 * 8 + t * 2) * 8);
+						ks[0] = __uint_as_float(s4.x);
+						ks[1] = __uint_as_float(s4.z);
+						vs[n8][0] = __uint_as_float(s4.y);
+						vs[n8][1] = __uint_as_float(s4.w);
+					}
 #pragma unroll
-						for (u32 r = 0; r < RT; ++r) {
-							bool const off = key < lo[r] || key >= n[r] || (bad_now >> (n8 / 2) & 1);
-							if (off) arg[n8][r][e] = __uint_as_float(NEG_INF);
-							seen |= !off;
-						}
-						if (!seen) vs[n8][e] = 0.0f;   // (what lies there may be anything)
+					for (u32 e = 0; e < 2 * RT; ++e) {
+						f32 const x = SCALED ? f32(c[e]) * ks[e % 2] : f32(c[e]);
+						arg[n8][e / 2][e % 2] = __fmaf_rn(x, temp[e / 2], neg_m[e / 2]);
 					}
 				}
-			}
-			key0 += KS;
-			// ---- the maximum, when a score has passed it ----
-			f32 top[RT];
-			bool passed = false;
-#pragma unroll
-			for (u32 r = 0; r < RT; ++r) {
-				top[r] = arg[0][r][0];
-#pragma unroll
-				for (u32 n8 = 0; n8 < KS / 8; ++n8) top[r] = fmaxf(top[r], fmaxf(arg[n8][r][0], arg[n8][r][1]));
-				passed |= top[r] > ARG_MAX;
-			}
-			if (__any_sync(0xffffffffu, passed)) {
-#pragma unroll
-				for (u32 r = 0; r < RT; ++r) {
-					top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-					top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-					f32 const up = fmaxf(top[r] - SHIFT, 0.0f), a = ex2_approx(-up);
-					f32 const a0 = __shfl_sync(0xffffffffu, a, t * 8), a1 = __shfl_sync(0xffffffffu, a, t * 8 + 4);
-					neg_m[r] -= up;
-					sum[r] *= a;
+				if (key0 < lo_max || key0 + KS > n_min || bad_now != 0) {
 #pragma unroll
 					for (u32 n8 = 0; n8 < KS / 8; ++n8) {
-						arg[n8][r][0] -= up;
-						arg[n8][r][1] -= up;
-					}
 #pragma unroll
-					for (u32 j = 0; j < D / 16; ++j) {
-						o[j][r][0] *= a0;
-						o[j][r][1] *= a1;
-						o[j][r][2] *= a0;
-						o[j][r][3] *= a1;
-					}
-				}
-			}
-			if constexpr (SCALED) {
-				f32 most = vs[0][0];
+						for (u32 e = 0; e < 2; ++e) {
+							u32 const key = key0 + n8 * 8 + t * 2 + e;
+							bool seen = false;
 #pragma unroll
-				for (u32 n8 = 0; n8 < KS / 8; ++n8) most = fmaxf(most, fmaxf(vs[n8][0], vs[n8][1]));
-				if (__any_sync(0xffffffffu, most > v_unit)) {
-#pragma unroll
-					for (u32 mask = 16; mask > 0; mask >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, mask));
-					f32 const unit = __uint_as_float(__float_as_uint(fminf(most, 0x1p125f)) & 0x7F800000u) * 2.0f;
-					f32 const a = v_unit * __frcp_rn(unit);   // powers of two
-					v_unit = unit;
-					v_inv = __frcp_rn(unit);
-#pragma unroll
-					for (u32 j = 0; j < D / 16; ++j) {
-#pragma unroll
-						for (u32 e = 0; e < 4 * RT; ++e) o[j][e / 4][e % 4] *= a;
+							for (u32 r = 0; r < RT; ++r) {
+								bool const off = key < lo[r] || key >= n[r] || (bad_now >> (n8 / 2) & 1);
+								if (off) arg[n8][r][e] = __uint_as_float(NEG_INF);
+								seen |= !off;
+							}
+							if (!seen) vs[n8][e] = 0.0f;   // (what lies there may be anything)
+						}
 					}
 				}
-			}
-			// ---- weights and values ----
+				// ---- the maximum, when a score has passed it ----
+				f32 top[RT];
+				bool passed = false;
 #pragma unroll
-			for (u32 j = 0; j < 2; ++j) {
-				u32 hi[RT][2], low[RT][2];
+				for (u32 r = 0; r < RT; ++r) {
+					top[r] = arg[0][r][0];
 #pragma unroll
-				for (u32 h = 0; h < 2; ++h) {
-					f32 vw[2] = {1.0f, 1.0f};
-					if constexpr (SCALED) {
-						vw[0] = vs[2 * j + h][0] * v_inv;
-						vw[1] = vs[2 * j + h][1] * v_inv;
-					}
+					for (u32 n8 = 0; n8 < KS / 8; ++n8) top[r] = fmaxf(top[r], fmaxf(arg[n8][r][0], arg[n8][r][1]));
+					passed |= top[r] > ARG_MAX;
+				}
+				if (__any_sync(0xffffffffu, passed)) {
 #pragma unroll
 					for (u32 r = 0; r < RT; ++r) {
-						f32 e0 = ex2_approx(arg[2 * j + h][r][0]), e1 = ex2_approx(arg[2 * j + h][r][1]);
-						sum[r] += e0 + e1;
+						top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+						top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+						f32 const up = fmaxf(top[r] - SHIFT, 0.0f), a = ex2_approx(-up);
+						f32 const a0 = __shfl_sync(0xffffffffu, a, t * 8), a1 = __shfl_sync(0xffffffffu, a, t * 8 + 4);
+						neg_m[r] -= up;
+						sum[r] *= a;
+#pragma unroll
+						for (u32 n8 = 0; n8 < KS / 8; ++n8) {
+							arg[n8][r][0] -= up;
+							arg[n8][r][1] -= up;
+						}
+#pragma unroll
+						for (u32 j = 0; j < D / 16; ++j) {
+							o[j][r][0] *= a0;
+							o[j][r][1] *= a1;
+							o[j][r][2] *= a0;
+							o[j][r][3] *= a1;
+						}
+					}
+				}
+				if constexpr (SCALED) {
+					f32 most = vs[0][0];
+#pragma unroll
+					for (u32 n8 = 0; n8 < KS / 8; ++n8) most = fmaxf(most, fmaxf(vs[n8][0], vs[n8][1]));
+					if (__any_sync(0xffffffffu, most > v_unit)) {
+#pragma unroll
+						for (u32 mask = 16; mask > 0; mask >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, mask));
+						f32 const unit = __uint_as_float(__float_as_uint(fminf(most, 0x1p125f)) & 0x7F800000u) * 2.0f;
+						f32 const a = v_unit * __frcp_rn(unit);   // powers of two
+						v_unit = unit;
+						v_inv = __frcp_rn(unit);
+#pragma unroll
+						for (u32 j = 0; j < D / 16; ++j) {
+#pragma unroll
+							for (u32 e = 0; e < 4 * RT; ++e) o[j][e / 4][e % 4] *= a;
+						}
+					}
+				}
+				// ---- weights and values ----
+#pragma unroll
+				for (u32 j = 0; j < 2; ++j) {
+					u32 hi[RT][2], low[RT][2];
+#pragma unroll
+					for (u32 h = 0; h < 2; ++h) {
+						f32 vw[2] = {1.0f, 1.0f};
 						if constexpr (SCALED) {
-							e0 *= vw[0];
-							e1 *= vw[1];
+							vw[0] = vs[2 * j + h][0] * v_inv;
+							vw[1] = vs[2 * j + h][1] * v_inv;
 						}
-						hi[r][h] = f32x2_to_f16x2(e0, e1);
-						if constexpr (LOW) {
-							f32 h0, h1;
-							f16x2_values(hi[r][h], h0, h1);
-							low[r][h] = f32x2_to_f16x2(e0 - h0, e1 - h1);
+#pragma unroll
+						for (u32 r = 0; r < RT; ++r) {
+							f32 e0 = ex2_approx(arg[2 * j + h][r][0]), e1 = ex2_approx(arg[2 * j + h][r][1]);
+							sum[r] += e0 + e1;
+							if constexpr (SCALED) {
+								e0 *= vw[0];
+								e1 *= vw[1];
+							}
+							hi[r][h] = f32x2_to_f16x2(e0, e1);
+							if constexpr (LOW) {
+								f32 h0, h1;
+								f16x2_values(hi[r][h], h0, h1);
+								low[r][h] = f32x2_to_f16x2(e0 - h0, e1 - h1);
+							}
 						}
 					}
-				}
-				u32 const v0 = src + (j * 16 + t * 2) * RB + D + g * VD;
-				u32 va[VW], vb[VW], vc[VW], vd[VW];
-				ld_shared_words(v0, va);
-				ld_shared_words(v0 + RB, vb);
-				ld_shared_words(v0 + 8 * RB, vc);
-				ld_shared_words(v0 + 9 * RB, vd);
+					u32 const v0 = src + j * 16 * RB + v_at[0], v1 = src + j * 16 * RB + v_at[1];
+					u32 va[VW], vb[VW], vc[VW], vd[VW];
+					ld_shared_words(v0, va);
+					ld_shared_words(v1, vb);
+					ld_shared_words(v0 + 8 * RB, vc);
+					ld_shared_words(v1 + 8 * RB, vd);
 #pragma unroll
-				for (u32 k = 0; k < VW; ++k) {
-					u32 const v[2][4] = {{codes_to_f16x2<0>(va[k], vb[k]), codes_to_f16x2<1>(va[k], vb[k]), codes_to_f16x2<0>(vc[k], vd[k]),
-										  codes_to_f16x2<1>(vc[k], vd[k])},
-										 {codes_to_f16x2<2>(va[k], vb[k]), codes_to_f16x2<3>(va[k], vb[k]), codes_to_f16x2<2>(vc[k], vd[k]),
-										  codes_to_f16x2<3>(vc[k], vd[k])}};
+					for (u32 k = 0; k < VW; ++k) {
+						u32 const v[2][4] = {{codes_to_f16x2<0>(va[k], vb[k]), codes_to_f16x2<1>(va[k], vb[k]), codes_to_f16x2<0>(vc[k], vd[k]),
+											  codes_to_f16x2<1>(vc[k], vd[k])},
+											 {codes_to_f16x2<2>(va[k], vb[k]), codes_to_f16x2<3>(va[k], vb[k]), codes_to_f16x2<2>(vc[k], vd[k]),
+											  codes_to_f16x2<3>(vc[k], vd[k])}};
 #pragma unroll
-					for (u32 r = 0; r < RT; ++r) {
-						mma_f16(o[2 * k][r], v[0], hi[r][0], hi[r][1]);
-						mma_f16(o[2 * k + 1][r], v[1], hi[r][0], hi[r][1]);
-						if constexpr (LOW) {
-							mma_f16(o[2 * k][r], v[0], low[r][0], low[r][1]);
-							mma_f16(o[2 * k + 1][r], v[1], low[r][0], low[r][1]);
+						for (u32 r = 0; r < RT; ++r) {
+							mma_f16(o[2 * k][r], v[0], hi[r][0], hi[r][1]);
+							mma_f16(o[2 * k + 1][r], v[1], hi[r][0], hi[r][1]);
+							if constexpr (LOW) {
+								mma_f16(o[2 * k][r], v[0], low[r][0], low[r][1]);
+								mma_f16(o[2 * k + 1][r], v[1], low[r][0], low[r][1]);
+							}
 						}
 					}
 				}
 			}
+			key0 = key_end;
 		}
 		// ---- out, where the run had all steps; else a part: of the run's beginning to scratch memory, of its end to the ring ----
 		step += n_here;
@@ -907,65 +931,77 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 	// ---- what the CTA's warps share ----
 	__syncthreads();
 	if (p.splits != 0) {
-		// ... and the CTAs of a cluster: their parts go to the first one's shared memory, [splits][rows][D + 4], in place of its ring
-		static_assert(MAX_SPLITS * RT * ROWS * (D + 4) * 4 <= WARPS * RING_BYTES<D, SCALED>);
-		constexpr u32 MINE = (RT * ROWS * (D / 4) + WARPS * 32 - 1) / (WARPS * 32);   // (rows of four dims that a thread has at most)
 		u32 const kvh = p.chunks(blockIdx.x), row0 = (blockIdx.x - kvh * p.chunks.d) * p.chunk_rows;
 		u32 const rows = min(p.chunk_rows, group * p.n_tokens - row0);
-		float4 ms[MINE], v[MINE];
-		u32 sink_v[MINE];
-		auto place = [&](u32 c, u32 &r, u32 &d, u64 &out_row, u32 &head) {
-			u32 const at = threadIdx.x + c * blockDim.x;
-			r = at / (D / 4);
-			d = at % (D / 4) * 4;
-			u32 const row = row0 + r, tok = p.group(row);
-			out_row = u64(blockIdx.y) * p.n_tokens + tok;
-			head = kvh * group + row - tok * group;
-			return r < rows;
-		};
-#pragma unroll
-		for (u32 c = 0; c < MINE; ++c) {
+		struct Place {
 			u32 r, d, head;
 			u64 out_row;
-			ms[c] = make_float4(NO_PART, 0.0f, 0.0f, 0.0f);
-			v[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-			if (place(c, r, d, out_row, head)) {
-				sink_v[c] = *reinterpret_cast<u32 const *>(p.sink_v + u64(head) * D + d);
-				paged_join(ms[c], v[c], warps, [&](u32 k, bool of_ms) {
-					return of_ms ? item_ms[k][r] : *reinterpret_cast<float4 const *>(reinterpret_cast<f32 const *>(smem + k * STAGES * SB) + r * D + d);
-				});
+		};
+		auto place = [&](u32 at) {
+			u32 const r = at / (D / 4), row = row0 + r, tok = p.group(row);
+			return Place{r, at % (D / 4) * 4, kvh * group + row - tok * group, u64(blockIdx.y) * p.n_tokens + tok};
+		};
+		auto join_warps = [&](Place const &at, float4 &ms, float4 &v) {
+			ms = make_float4(NO_PART, 0.0f, 0.0f, 0.0f);
+			v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+			paged_join(ms, v, warps, [&](u32 k, bool of_ms) {
+				return of_ms ? item_ms[k][at.r] : *reinterpret_cast<float4 const *>(reinterpret_cast<f32 const *>(smem + k * STAGES * SB) + at.r * D + at.d);
+			});
+		};
+		auto finish = [&](Place const &at, float4 ms, float4 v, u32 sink_v) {
+			f32 out[4] = {v.x, v.y, v.z, v.w};
+			u32 const sv[1] = {sink_v};
+			paged_finish<D, 4>(p, at.out_row, at.head, at.d, ms.x, ms.y, out, ms.z, sv);
+		};
+		auto sink_values = [&](Place const &at) { return *reinterpret_cast<u32 const *>(p.sink_v + u64(at.head) * D + at.d); };
+		if (p.splits == 1) {
+			pdl_launch_dependents();
+			for (u32 i = threadIdx.x; i < rows * (D / 4); i += blockDim.x) {
+				Place const at = place(i);
+				u32 const sv = sink_values(at);
+				float4 ms, v;
+				join_warps(at, ms, v);
+				finish(at, ms, v, sv);
+			}
+			return;
+		}
+		// The CTAs of a cluster: their parts go to the first one's shared memory, [splits][rows][D + 4], in place of its ring.
+		static_assert(MAX_SPLITS * RT * ROWS * (D + 4) * 4 <= SM_WARPS<D, RT> * RING_BYTES<D, SCALED>);
+		constexpr u32 MINE = (RT * ROWS * (D / 4) + SM_WARPS<D, RT> * 32 - 1) / (SM_WARPS<D, RT> * 32);   // (clusters' CTAs have all warps)
+		float4 ms[MINE], v[MINE];
+		u32 sv[MINE];
+#pragma unroll
+		for (u32 c = 0; c < MINE; ++c) {
+			Place const at = place(threadIdx.x + c * blockDim.x);
+			if (at.r < rows) {
+				sv[c] = sink_values(at);
+				join_warps(at, ms[c], v[c]);
 			}
 		}
 		pdl_launch_dependents();   // not earlier: a next call's clusters would be packed onto the few SMs with room
-		if (p.splits > 1) {
-			cluster_arrive();
-			cluster_wait();        // every CTA runs, and has read its ring
-			u32 const to = map_to_cta(smem_u32(smem) + blockIdx.z * rows * (D + 4) * 4, 0);
-#pragma unroll
-			for (u32 c = 0; c < MINE; ++c) {
-				u32 r, d, head;
-				u64 out_row;
-				if (place(c, r, d, out_row, head)) {
-					st_cluster_f32x4(to + (r * (D + 4) + d) * 4, v[c]);
-					if (d == 0) st_cluster_f32x4(to + (r * (D + 4) + D) * 4, ms[c]);
-				}
-			}
-			__syncwarp();
-			cluster_arrive();      // this CTA's part is stored
-			if (blockIdx.z != 0) return;
-			cluster_wait();
-		}
+		cluster_arrive();
+		cluster_wait();            // every CTA runs, and has read its ring
+		u32 const to = map_to_cta(smem_u32(smem) + blockIdx.z * rows * (D + 4) * 4, 0);
 #pragma unroll
 		for (u32 c = 0; c < MINE; ++c) {
-			u32 r, d, head;
-			u64 out_row;
-			if (place(c, r, d, out_row, head)) {
+			Place const at = place(threadIdx.x + c * blockDim.x);
+			if (at.r < rows) {
+				st_cluster_f32x4(to + (at.r * (D + 4) + at.d) * 4, v[c]);
+				if (at.d == 0) st_cluster_f32x4(to + (at.r * (D + 4) + D) * 4, ms[c]);
+			}
+		}
+		__syncwarp();
+		cluster_arrive();          // this CTA's part is stored
+		if (blockIdx.z != 0) return;
+		cluster_wait();
+#pragma unroll
+		for (u32 c = 0; c < MINE; ++c) {
+			Place const at = place(threadIdx.x + c * blockDim.x);
+			if (at.r < rows) {
 				paged_join(ms[c], v[c], p.splits - 1, [&](u32 z, bool of_ms) {
-					return *reinterpret_cast<float4 const *>(reinterpret_cast<f32 const *>(smem) + ((z + 1) * rows + r) * (D + 4) + (of_ms ? D : d));
+					return *reinterpret_cast<float4 const *>(reinterpret_cast<f32 const *>(smem) + ((z + 1) * rows + at.r) * (D + 4) + (of_ms ? D : at.d));
 				});
-				f32 out[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-				u32 const sv[1] = {sink_v[c]};
-				paged_finish<D, 4>(p, out_row, head, d, ms[c].x, ms[c].y, out, ms[c].z, sv);
+				finish(at, ms[c], v[c], sv[c]);
 			}
 		}
 		return;
