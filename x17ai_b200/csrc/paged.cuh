@@ -1006,39 +1006,63 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 		}
 		return;
 	}
+	// (a CTA of the list has WARPS warps)
 #pragma unroll 1
-	for (u32 i = 0; i < warps * 2;) {
+	for (u32 i = 0; i < WARPS * 2;) {
 		uint2 const first = items[i];
 		if (!(first.y & THERE)) {
 			++i;
 			continue;
 		}
-		u32 end = i + 1, last = i;
-		for (; end < warps * 2 && (!(items[end].y & THERE) || items[end].x == first.x); ++end) {
-			if (items[end].y & THERE) last = end;
+		u32 mine = 0, last = i;   // the items of this (sequence, x): bit by item
+#pragma unroll
+		for (u32 k = 0; k < WARPS * 2; ++k) {
+			uint2 const item = items[k];
+			if ((item.y & THERE) && item.x == first.x && k >= i) {
+				mine |= 1u << k;
+				last = k;
+			}
 		}
 		bool const began = first.y & BEGAN, whole = began && (items[last].y & ENDED);
 		u32 const seq = first.x / n_x, x_of = first.x - seq * n_x, kvh = p.chunks(x_of), row0 = (x_of - kvh * p.chunks.d) * p.chunk_rows;
 		u32 const rows = min(p.chunk_rows, group * p.n_tokens - row0);
-		for (u32 at = threadIdx.x; at < rows * (D / 4); at += blockDim.x) {
+		for (u32 at = threadIdx.x; at < rows * (D / 4); at += WARPS * 32) {
 			u32 const r = at / (D / 4), d = at % (D / 4) * 4;
-			float4 ms = make_float4(NO_PART, 0.0f, 0.0f, 0.0f), v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-			paged_join(ms, v, last + 1 - i, [&](u32 from_i, bool of_ms) {
-				u32 const k = i + from_i;
-				if (!(items[k].y & THERE)) return make_float4(NO_PART, 0.0f, 0.0f, 0.0f);
-				u64 const slot = u64(blockIdx.x * warps + k / 2) * p.chunk_rows + r;
-				if (of_ms) return k & 1 ? item_ms[k / 2][r] : scratch.ms[slot];
-				f32 const *part = k & 1 ? reinterpret_cast<f32 const *>(smem + k / 2 * STAGES * SB) + r * D : scratch.o + slot * D;
-				return *reinterpret_cast<float4 const *>(part + d);
-			});
+			u32 const row = row0 + r, tok = p.group(row), head = kvh * group + row - tok * group;
+			u32 const sink_v[1] = {*reinterpret_cast<u32 const *>(p.sink_v + u64(head) * D + d)};
+			// everything is on its way before any of it is used
+			float4 ms[WARPS * 2], part[WARPS * 2];
+#pragma unroll
+			for (u32 k = 0; k < WARPS * 2; ++k) {
+				ms[k] = make_float4(NO_PART, 0.0f, 0.0f, 0.0f);
+				part[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+				if (mine >> k & 1) {
+					u64 const slot = u64(blockIdx.x * WARPS + k / 2) * p.chunk_rows + r;
+					ms[k] = k & 1 ? item_ms[k / 2][r] : scratch.ms[slot];
+					part[k] = *reinterpret_cast<float4 const *>(
+						(k & 1 ? reinterpret_cast<f32 const *>(smem + k / 2 * STAGES * SB) + r * D : scratch.o + slot * D) + d);
+				}
+			}
+			float4 all = make_float4(NO_PART, 0.0f, 0.0f, 0.0f), v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+			for (u32 k = 0; k < WARPS * 2; ++k) all.x = fmaxf(all.x, ms[k].x);
+#pragma unroll
+			for (u32 k = 0; k < WARPS * 2; ++k) {
+				f32 const e = ex2_approx(ms[k].x - all.x);
+				v.x = __fmaf_rn(part[k].x, e, v.x);
+				v.y = __fmaf_rn(part[k].y, e, v.y);
+				v.z = __fmaf_rn(part[k].z, e, v.z);
+				v.w = __fmaf_rn(part[k].w, e, v.w);
+				all.y = __fmaf_rn(ms[k].y, e, all.y);
+				if (mine >> k & 1) all.z = ms[k].z;   // (the same in every part)
+			}
 			if (whole) {
-				u32 const row = row0 + r, tok = p.group(row);
 				f32 out[4] = {v.x, v.y, v.z, v.w};
-				paged_finish<D, 4>(p, u64(seq) * p.n_tokens + tok, kvh * group + row - tok * group, d, ms.x, ms.y, out, ms.z);
+				paged_finish<D, 4>(p, u64(seq) * p.n_tokens + tok, head, d, all.x, all.y, out, all.z, sink_v);
 			} else {
 				u64 const slot = (u64(n_warps) + blockIdx.x * 2 + began) * p.chunk_rows + r;
 				*reinterpret_cast<float4 *>(scratch.o + slot * D + d) = v;
-				if (d == 0) scratch.ms[slot] = ms;
+				if (d == 0) scratch.ms[slot] = all;
 			}
 		}
 		i = last + 1;
