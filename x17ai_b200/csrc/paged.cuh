@@ -301,8 +301,8 @@ template <u32 D>
 constexpr u32 RUNS = STEP<D> / 16;
 constexpr u32 STAGES = 2;
 constexpr u32 ROWS = 8;          // of a tile; a warp has one or two
-constexpr u32 LONG_RUN = 100;    // steps of a warp, from which the list is not dealt out equally
-constexpr u32 MORE_CTAS = 3;     // CTAs of the list then, as a multiple of what the chip holds at once
+constexpr u32 LONG_RUN = 30;    // steps of a warp, from which the list is not dealt out equally
+constexpr u32 MORE_CTAS = 2;    // CTAs of the list then, as a multiple of what the chip holds at once
 constexpr f32 SHIFT = 8.0f, ARG_MAX = 14.0f;   // weights are 2^(x - m + SHIFT), at most 2^ARG_MAX (f16 ends below 2^16)
 constexpr u32 MAX_SPLITS = 8;    // CTAs of a cluster
 constexpr u32 MOST_STEPS = 23;   // of a warp, where every (sequence, x) has CTAs of its own
@@ -458,16 +458,15 @@ X17_DEV void paged_finish(PagedDecodeParams const &p, u64 out_row, u32 head, u32
 }
 
 // The list dealt out to CTAs in order. SMs do not read equally fast: with equal runs of 350 us the first are done 60 to 90 us before
-// the last. Where the runs are long, the CTAs that are there from the beginning get four fifths of the work, and twice as many smaller
-// ones the rest, each where one has ended (64 x 4096 keys x 32 heads: 362 -> 342 us). A CTA more costs an SM about as long as
-// 6 us of its reading: with runs of 100 us (128 ragged sequences, 543 MB) that is what the balance gains, below it is a loss
-// (131072 keys of one sequence: 59 -> 78 us).
+// the last. From 30 steps a warp on, the CTAs that are there from the beginning get nine tenths of the work, and as many smaller
+// ones the rest, each where one has ended: 64 x 4096 keys x 32 heads (148 steps a warp) 362 -> 328 us, 128 ragged sequences of 543 MB
+// (37 steps) 104 -> 102; 131072 keys of one sequence (18 steps) 58.5 -> 75 us, so shorter runs stay equal.
 struct PagedRuns {
 	u32 total, first, large, small;
 	X17_DEV PagedRuns() = default;
 	X17_DEV PagedRuns(u32 total, u32 first, u32 ctas) : total(total), first(first) {
 		bool const equal = ctas == first || total / (first * paged_cfg::WARPS) < paged_cfg::LONG_RUN;
-		large = (equal ? total : total / 5 * 4) / first + 1;
+		large = (equal ? total : total / 10 * 9) / first + 1;
 		u32 const rest = total - min(total, large * first);
 		small = equal ? 1 : rest / (ctas - first) + 1;
 	}
