@@ -621,3 +621,121 @@ def test_reads_what_torch_wrote_in_front(room):
     side.synchronize()
     assert st.read_status() == [0, 0, 0, 0]
     assert want.any() and all(torch.equal(outs[i], want[i % 3]) for i in range(n))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fixed", "scaled"])
+@pytest.mark.parametrize("H,Hk", [(8, 8), (80, 8)])
+def test_decode_more_work_than_the_chip_holds(stream, kind, H, Hk):
+    """More than 30 steps for every warp, so that more CTAs than the chip holds at once share the list. All sequences name the same
+    pages, each up to a length of its own. Twice, with the same bits."""
+    D, page, B, cap, scaled, fixed = 128, 64, 66, 3712, kind == "scaled", kind == "fixed"
+    rng = np.random.default_rng([71, H])
+    ends = [int(n) for n in rng.integers(3300, cap + 1, B)]
+    ends[7], ends[40] = 0, 1
+    one, n_pages = _table(rng, page, [cap])
+    pages, scales, ((k, ks, v, vs),) = _cache(rng, one, n_pages, Hk, page, D, scaled, [cap])
+    q = _codes(rng, B, H * D)
+    q_scale = (2.0 ** rng.uniform(-5, -2, (B, H))).astype(np.float32) if scaled else np.full((B, H), 0.125, dtype=np.float32)
+    sk, sv, temp = _codes(rng, H, D), _codes(rng, H, D, std=1.3), (0.3 + rng.random(H)).astype(np.float32)
+    kern = _kernel(H, Hk, D, page)
+    t = [_gpu(a) for a in (q, pages, np.repeat(one, B, axis=0), np.array(ends, dtype=np.int32), sk, sv, temp)]
+    t_qs, t_s = _gpu(q_scale), _gpu(scales)
+    results = []
+    for _ in range(2):
+        out, l = torch.zeros((B, H * D), dtype=torch.int8 if fixed else torch.bfloat16, device="cuda"), torch.zeros((B, H), device="cuda")
+        torch.cuda.synchronize()
+        if scaled:
+            kern.decode_scaled(stream, t[0], t_qs, t[1], t_s, *t[2:], out, l)
+        else:
+            kern.decode(stream, *t, out, l)
+        stream.synchronize()
+        results.append((out, l))
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+    got, got_l = results[0][0].float().cpu().numpy(), results[0][1].cpu().numpy()
+    for b in (0, 1, 6, 7, 8, 31, 32, 39, 40, 41, 64, 65):
+        n = ends[b]
+        want, want_l, mean, top = o_paged.attend(q[b].reshape(H, D), q_scale[b], k[:n], ks[:n], v[:n], vs[:n], sk, sv, temp, 0)
+        bound, bound_l = _decode_bounds(n, top[:, None], mean, v[:n], vs[:n], fixed)
+        _check_decode(got[b].reshape(H, D), got_l[b], want, want_l, bound, bound_l[:, 0], fixed)
+
+
+@pytest.mark.parametrize("kind", ["fixed", "scaled"])
+@pytest.mark.parametrize("room", [0, 300000])
+def test_decode_most_rows(stream, kind, room):
+    """64 query heads of one key head, 64 new tokens: 4096 rows, 256 chunks of them."""
+    _run_decode(stream, 64, 1, 32, 32, [70], 64, 32, kind == "scaled", kind == "fixed", room=room)
+
+
+def test_append_and_decode_at_the_same_time(stream):
+    """Two sequences of calls on two streams, not captured, without scratch memory of their own: what each writes is its own."""
+    from x17ai_b200 import device, kernels as K
+    H, Hk, D, page, B = 8, 2, 128, 16, 3
+    rng = np.random.default_rng(51)
+    table, n_pages = _table(rng, page, [900] * (2 * B), room=300000)
+    pages, _, _ = _cache(rng, table, n_pages, Hk, page, D, False, [900] * (2 * B))
+    kern, rope, t_pages = _kernel(H, Hk, D, page, rotary=D), K.rope_table(1024, D), _gpu(pages)
+    sk, sv, temp = _gpu(_codes(rng, H, D)), _gpu(_codes(rng, H, D)), _gpu(np.ones(H, dtype=np.float32))
+    streams = [stream, device.CudaStream(0)]
+    n = 40
+    sides = [dict(q=_gpu(_codes(rng, n, B, H * D)), kv=_gpu(_codes(rng, n, B, 2 * Hk * D)), seqs=_gpu(np.arange(B, dtype=np.int32)),
+                  pos=_gpu((np.arange(n)[:, None] + rng.integers(0, 850, B)).astype(np.int32)), table=_gpu(table[i * B:i * B + B]),
+                  q_out=torch.zeros((n, B, H * D), dtype=torch.int8, device="cuda")) for i in range(2)]
+
+    def go(s, x, i, out):
+        kern.append(s, x["q"][i], x["kv"][i], x["seqs"], x["pos"][i], x["table"], t_pages, x["q_out"][i], rope)
+        kern.decode(s, x["q_out"][i], t_pages, x["table"], x["pos"][i], sk, sv, temp, out[i])
+    start = t_pages.clone()
+    outs = []
+    for together in (False, True):
+        t_pages.copy_(start)
+        o = [torch.zeros((n, B, H * D), dtype=torch.bfloat16, device="cuda") for _ in sides]
+        torch.cuda.synchronize()
+        for i in range(n):
+            for s, x, out in zip(streams, sides, o):
+                go(s, x, i, out)
+                if not together:
+                    s.synchronize()
+        torch.cuda.synchronize()
+        outs.append((o, t_pages.clone()))
+    assert torch.equal(outs[0][1], outs[1][1])
+    for a, b in zip(outs[0][0], outs[1][0]):
+        assert a.any() and torch.equal(a, b)
+    streams[1].close()
+
+
+FIRST_IN_A_CAPTURE = """
+import torch
+from x17ai_b200 import device, kernels as K
+H, D, page = 2, 64, 16
+kern = K.PagedAttnKernel(K.PagedConfig(H, H, D, page, H * D, 2 * H * D, H * D))
+s = device.CudaStream(0)
+gen = torch.Generator(device="cuda").manual_seed(1)
+codes = lambda *shape: torch.randint(-20, 21, shape, dtype=torch.int8, device="cuda", generator=gen)
+pages, q, sk, sv = codes(8, H, page, 2 * D), codes(1, H * D), codes(H, D), codes(H, D)
+table = torch.zeros((1, 20000), dtype=torch.int32, device="cuda")
+table[0, :8] = torch.arange(8, device="cuda")
+lens, temp = torch.full((1,), 100, dtype=torch.int32, device="cuda"), torch.ones(H, device="cuda")
+out, again = (torch.zeros((1, H * D), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+torch.cuda.synchronize()
+with device.CudaGraph(s) as g:
+    kern.decode(s, q, pages, table, lens, sk, sv, temp, out)
+assert g.kernel_nodes == 2   # the list and what joins its parts
+for _ in range(3):
+    g.launch()
+kern.decode(s, q, pages, table, lens, sk, sv, temp, again)
+s.synchronize()
+assert s.read_status() == [0, 0, 0, 0] and out.any() and torch.equal(out, again)
+g.destroy()
+s.close()
+print("done")
+"""
+
+
+def test_first_call_inside_a_capture():
+    """A process whose first call of any kind is one that is recorded."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    r = subprocess.run([sys.executable, "-c", FIRST_IN_A_CAPTURE], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("done"), r.stderr[-2000:]

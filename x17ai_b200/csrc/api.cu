@@ -942,7 +942,9 @@ x17ai_DiagnosticBuffer *paged_append(char const *who, x17ai_CudaStreamHandle *st
 }
 
 // Memory that calls take and give back in stream order. A pool of the library's own, which keeps what it has: the default pool
-// gives it back to the system at every synchronise. Created at the first call in a context.
+// gives it back to the system at every synchronise. Created at the first call in a context; where that one is being captured the
+// thread may do no more than enqueue, unless it says for the moment that it knows better (nothing recorded depends on the pool's
+// creation).
 cudaError_t scratch_pool(StreamScope const &on, cudaMemPool_t *pool) {
 	ContextState &c = *on.context;
 	*pool = c.pool.load(std::memory_order_acquire);
@@ -954,16 +956,18 @@ cudaError_t scratch_pool(StreamScope const &on, cudaMemPool_t *pool) {
 	props.allocType = cudaMemAllocationTypePinned;
 	props.location.type = cudaMemLocationTypeDevice;
 	props.location.id = on.device;
-	cudaError_t e = cudaMemPoolCreate(pool, &props);
+	cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+	cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
 	if (e != cudaSuccess) return e;
+	e = cudaMemPoolCreate(pool, &props);
 	uint64_t keep = UINT64_MAX;
-	e = cudaMemPoolSetAttribute(*pool, cudaMemPoolAttrReleaseThreshold, &keep);
-	if (e != cudaSuccess) {
-		(void)cudaMemPoolDestroy(*pool);
-		return e;
+	if (e == cudaSuccess) {
+		e = cudaMemPoolSetAttribute(*pool, cudaMemPoolAttrReleaseThreshold, &keep);
+		if (e == cudaSuccess) c.pool.store(*pool, std::memory_order_release);
+		else (void)cudaMemPoolDestroy(*pool);
 	}
-	c.pool.store(*pool, std::memory_order_release);
-	return cudaSuccess;
+	cudaError_t const back = cudaThreadExchangeStreamCaptureMode(&mode);
+	return e != cudaSuccess ? e : back;
 }
 
 constexpr size_t ANY_KEYS = size_t(1) << 31;   // of a sequence: what scratch memory has to suffice for
