@@ -83,14 +83,21 @@ X17_DEV bool paged_slot(PagedPool const &pool, i32 seq, i32 pos, u32 &page, u32 
 // Reads and writes every row once: HBM-bound for prompts, one chain of four loads (position, page, row of the rope table) for a
 // decode step. A warp takes a token, or where there are few tokens a part of its heads. A lane holds 32 dims of a head, in two runs
 // of 16: both halves of 16 pairs, whose cosines and sines it loads once and keeps for all heads of the token. Lanes of one head
-// lie side by side, so loads and stores are whole sectors. Rows of the next heads are on their way under the arithmetic.
+// lie side by side, so loads and stores are whole sectors. The next heads' row is on its way under the arithmetic.
+// Measured: 8192 tokens of 32 + 32 heads of width 128, with a copy of the keys and values, 271 MB, 49.4 us: 5.5 TB/s. Scaled, 13001
+// tokens of 64 + 8 heads of width 64, 205 MB, 41.0 us: 5.0 TB/s, with the issue slots half taken. One token 2.0 us, 121 tokens 3.0.
 //
 // FixedI8: x' = (x cos - y sin + 2^13) >> 14 is one dp2a (two products of 16 by 8 bits and a sum) and a shift, exact in 32 bits.
-// Scaled: x' in f32; bf16 times a 15-bit table value is exact, so x' has one rounding and is the same however it is fused;
-// absmax over the lanes of a head; code = rint(x' * (127 / absmax)) by adding 1.5 * 2^23 (|code| <= 127, so its low byte is it).
+// Scaled: x' in f32, two pairs an instruction (46.0 us -> 41.6 for the second case); bf16 times a 15-bit table value is exact, so x'
+// has one rounding and is the same however it is fused; absmax over the lanes of a head; code = rint(x' * (127 / absmax)) by
+// adding 1.5 * 2^23 (|code| <= 127, so its low byte is it).
 
 namespace append_cfg {
-constexpr u32 THREADS = 128, WARPS = THREADS / 32;
+constexpr u32 THREADS = 64, WARPS = THREADS / 32;
+// CTAs of an SM: 28 warps of 72 registers; the scaled form 20 of 96, 32 of which are the cosines and sines in f32. A row ahead a
+// warp and these many warps are faster than two rows ahead and the 24 or 16 that those leave place for (52.0, 46.5 us below).
+template <bool SCALED>
+constexpr u32 CTAS = SCALED ? 10 : 14;
 }
 
 // a: two signed 16-bit values, pair PAIR of b's signed bytes
@@ -118,7 +125,7 @@ struct AppendRow {
 };
 
 template <u32 D, bool SCALED, bool ADJACENT>
-__global__ void __launch_bounds__(append_cfg::THREADS)
+__global__ void __launch_bounds__(append_cfg::THREADS, append_cfg::CTAS<SCALED>)
 paged_append_kernel(const PagedAppendParams p) {
 	constexpr u32 C = D / 32;        // lanes of a head
 	constexpr u32 HEADS = 32 / C;    // heads of a warp at once
@@ -152,9 +159,8 @@ paged_append_kernel(const PagedAppendParams p) {
 			row.hi[i] = reinterpret_cast<uint4 const *>(src + off1 * SIZE)[i];
 		}
 	};
-	AppendRow<SCALED> row, next;
+	AppendRow<SCALED> row;
 	load(from, row);
-	load(from + 1, next);
 	if (seq < 0) return;   // padding
 	u32 page = 0, slot = 0;
 	if (!paged_slot(p.pool, seq, pos, page, slot) || (p.rotary != 0 && u32(pos) >= p.rope_rows)) {
@@ -168,12 +174,26 @@ paged_append_kernel(const PagedAppendParams p) {
 #pragma unroll
 		for (u32 i = 0; i < 4; ++i) *reinterpret_cast<uint4 *>(cs + 4 * i) = src[i];
 	}
+	// the scaled form has them in f32
+	u64 cos2[SCALED ? 8 : 1], sin2[SCALED ? 8 : 1], nothing2 = 0;
+	if constexpr (SCALED) {
+		f32 const nothing = __uint_as_float(p.parts >> 31);   // 0, which the compiler does not know
+		nothing2 = pack_f32x2(nothing, nothing);
+		if (turns) {
+#pragma unroll
+			for (u32 i = 0; i < 8; ++i) {
+				auto c = [&](u32 j) { return f32(i32(cs[j] << 16) >> 16) * 0x1p-14f; };
+				auto sn = [&](u32 j) { return f32(i32(cs[j]) >> 16) * 0x1p-14f; };
+				cos2[i] = pack_f32x2(c(2 * i), c(2 * i + 1));
+				sin2[i] = pack_f32x2(sn(2 * i), sn(2 * i + 1));
+			}
+		}
+	}
 	u64 const slot_row = p.pool.row(page, 0, slot);
 
 	for (u32 round = from; round < to; ++round) {
 		AppendRow<SCALED> const now = row;
-		row = next;
-		load(round + 2, next);
+		load(round + 1, row);
 		u32 const h = round * HEADS + lane / C;
 		bool const live = h < per_token, is_q = h < n_q, is_v = !is_q && h - n_q >= n_kv;
 		u32 const kv_head = is_q ? 0u : is_v ? h - n_q - n_kv : h - n_q;
@@ -212,31 +232,46 @@ paged_append_kernel(const PagedAppendParams p) {
 				}
 			}
 		} else {
-			f32 v[32];
+			// pairs of x (and of y) lie side by side: x2[i] is x of pairs 2 i and 2 i + 1 in either order of a head's dims
+			u64 x2[8], y2[8];
+			auto low = [](u32 w) { return __uint_as_float(w << 16); };
+			auto high = [](u32 w) { return __uint_as_float(w & 0xFFFF0000u); };
 #pragma unroll
 			for (u32 i = 0; i < 2; ++i) {
 				u32 const a[4] = {now.lo[i].x, now.lo[i].y, now.lo[i].z, now.lo[i].w}, c[4] = {now.hi[i].x, now.hi[i].y, now.hi[i].z, now.hi[i].w};
+				if constexpr (ADJACENT) {
 #pragma unroll
-				for (u32 w = 0; w < 4; ++w) {
-					v[8 * i + 2 * w] = __uint_as_float(a[w] << 16);
-					v[8 * i + 2 * w + 1] = __uint_as_float(a[w] & 0xFFFF0000u);
-					v[16 + 8 * i + 2 * w] = __uint_as_float(c[w] << 16);
-					v[16 + 8 * i + 2 * w + 1] = __uint_as_float(c[w] & 0xFFFF0000u);
+					for (u32 w = 0; w < 2; ++w) {
+						x2[2 * i + w] = pack_f32x2(low(a[2 * w]), low(a[2 * w + 1]));
+						y2[2 * i + w] = pack_f32x2(high(a[2 * w]), high(a[2 * w + 1]));
+						x2[4 + 2 * i + w] = pack_f32x2(low(c[2 * w]), low(c[2 * w + 1]));
+						y2[4 + 2 * i + w] = pack_f32x2(high(c[2 * w]), high(c[2 * w + 1]));
+					}
+				} else {
+#pragma unroll
+					for (u32 w = 0; w < 4; ++w) {
+						x2[4 * i + w] = pack_f32x2(low(a[w]), high(a[w]));
+						y2[4 * i + w] = pack_f32x2(low(c[w]), high(c[w]));
+					}
 				}
 			}
 			if (turn) {
 #pragma unroll
-				for (u32 j = 0; j < 16; ++j) {
-					u32 const at_x = ADJACENT ? 2 * j : j, at_y = ADJACENT ? 2 * j + 1 : 16 + j;
-					f32 const c = f32(i32(cs[j] << 16) >> 16) * 0x1p-14f, sn = f32(i32(cs[j]) >> 16) * 0x1p-14f;
-					f32 const x = v[at_x], y = v[at_y];
-					v[at_x] = __fmaf_rn(x, c, -__fmul_rn(y, sn));
-					v[at_y] = __fmaf_rn(x, sn, __fmul_rn(y, c));
+				for (u32 i = 0; i < 8; ++i) {
+					u64 const x = x2[i], y = y2[i];
+					x2[i] = fma_f32x2(x, cos2[i], mul_f32x2(y, sin2[i]) ^ 0x8000000080000000ull);
+					y2[i] = fma_f32x2(x, sin2[i], mul_f32x2(y, cos2[i]));
 				}
 			}
 			f32 top = 0.0f;
 #pragma unroll
-			for (u32 j = 0; j < 32; ++j) top = fmaxf(top, fabsf(v[j]));
+			for (u32 i = 0; i < 8; ++i) {
+				f32 v[4];
+				unpack_f32x2(x2[i], v[0], v[1]);
+				unpack_f32x2(y2[i], v[2], v[3]);
+#pragma unroll
+				for (u32 j = 0; j < 4; ++j) top = fmaxf(top, fabsf(v[j]));
+			}
 #pragma unroll
 			for (u32 mask = 1; mask < C; mask <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, mask));
 			bool const some = top > PAGED_TINY;
@@ -246,12 +281,25 @@ paged_append_kernel(const PagedAppendParams p) {
 				if (is_q) p.q_scale[u64(token) * p.n_heads + h] = scale;
 				else p.pool.scales[(slot_row + (u64(kv_head) << p.pool.page_shift)) * 2 + is_v] = scale;
 			}
-			// (not the packed forms: product and sum of those become one operation, and a value on a tie another code)
-			auto code = [&](f32 x) { return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.0f)); };
+			// (a product plus nothing, since product and sum would become one operation, and a value on a tie another code)
+			u64 const inv2 = pack_f32x2(inv, inv);
+			auto codes = [&](u64 v, u32 &a, u32 &b) {
+				f32 c0, c1;
+				unpack_f32x2(add_f32x2(fma_f32x2(v, inv2, nothing2), pack_f32x2(12582912.0f, 12582912.0f)), c0, c1);
+				a = __float_as_uint(c0);
+				b = __float_as_uint(c1);
+			};
 #pragma unroll
 			for (u32 w = 0; w < 8; ++w) {
-				u32 const word = __byte_perm(__byte_perm(code(v[4 * w]), code(v[4 * w + 1]), 0x0040),
-											 __byte_perm(code(v[4 * w + 2]), code(v[4 * w + 3]), 0x0040), 0x5410);
+				u32 c[4];   // of four dims in order
+				if constexpr (ADJACENT) {
+					codes(x2[w], c[0], c[2]);
+					codes(y2[w], c[1], c[3]);
+				} else {
+					codes(w < 4 ? x2[2 * w] : y2[2 * w - 8], c[0], c[1]);
+					codes(w < 4 ? x2[2 * w + 1] : y2[2 * w - 7], c[2], c[3]);
+				}
+				u32 const word = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
 				if (w < 4) lo[w] = word;
 				else hi[w - 4] = word;
 			}
@@ -463,7 +511,7 @@ X17_DEV void paged_finish(PagedDecodeParams const &p, u64 out_row, u32 head, u32
 // (37 steps) 104 -> 102; 131072 keys of one sequence (18 steps) 58.5 -> 75 us, so shorter runs stay equal.
 struct PagedRuns {
 	u32 total, first, large, small;
-	X17_DEV PagedRuns() = default;
+	PagedRuns() = default;
 	X17_DEV PagedRuns(u32 total, u32 first, u32 ctas) : total(total), first(first) {
 		bool const equal = ctas == first || total / (first * paged_cfg::WARPS) < paged_cfg::LONG_RUN;
 		large = (equal ? total : total / 10 * 9) / first + 1;
