@@ -336,7 +336,7 @@ x17ai_DiagnosticBuffer *x17ai_b200_attn_decode_i8_noalloc(
  *   pages int8 [n_pages][n_kv_heads][page_size][K(D) | V(D)]: a page of one head is one run of memory
  *   page_scales f32 [n_pages][n_kv_heads][page_size][2] (K, V): the scaled calls; value = scale * code. The others: FixedI8
  *   page_table int32 [n_seqs][max_pages]; entries behind a sequence's last page are not read
- * n_heads is a multiple of n_kv_heads: query head h attends key head h / (n_heads / n_kv_heads).
+ * n_heads (at most 4096) is a multiple of n_kv_heads: query head h attends key head h / (n_heads / n_kv_heads).
  * What the calls read as indexes from device memory (sequences, positions, pages) is checked there: a token with an index out
  * of range is not stored, a key on a page outside the pool is not attended to, and the status words (x17ai_b200_read_status)
  * hold code 16 with the token or sequence as detail.
@@ -394,8 +394,8 @@ x17ai_DiagnosticBuffer *x17ai_b200_paged_append_scaled(
  *   q, out: row b * n_tokens + i, strides q_stride and o_stride; page_table [batch][max_pages]; kv_lens int32 [batch] (clamped to
  *   0 .. max_pages * page_size); out FixedI8 (X17AI_DTYPE_INT8) or bf16 (X17AI_DTYPE_BF16, value = code / 8);
  *   l [batch * n_tokens][n_heads] or NULL: log2(255 * sum) + max, as the other int8 kernels write it.
- * Scores are exact integer products, probabilities keep 22 bits, sums are f32. The work is dealt out evenly whatever the lengths
- * are, and the parts of a sequence meet in scratch memory: with scratch NULL it is taken from and given back to a pool of the
+ * Scores are exact integer products, sums are f32; probabilities keep 22 bits for FixedI8 output and the 11 of f16 for bf16
+ * output. The work is dealt out evenly whatever the lengths are, and the parts of a long sequence meet in scratch memory: with scratch NULL it is taken from and given back to a pool of the
  * library in stream order (in a captured graph it belongs to the graph); otherwise x17ai_b200_paged_scratch_bytes says how many
  * bytes it must have (16-byte aligned), nothing is allocated, and calls that may run at the same time need one each.
  */

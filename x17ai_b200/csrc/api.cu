@@ -998,26 +998,66 @@ PagedPlan paged_plan(x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens
 	return plan;
 }
 
-// CTAs for every (sequence, x), and warps of each, where the whole call finds place on the chip at once and none of its warps
-// gets more than a few steps; splits 0: the list.
+// Clusters of `size` decode CTAs that the chip holds at once (2: 74, 3: 45, 4: 33, 5: 26, 6: 22, 7 and 8: 15 on a chip whose 148 SMs
+// hold a CTA each; one more waits for all the others: two sequences of 16000 keys and 8 key heads 27.9 us as 16 clusters of 8,
+// 17.2 as 16 of 6). Asked once per device; a CTA of any width takes more than half of an SM's shared memory.
+uint32_t paged_clusters(StreamScope const &on, uint32_t size) {
+	static std::atomic<uint32_t> cached[MAX_DEVICES][x17::paged_cfg::MAX_SPLITS + 1];   // plus one; 0 = not asked yet
+	std::atomic<uint32_t> &known = cached[on.device][size];
+	uint32_t n = known.load(std::memory_order_relaxed);
+	if (n == 0) {
+		using K = Kernel<&x17::paged_decode_kernel<128, false, 1, false>>;
+		constexpr uint32_t warps = x17::paged_cfg::SM_WARPS<128, 1>, smem = x17::paged_cfg::RING_BYTES<128, false> * warps;
+		cudaLaunchAttribute attr{};
+		attr.id = cudaLaunchAttributeClusterDimension;
+		attr.val.clusterDim.x = 1;
+		attr.val.clusterDim.y = 1;
+		attr.val.clusterDim.z = size;
+		cudaLaunchConfig_t cfg{};
+		cfg.gridDim = dim3(1, 1, size);
+		cfg.blockDim = dim3(warps * 32);
+		cfg.dynamicSmemBytes = smem;
+		cfg.attrs = &attr;
+		cfg.numAttrs = 1;
+		int active = 0;
+		if (allow_smem(K{}, on, smem) != cudaSuccess || cudaOccupancyMaxActiveClusters(&active, &x17::paged_decode_kernel<128, false, 1, false>, &cfg) != cudaSuccess || active < 0) {
+			(void)cudaGetLastError();
+			active = 0;   // (no clusters, then)
+		}
+		n = uint32_t(active) + 1;
+		known.store(n, std::memory_order_relaxed);
+	}
+	return n - 1;
+}
+
+// CTAs for every (sequence, x), and warps of each, where the whole call finds place on the chip at once and that is not slower than
+// the list; splits 0: the list. With 8 key heads of width 128, apart and as a list, in us:
+//   sequences x keys   1 x 2000    1 x 64000   2 x 16000   3 x 32000   16 x 2000   16 x 8000   128 x 500   19 x 4000
+//   apart / list       6.8 / 9.5   37 / 31.6   17 / 20.8   35 / 41     15 / 20.5   42 / 50     28 / 36     34 / 37
+// Over 54 shapes, half of them ragged, the rule takes the faster form or one that is no more than 7 % slower.
 struct PagedPlaces {
 	uint32_t splits, warps;
 };
-PagedPlaces paged_places(PagedPlan const &plan, size_t pairs, size_t keys, int sm_count) {
+PagedPlaces paged_places(PagedPlan const &plan, size_t pairs, size_t keys, StreamScope const &on) {
 	using namespace x17::paged_cfg;
-	size_t const steps = (keys + plan.step - 1) / plan.step;
+	size_t const sm_count = size_t(on.state().sm_count), steps = (keys + plan.step - 1) / plan.step;
 	size_t const each = (pairs + sm_count - 1) / sm_count;   // CTAs on an SM
 	if (each > plan.sm_warps) return {0, WARPS};
 	size_t warps = plan.sm_warps / each, splits = 1;
 	if (each == 1) {
-		splits = size_t(sm_count) / pairs;
+		splits = sm_count / pairs;
 		if (splits > MAX_SPLITS) splits = MAX_SPLITS;
 		if (splits * warps > steps) splits = (steps + warps - 1) / warps;   // (no more than there are steps)
-		if (splits == 0) splits = 1;
+		while (splits > 1 && pairs > paged_clusters(on, uint32_t(splits))) --splits;
 	}
-	// a warp's steps, against those that the list would give it
-	size_t const mine = (steps + splits * warps - 1) / (splits * warps), shared = pairs * steps / (size_t(sm_count) * plan.sm_warps);
-	return {mine <= MOST_STEPS && mine <= shared + 5 ? uint32_t(splits) : 0, uint32_t(warps)};
+	// In units of what a step costs one of an SM's warps where all SMs read at once: with CTAs of its own every warp does the longest
+	// sequence's steps, each as dear as the chip's warps or its SM's make it (an SM reads a third faster than its share while others
+	// rest; a second tile of rows costs a third more); the list is even, but its parts go through memory to a second kernel.
+	size_t const mine = (steps + splits * warps - 1) / (splits * warps);
+	double const load = double(pairs * splits * warps) / double(sm_count), here = 0.75 * double(each * warps);
+	double const apart = double(mine) * (load > here ? load : here) * (plan.tiles > 1 ? 1.3 : 1.0);
+	double const list = double(pairs * steps) / double(sm_count) + 30.0;
+	return {mine <= MOST_STEPS && apart <= list ? uint32_t(splits) : 0, uint32_t(warps)};
 }
 
 x17ai_DiagnosticBuffer *check_paged_decode(x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, char const *who) {
@@ -1082,7 +1122,7 @@ x17ai_DiagnosticBuffer *paged_decode(char const *who, x17ai_CudaStreamHandle *st
 	p.group = fast(uint32_t(cfg->n_heads / cfg->n_kv_heads));
 	p.n_x = uint32_t(plan.n_x);
 	p.first_ctas = plan.first_ctas;
-	PagedPlaces places = paged_places(plan, batch * plan.n_x, keys, scope.state().sm_count);
+	PagedPlaces places = paged_places(plan, batch * plan.n_x, keys, scope);
 	p.splits = places.splits;
 	bool const own = scratch == nullptr && p.splits == 0;
 	if (scratch != nullptr) {

@@ -369,7 +369,7 @@ def rope_table(n_positions: int, rotary_dim: int, base: float = 10000.0, device=
 
 @dataclass(frozen=True)
 class PagedConfig:
-    """Heads, pages and row strides (elements) of a paged cache. n_heads is a multiple of n_kv_heads; page_size a power of two
+    """Heads, pages and row strides (elements) of a paged cache. n_heads (at most 4096) is a multiple of n_kv_heads; page_size a power of two
     from 16 to 1024; rotary_dim the leading dims of a head that append rotates (a multiple of 32, 0 = none), in pairs
     (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with adjacent_pairs."""
     n_heads: int
@@ -524,6 +524,7 @@ class PagedAttnKernel(_Configured):
         """New tokens over the cache: `q` [sequences * n, q_stride] holds n (1 to 64) new tokens of each sequence, token i of
         sequence b at position kv_lens[b] + i, which attends the keys in front of that position (the last `window_size` of them,
         0 = all) and the sink, as AttnKernel.decode does. `out` [rows, o_stride] int8 (FixedI8) or bf16; `l` [rows, n_heads].
+        Lengths are taken as 0 to max_pages * page_size.
         A sequence of length 0 sees the sink alone (a row of padding costs no more). `scratch`: memory from scratch() for this
         call's shape, used by one call at a time; without it the call takes its own from the library's pool, in stream order."""
         held = self._c_config   # the C form lives as long as the call
