@@ -715,16 +715,19 @@ pages, q, sk, sv = codes(8, H, page, 2 * D), codes(1, H * D), codes(H, D), codes
 table = torch.zeros((1, 20000), dtype=torch.int32, device="cuda")
 table[0, :8] = torch.arange(8, device="cuda")
 lens, temp = torch.full((1,), 100, dtype=torch.int32, device="cuda"), torch.ones(H, device="cuda")
-out, again = (torch.zeros((1, H * D), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+out, again, narrow = (torch.zeros((1, H * D), dtype=torch.bfloat16, device="cuda") for _ in range(3))
+narrow_table = table[:, :200].contiguous()
 torch.cuda.synchronize()
 with device.CudaGraph(s) as g:
+    kern.decode(s, q, pages, narrow_table, lens, sk, sv, temp, narrow)
     kern.decode(s, q, pages, table, lens, sk, sv, temp, out)
-assert g.kernel_nodes == 2   # the list and what joins its parts
+assert g.kernel_nodes == 3   # a cluster for every key head; the list and what joins its parts
 for _ in range(3):
     g.launch()
 kern.decode(s, q, pages, table, lens, sk, sv, temp, again)
 s.synchronize()
 assert s.read_status() == [0, 0, 0, 0] and out.any() and torch.equal(out, again)
+assert (narrow.float() - out.float()).abs().max() <= 2.0 ** -7 * out.float().abs().max()   # two roundings to bf16, and the weights'
 g.destroy()
 s.close()
 print("done")
@@ -732,7 +735,7 @@ print("done")
 
 
 def test_first_call_inside_a_capture():
-    """A process whose first call of any kind is one that is recorded."""
+    """A process whose first calls of any kind are recorded ones."""
     import subprocess
     import sys
     from pathlib import Path
