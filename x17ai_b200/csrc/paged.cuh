@@ -587,7 +587,15 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 	// what the warps leave for the end: [warp][of the run's beginning, of its end]; those of the end lie in the warps' rings
 	enum : u32 { THERE = 1, BEGAN = 2, ENDED = 4 };
 	__shared__ uint2 items[MAX_WARPS * 2];   // (sequence, x), flags
-	__shared__ float4 item_ms[MAX_WARPS][RT * ROWS];
+	// m, sum and the sink's score of each row of those; behind the values in the ring where an SM would else not hold three CTAs (only
+	// there: 128 ragged sequences of width 128 take 103 us this way and 107 with all of it in the ring)
+	constexpr bool MS_IN_RING = SM_WARPS<D, RT> / WARPS * (RING_BYTES<D, SCALED> * WARPS + MAX_WARPS * (RT * ROWS + 1) * 16 + 1024) > 228 * 1024;
+	static_assert(!MS_IN_RING || RT * ROWS * (D + 4) * 4 <= RING_BYTES<D, SCALED>);
+	__shared__ float4 item_ms[MS_IN_RING ? 1 : MAX_WARPS][RT * ROWS];
+	auto end_ms = [&](u32 of_warp) -> float4 * {
+		if constexpr (MS_IN_RING) return reinterpret_cast<float4 *>(smem + of_warp * STAGES * SB + RT * ROWS * D * 4);
+		return item_ms[of_warp];
+	};
 	u32 const warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
 	u32 const g = lane >> 2, t = lane & 3;
 	u32 const n_warps = gridDim.x * warps, w = blockIdx.x * warps + warp;
@@ -650,7 +658,7 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 	Span span(p, n_units != 0 ? p.kv_lens[b] : 0);
 	u32 steps = span.steps(p.n_tokens);
 	if (lane < 2) items[warp * 2 + lane] = make_uint2(0, 0);
-	if (lane < RT * ROWS) item_ms[warp][lane] = make_float4(NO_PART, 0.0f, 0.0f, 0.0f);
+	if ((!MS_IN_RING || n_units == 0) && lane < RT * ROWS) end_ms(warp)[lane] = make_float4(NO_PART, 0.0f, 0.0f, 0.0f);
 	// page table entries of the 32 runs of 16 keys from `run` on, one a lane
 	auto page_entries = [&](Span const &sp, u32 seq, u32 run) -> u32 {
 		u32 const key = sp.base() + (run + lane) * 16;
@@ -971,7 +979,7 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 						f32 *dst = at_end ? reinterpret_cast<f32 *>(smem + warp * STAGES * SB) + at * D : scratch.o + slot * D;
 #pragma unroll
 						for (u32 j = 0; j < VD; j += 4) *reinterpret_cast<float4 *>(dst + g * VD + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-						if (g == 0) *(at_end ? item_ms[warp] + at : scratch.ms + slot) = make_float4(m_r, s_r, sink_r, 0.0f);
+						if (g == 0) *(at_end ? end_ms(warp) + at : scratch.ms + slot) = make_float4(m_r, s_r, sink_r, 0.0f);
 					}
 				}
 			}
@@ -1002,7 +1010,7 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 			ms = make_float4(NO_PART, 0.0f, 0.0f, 0.0f);
 			v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 			paged_join(ms, v, warps, [&](u32 k, bool of_ms) {
-				return of_ms ? item_ms[k][at.r] : *reinterpret_cast<float4 const *>(reinterpret_cast<f32 const *>(smem + k * STAGES * SB) + at.r * D + at.d);
+				return of_ms ? end_ms(k)[at.r] : *reinterpret_cast<float4 const *>(reinterpret_cast<f32 const *>(smem + k * STAGES * SB) + at.r * D + at.d);
 			});
 		};
 		auto finish = [&](Place const &at, float4 ms, float4 v, u32 sink_v) {
@@ -1095,7 +1103,7 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 				part[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 				if (mine >> k & 1) {
 					u64 const slot = u64(blockIdx.x * WARPS + k / 2) * p.chunk_rows + r;
-					ms[k] = k & 1 ? item_ms[k / 2][r] : scratch.ms[slot];
+					ms[k] = k & 1 ? end_ms(k / 2)[r] : scratch.ms[slot];
 					part[k] = *reinterpret_cast<float4 const *>(
 						(k & 1 ? reinterpret_cast<f32 const *>(smem + k / 2 * STAGES * SB) + r * D : scratch.o + slot * D) + d);
 				}
