@@ -307,6 +307,28 @@ def test_decode_many_sequences(stream, kind):
     _run_decode(stream, 24, 8, 32, 32, [(91 * i) % 777 for i in range(70)], 3, 64, kind == "scaled", kind == "fixed", seed=1)
 
 
+@pytest.mark.parametrize("H,Hk,D,page,lens,new,window", [
+    (20, 1, 128, 64, [0, 1, 33, 2100], 1, 0),
+    (6, 2, 128, 16, [0, 40, 700], 7, 48),
+    (24, 1, 64, 32, [5, 3000], 1, 0),
+    (14, 2, 64, 16, [0, 63, 64, 900], 3, 0),
+    (17, 1, 32, 128, [1, 130, 2500], 1, 0),
+    (8, 1, 32, 16, [0, 200, 201], 3, 128),
+    (25, 1, 64, 16, [300, 0], 1, 0),
+])
+@pytest.mark.parametrize("kind", ["bf16", "fixed", "scaled"])
+@pytest.mark.parametrize("room", [0, 300000])
+def test_decode_rows_of_three_tiles(stream, kind, H, Hk, D, page, lens, new, window, room):
+    """17 to 24 rows of a key head, and one more."""
+    _run_decode(stream, H, Hk, D, page, lens, new, window, kind == "scaled", kind == "fixed", room=room)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fixed", "scaled"])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_decode_rows_of_three_tiles_many_sequences(stream, kind, D):
+    _run_decode(stream, 36, 6, D, 32, [(53 * i) % 700 for i in range(70)], 4, 0, kind == "scaled", kind == "fixed", seed=3)
+
+
 def test_scratch_that_is_too_small(stream):
     from x17ai_b200 import X17Error
     H, D, page = 4, 64, 16

@@ -979,16 +979,18 @@ struct PagedPlan {
 PagedPlan paged_plan(x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, size_t keys, int sm_count) {
 	using namespace x17::paged_cfg;
 	PagedPlan plan{};
-	// the rows of a key head in as few chunks of at most two tiles as they need, evenly
+	// The rows of a key head in one chunk of up to three tiles, else in as few of up to two as they need, evenly. 20 rows of width 128
+	// as one chunk 51 us, as two 66; 24 of width 64 with scales 33.8 and 37.4, of width 32 21 and 26.6; of short calls 12.9 and 12.0. More
+	// rows in chunks of three tiles: 48 of width 128 56 us, in chunks of two 52; 36 24.6 and 21.7.
 	size_t const rows = cfg->n_heads / cfg->n_kv_heads * n_tokens;
-	size_t const most = (rows + 2 * ROWS - 1) / (2 * ROWS);
+	size_t const most = rows <= MOST_TILES * ROWS ? 1 : (rows + 2 * ROWS - 1) / (2 * ROWS);
 	plan.chunk_rows = uint32_t((rows + most - 1) / most);
 	plan.chunks = uint32_t((rows + plan.chunk_rows - 1) / plan.chunk_rows);
-	plan.tiles = plan.chunk_rows > ROWS ? 2 : 1;
+	plan.tiles = (plan.chunk_rows + ROWS - 1) / ROWS;
 	plan.step = uint32_t(KS * (128 / cfg->head_dim));
 	plan.n_x = cfg->n_kv_heads * plan.chunks;
-	static_assert(SM_WARPS<64, 2> == SM_WARPS<128, 1> && SM_WARPS<32, 2> == SM_WARPS<128, 1>);
-	plan.sm_warps = cfg->head_dim == 128 && plan.tiles == 2 ? SM_WARPS<128, 2> : SM_WARPS<128, 1>;
+	static_assert(SM_WARPS<64, 3> == SM_WARPS<128, 1> && SM_WARPS<32, 3> == SM_WARPS<128, 1> && SM_WARPS<128, 3> == SM_WARPS<128, 2>);
+	plan.sm_warps = cfg->head_dim == 128 && plan.tiles > 1 ? SM_WARPS<128, 2> : SM_WARPS<128, 1>;
 	plan.first_ctas = uint32_t(sm_count) * (plan.sm_warps / WARPS);
 	plan.ctas = batch * plan.n_x * (keys / plan.step + 1) / (plan.first_ctas * WARPS) >= LONG_RUN ? plan.first_ctas * MORE_CTAS : plan.first_ctas;
 	size_t const slots = size_t(plan.ctas) * (WARPS + 2) * plan.chunk_rows;
@@ -1052,10 +1054,10 @@ PagedPlaces paged_places(PagedPlan const &plan, size_t pairs, size_t keys, Strea
 	}
 	// In units of what a step costs one of an SM's warps where all SMs read at once: with CTAs of its own every warp does the longest
 	// sequence's steps, each as dear as the chip's warps or its SM's make it (an SM reads a third faster than its share while others
-	// rest; a second tile of rows costs a third more); the list is even, but its parts go through memory to a second kernel.
+	// rest; another tile of rows costs a third more); the list is even, but its parts go through memory to a second kernel.
 	size_t const mine = (steps + splits * warps - 1) / (splits * warps);
 	double const load = double(pairs * splits * warps) / double(sm_count), here = 0.75 * double(each * warps);
-	double const apart = double(mine) * (load > here ? load : here) * (plan.tiles > 1 ? 1.3 : 1.0);
+	double const apart = double(mine) * (load > here ? load : here) * (0.7 + 0.3 * plan.tiles);
 	double const list = double(pairs * steps) / double(sm_count) + 30.0;
 	return {mine <= MOST_STEPS && apart <= list ? uint32_t(splits) : 0, uint32_t(warps)};
 }
@@ -1175,7 +1177,8 @@ x17ai_DiagnosticBuffer *paged_decode(char const *who, x17ai_CudaStreamHandle *st
 		go(dim, tiles, std::false_type{});
 	};
 	auto go_dim = [&](auto dim) {
-		if (plan.tiles == 2) go_tiles(dim, std::integral_constant<uint32_t, 2>{});
+		if (plan.tiles == 3) go_tiles(dim, std::integral_constant<uint32_t, 3>{});
+		else if (plan.tiles == 2) go_tiles(dim, std::integral_constant<uint32_t, 2>{});
 		else go_tiles(dim, std::integral_constant<uint32_t, 1>{});
 	};
 	if (cfg->head_dim == 128) go_dim(std::integral_constant<uint32_t, 128>{});

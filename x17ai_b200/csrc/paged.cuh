@@ -322,7 +322,7 @@ paged_append_kernel(const PagedAppendParams p) {
 //
 // A pass over a cache is bound by HBM: the kernel's job is to keep enough bytes in flight on every SM, whatever the sequences'
 // lengths, and to stay out of their way. The rows (query heads of a group, times new tokens) that share a key head are taken up to
-// sixteen at a time, so a key is read once for all of them. A warp works alone: it fills a ring of two steps of 8 KB (32 keys at
+// twenty-four at a time, so a key is read once for all of them. A warp works alone: it fills a ring of two steps of 8 KB (32 keys at
 // width 128) in shared memory (cp.async; page table entries are fetched 32 runs of keys at once). A page of a head is one run of
 // memory, so pages cost no more than a contiguous cache. The work is dealt out in one of two ways (paged_places in api.cu):
 //   - Where the call finds place on the chip at once, every (sequence, x) has a CTA of up to 12 warps or a cluster of up to 8 of
@@ -345,8 +345,8 @@ paged_append_kernel(const PagedAppendParams p) {
 // chain length - page - keys - join - store are all but 2; 48 ragged sequences in windows of 1024 (8 key heads) 19.3 us, 4.6
 // TB/s; 64 x 4096 x 32 heads 2.15 GB, 320 to 330 us, 6.5 TB/s; 128 ragged ones 543 MB, 102 us, 5.3 TB/s (SMs read at different
 // rates, and the list's end is 8 KB a warp); one sequence of 131072 keys with scales 277 MB, 58 us, 4.8 TB/s, of which the merge
-// is 4. With two tiles of rows, 24 ragged sequences of 54 MB in 24 rows of width 64 take 37 us: latency of the products' chain
-// at three warps a scheduler, not HBM (54 % of the issue slots empty, products a fifth of the time).
+// is 4. With three tiles of rows, 24 ragged sequences of 54 MB in 24 rows of width 64 with scales take 34 us: latency of the products'
+// chain at three warps a scheduler, not HBM.
 
 namespace paged_cfg {
 constexpr u32 WARPS = 4;         // of a CTA at least
@@ -358,17 +358,18 @@ constexpr u32 STEP = KS * (128 / D);
 template <u32 D>
 constexpr u32 RUNS = STEP<D> / 16;
 constexpr u32 STAGES = 2;
-constexpr u32 ROWS = 8;          // of a tile; a warp has one or two
+constexpr u32 ROWS = 8;          // of a tile
+constexpr u32 MOST_TILES = 3;    // of a warp
 constexpr u32 LONG_RUN = 30;    // steps of a warp, from which the list is not dealt out equally
 constexpr u32 MORE_CTAS = 2;    // CTAs of the list then, as a multiple of what the chip holds at once
 constexpr f32 SHIFT = 8.0f, ARG_MAX = 14.0f;   // weights are 2^(x - m + SHIFT), at most 2^ARG_MAX (f16 ends below 2^16)
 constexpr u32 MAX_SPLITS = 8;    // CTAs of a cluster
 constexpr u32 MOST_STEPS = 23;   // of a warp, where every (sequence, x) has CTAs of its own
 constexpr u32 MERGE_WARPS = 8;   // of a CTA that joins parts
-// Warps on an SM: 12 with a step in work and a step on its way each, 210 KB of rings. With two tiles at width 128 the sums
-// alone are 64 registers: eight.
+// Warps on an SM: 12 with a step in work and a step on its way each, 210 KB of rings. With two or three tiles at width 128 the
+// sums alone are 64 or 96 registers: eight.
 template <u32 D, u32 RT>
-constexpr u32 SM_WARPS = D == 128 && RT == 2 ? 8 : 12;
+constexpr u32 SM_WARPS = D == 128 && RT > 1 ? 8 : 12;
 template <u32 D, u32 RT>
 constexpr u32 REGS = 65536 / (SM_WARPS<D, RT> * 32) / 8 * 8 - (SM_WARPS<D, RT> == 8 ? 8 : 0);
 // In the ring a key's row [K | V] keeps its 2 D bytes, its 16-byte pieces in places i ^ ring_swap(row): without bank conflicts for the
@@ -579,6 +580,7 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 	constexpr u32 KW = D / 16;                       // words of a key row that a lane holds
 	constexpr u32 VW = D / 32;                       // words of a value row that a lane holds
 	constexpr u32 VD = D / 8;                        // dims of a lane
+	constexpr u32 QT = (RT + 1) / 2;                 // products that the tiles' queries take
 	constexpr u32 RB = 2 * D, SB = STAGE_BYTES<D, SCALED>, S_AT = STEP<D> * RB;   // pitch of a row, of a stage; its scales
 	using Span = PagedSpan<STEP<D>>;
 	constexpr u32 NEG_INF = 0xFF800000u;
@@ -723,7 +725,7 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 		}
 
 		// ---- this lane's rows: heads of the group for one of the new tokens (rows behind the last one repeat it and are not stored) ----
-		u32 qa[KW / 2][4];   // as the products' first operand
+		u32 qa[QT][KW / 2][4];   // as the products' first operand, two tiles each
 		u32 n[RT], lo[RT];
 		f32 temp[RT], sink[RT], neg_m[RT], sum[RT];
 		u32 qw[RT][KW], skw[RT][KW];
@@ -749,8 +751,8 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 #pragma unroll
 			for (u32 k = 0; k < KW; ++k) {
 				dot = __dp4a(i32(qw[r][k]), i32(skw[r][k]), dot);
-				qa[k / 2][k % 2 * 2 + r] = qw[r][k];
-				if (RT == 1) qa[k / 2][k % 2 * 2 + 1] = 0;
+				qa[r / 2][k / 2][k % 2 * 2 + r % 2] = qw[r][k];
+				if (r + 1 == RT && r % 2 == 0) qa[r / 2][k / 2][k % 2 * 2 + 1] = 0;
 			}
 			dot += __shfl_xor_sync(0xffffffffu, dot, 1);
 			dot += __shfl_xor_sync(0xffffffffu, dot, 2);
@@ -760,7 +762,10 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 		}
 		// (zeros that the compiler does not know, or it would move them in front of every product)
 #pragma unroll
-		for (u32 k = 0; k < KW / 2; ++k) asm volatile("" : "+r"(qa[k][0]), "+r"(qa[k][1]), "+r"(qa[k][2]), "+r"(qa[k][3]));
+		for (u32 k = 0; k < QT * KW / 2; ++k) {
+			u32 (&q4)[4] = qa[k / (KW / 2)][k % (KW / 2)];
+			asm volatile("" : "+r"(q4[0]), "+r"(q4[1]), "+r"(q4[2]), "+r"(q4[3]));
+		}
 		f32 v_unit = 0.0f, v_inv = 0.0f;   // SCALED: weights carry v_scale / v_unit, a power of two no smaller than any seen
 #pragma unroll
 		for (u32 j = 0; j < D / 16; ++j) {
@@ -804,10 +809,13 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 					} else {
 						ld_shared_words(src + n8 * 8 * RB + k_at, kw);
 					}
-					i32 c[4];
-					mma_s8<true>(c, qa[0], kw[0], kw[1]);
+					i32 c[QT][4];
 #pragma unroll
-					for (u32 k = 2; k < KW; k += 2) mma_s8<false>(c, qa[k / 2], kw[k], kw[k + 1]);
+					for (u32 q = 0; q < QT; ++q) {
+						mma_s8<true>(c[q], qa[q][0], kw[0], kw[1]);
+#pragma unroll
+						for (u32 k = 2; k < KW; k += 2) mma_s8<false>(c[q], qa[q][k / 2], kw[k], kw[k + 1]);
+					}
 					f32 ks[2] = {1.0f, 1.0f};
 					if constexpr (SCALED) {
 						uint4 const s4 = ld_shared_v4(src_scales + (n8 * 8 + t * 2) * 8);
@@ -818,7 +826,7 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 					}
 #pragma unroll
 					for (u32 e = 0; e < 2 * RT; ++e) {
-						f32 const x = SCALED ? f32(c[e]) * ks[e % 2] : f32(c[e]);
+						f32 const x = SCALED ? f32(c[e / 4][e % 4]) * ks[e % 2] : f32(c[e / 4][e % 4]);
 						arg[n8][e / 2][e % 2] = __fmaf_rn(x, temp[e / 2], neg_m[e / 2]);
 					}
 				}
