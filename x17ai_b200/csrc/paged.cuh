@@ -336,9 +336,10 @@ paged_append_kernel(const PagedAppendParams p) {
 // query's are permuted the same way. Values: mma m16n8k16 (f16 x f16 -> f32) with V transposed as its first operand (dims as M)
 // and the weights as the second (rows as N), which is how the scores' fragments lie; accumulators are a lane's 16 dims of two rows.
 // V's codes are exact in f16 (integer added to 1024 as bits). Weights are rounded to f16's 11 bits for a bf16 output, which
-// has 8: the roundings of many keys average out, a single key's is 2^-12. A FixedI8 output keeps 22 bits (e = hi + lo in f16, two
-// products into the same sums), so that its codes are those of the exact value but for near ties (1 code in a million, as with
-// f32 weights). Weights are 2^(x - m + 8) against a maximum m that moves only when a score passes it by 6: between 2^-38 and 2^14 of
+// has 8: the roundings of many keys average out, a single key's is 2^-12. A FixedI8 output keeps 22 bits (e = hi + lo in f16) and
+// sums of 16 keys are added in f32, so that its codes are those of the exact value but for near ties: of 14.8 million codes 9 differ, 18
+// with f32 weights and matrix products in f32 (with the products' own long sums, which round toward zero, 37).
+// Weights are 2^(x - m + 8) against a maximum m that moves only when a score passes it by 6: between 2^-38 and 2^14 of
 // m's nothing is lost to f16's range. m starts at the sink's score, so no key and no row leaves it undefined.
 //
 // Measured (L2 does not hold the cache but in the first two): 1500 keys x 32 heads of width 128 6.5 us, of which launch and the
@@ -420,7 +421,14 @@ X17_DEV void mma_s8(i32 (&c)[4], u32 const (&a)[4], u32 b0, u32 b1) {
 			: "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 	}
 }
+template <bool FIRST>
 X17_DEV void mma_f16(f32 (&c)[4], u32 const (&a)[4], u32 b0, u32 b1) {
+	if constexpr (FIRST) {
+		asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+			: "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+			: "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+		return;
+	}
 	asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
 		: "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
 		: "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -939,11 +947,19 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 											  codes_to_f16x2<3>(vc[k], vd[k])}};
 #pragma unroll
 						for (u32 r = 0; r < RT; ++r) {
-							mma_f16(o[2 * k][r], v[0], hi[r][0], hi[r][1]);
-							mma_f16(o[2 * k + 1][r], v[1], hi[r][0], hi[r][1]);
 							if constexpr (LOW) {
-								mma_f16(o[2 * k][r], v[0], low[r][0], low[r][1]);
-								mma_f16(o[2 * k + 1][r], v[1], low[r][0], low[r][1]);
+								// sums of 16 keys, low parts first: the product's own addition to a long sum rounds toward zero
+#pragma unroll
+								for (u32 h = 0; h < 2; ++h) {
+									f32 c[4];
+									mma_f16<true>(c, v[h], low[r][0], low[r][1]);
+									mma_f16<false>(c, v[h], hi[r][0], hi[r][1]);
+#pragma unroll
+									for (u32 e = 0; e < 4; ++e) o[2 * k + h][r][e] += c[e];
+								}
+							} else {
+#pragma unroll
+								for (u32 h = 0; h < 2; ++h) mma_f16<false>(o[2 * k + h][r], v[h], hi[r][0], hi[r][1]);
 							}
 						}
 					}
