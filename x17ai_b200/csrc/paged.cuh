@@ -579,7 +579,7 @@ X17_DEV void st_cluster_f32x4(u32 addr_cluster, float4 v) {
 	st_cluster_v4(addr_cluster, __float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w));
 }
 
-// One warp takes units w * per .. of the call's list, in order of sequence, x (key head, chunk of rows), step. RT: tiles of eight
+// One warp takes a run of steps, in order of sequence, x (key head, chunk of rows), step (the list). RT: tiles of eight
 // rows that a chunk has. LOW: weights with their low parts.
 template <u32 D, bool SCALED, u32 RT, bool LOW>
 __global__ void __maxnreg__((paged_cfg::REGS<D, RT>))
