@@ -335,12 +335,14 @@ paged_append_kernel(const PagedAppendParams p) {
 // Scores: mma m16n8k32 (s8 x s8 -> s32, exact), rows as its M, keys as its N; a lane's bytes of a key row are consecutive, the
 // query's are permuted the same way. Values: mma m16n8k16 (f16 x f16 -> f32) with V transposed as its first operand (dims as M)
 // and the weights as the second (rows as N), which is how the scores' fragments lie; accumulators are a lane's 16 dims of two rows.
-// V's codes are exact in f16 (integer added to 1024 as bits). Weights are rounded to f16's 11 bits for a bf16 output, which
-// has 8: the roundings of many keys average out, a single key's is 2^-12. A FixedI8 output keeps 22 bits (e = hi + lo in f16) and
-// sums of 16 keys are added in f32, so that its codes are those of the exact value but for near ties: of 14.8 million codes 9 differ, 18
-// with f32 weights and matrix products in f32 (with the products' own long sums, which round toward zero, 37).
-// Weights are 2^(x - m + 8) against a maximum m that moves only when a score passes it by 6: between 2^-38 and 2^14 of
-// m's nothing is lost to f16's range. m starts at the sink's score, so no key and no row leaves it undefined.
+// V's codes are exact in f16 (integer added to 1024 as bits). Weights are 2^(x - m + 8) against a maximum m that moves only when a
+// score passes it by 6; m starts at the sink's score, so no key and no row leaves it undefined. A FixedI8 cache's are two f16
+// numbers, hi + lo: 22 bits down to 2^-10 of m's weight, below that an error of at most 2^-33 of the total. With hi alone (11 bits)
+// 0.6 to 4 % of the bf16 outputs were not those of the exact value, with both 0.02 to 0.07 %, as with f32 weights and f32 products;
+// it costs 1.3 % (2.15 GB), 3 % (one user) to 6 % (64 heads of width 32, five rows). For a FixedI8 output sums of 16 keys are added in
+// f32, so that its codes are those of the exact value but for near ties: of 14.8 million codes 9 differ, 18 with f32 weights and
+// matrix products in f32 (with the products' own long sums, which round toward zero, 37). A scaled cache's weights carry the value's
+// scale and are rounded to f16's 11 bits.
 //
 // Measured (L2 does not hold the cache but in the first two): 1500 keys x 32 heads of width 128 6.5 us, of which launch and the
 // chain length - page - keys - join - store are all but 2; 48 ragged sequences in windows of 1024 (8 key heads) 19.3 us, 4.6
@@ -580,8 +582,8 @@ X17_DEV void st_cluster_f32x4(u32 addr_cluster, float4 v) {
 }
 
 // One warp takes a run of steps, in order of sequence, x (key head, chunk of rows), step (the list). RT: tiles of eight
-// rows that a chunk has. LOW: weights with their low parts.
-template <u32 D, bool SCALED, u32 RT, bool LOW>
+// rows that a chunk has. SUMS: sums of 16 keys leave the products and are added in f32.
+template <u32 D, bool SCALED, u32 RT, bool SUMS>
 __global__ void __maxnreg__((paged_cfg::REGS<D, RT>))
 paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 	using namespace paged_cfg;
@@ -926,7 +928,7 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 								e1 *= vw[1];
 							}
 							hi[r][h] = f32x2_to_f16x2(e0, e1);
-							if constexpr (LOW) {
+							if constexpr (!SCALED) {
 								f32 h0, h1;
 								f16x2_values(hi[r][h], h0, h1);
 								low[r][h] = f32x2_to_f16x2(e0 - h0, e1 - h1);
@@ -947,7 +949,7 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 											  codes_to_f16x2<3>(vc[k], vd[k])}};
 #pragma unroll
 						for (u32 r = 0; r < RT; ++r) {
-							if constexpr (LOW) {
+							if constexpr (SUMS) {
 								// sums of 16 keys, low parts first: the product's own addition to a long sum rounds toward zero
 #pragma unroll
 								for (u32 h = 0; h < 2; ++h) {
@@ -958,6 +960,10 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 									for (u32 e = 0; e < 4; ++e) o[2 * k + h][r][e] += c[e];
 								}
 							} else {
+								if constexpr (!SCALED) {
+#pragma unroll
+									for (u32 h = 0; h < 2; ++h) mma_f16<false>(o[2 * k + h][r], v[h], low[r][0], low[r][1]);
+								}
 #pragma unroll
 								for (u32 h = 0; h < 2; ++h) mma_f16<false>(o[2 * k + h][r], v[h], hi[r][0], hi[r][1]);
 							}
