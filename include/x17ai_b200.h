@@ -395,7 +395,7 @@ x17ai_DiagnosticBuffer *x17ai_b200_paged_append_scaled(
  *   0 .. max_pages * page_size); out FixedI8 (X17AI_DTYPE_INT8) or bf16 (X17AI_DTYPE_BF16, value = code / 8);
  *   l [batch * n_tokens][n_heads] or NULL: log2(255 * sum) + max, as the other int8 kernels write it.
  * Scores are exact integer products, sums are f32; probabilities keep 22 bits down to 2^-10 of the largest, smaller ones are off
- * by at most 2^-33 of the total (over a scaled cache they keep the 11 bits of f16). The work is dealt out evenly whatever the
+ * by at most 2^-33 of the total; over a scaled cache their products with the scales keep 16 bits, whatever the scales are. The work is dealt out evenly whatever the
  * lengths are, and the parts of a long sequence meet in scratch memory: with scratch NULL it is taken from and given back to a pool of the
  * library in stream order (in a captured graph it belongs to the graph); otherwise x17ai_b200_paged_scratch_bytes says how many
  * bytes it must have (16-byte aligned), nothing is allocated, and calls that may run at the same time need one each.

@@ -64,3 +64,43 @@ def test_bf16_output_is_the_exact_values_but_for_near_ties(stream, H, Hk, D, pag
         n, (k, ks, v, vs) = lens[row // new] + row % new, seqs[row // new]
         want, _, mean, top = o_paged.attend(q[row].reshape(H, D), q_scale[row], k[:n], ks[:n], v[:n], vs[:n], sk, sv, temp, window)
         _check(got[row], want, _bound(n, top, mean, v[:n], 0.125, 4))
+
+
+# (what the value scales are like)
+SCALES = ["one_far_above", "two_far_above", "wide", "negative"]
+
+
+@pytest.mark.parametrize("H,Hk,D,page,lens,new", [
+    (4, 2, 128, 16, [1, 17, 300], 1),
+    (6, 2, 64, 32, [40, 200], 3),
+    (8, 1, 32, 16, [33, 129], 2),
+    (20, 1, 128, 64, [90], 1),
+    (24, 1, 64, 16, [31, 160], 1),
+])
+@pytest.mark.parametrize("kind", SCALES)
+@pytest.mark.parametrize("room", [0, 300000])
+def test_value_scales_of_any_size(stream, kind, H, Hk, D, page, lens, new, room):
+    """A value with a scale far above the others' takes no bits from theirs: keys that carry next to no weight have scales of 2^60, or
+    of 2^20 and 2^100; scales are spread over 2^80; some are below zero."""
+    rng = np.random.default_rng([6, H, D])
+    ends = [n + new - 1 for n in lens]
+    table, n_pages = _table(rng, page, ends, room=room)
+    pages, scales, seqs = _cache(rng, table, n_pages, Hk, page, D, True, ends)
+    q, sk, sv = np.abs(_codes(rng, len(lens) * new, H * D)), _codes(rng, H, D), _codes(rng, H, D, std=1.3)
+    for i, (k, ks, v, vs) in enumerate(seqs):
+        n = len(k)
+        if kind.endswith("above"):
+            for size, at in zip([60] if kind.startswith("one") else [20, 100], rng.permutation(n)):
+                k[at], ks[at], vs[at] = -127, 1.0, 2.0 ** size   # (queries have no negative codes: a score hundreds below the others')
+        else:
+            vs *= np.exp2(rng.uniform(-40, 40, vs.shape)).astype(np.float32) if kind == "wide" else np.where(rng.random(vs.shape) < 0.7, -1, 1)
+        p = np.arange(n)
+        where = table[i, p // page], slice(None), p % page
+        pages[where], scales[where] = np.concatenate((k, v), axis=-1), np.stack((ks, vs), axis=-1)
+    temp, q_scale = (0.3 + rng.random(H)).astype(np.float32), (2.0 ** rng.uniform(-5, -2, (len(q), H))).astype(np.float32)
+    got, got_l = _decode(stream, _kernel(H, Hk, D, page), True, q, q_scale, pages, scales, table, lens, sk, sv, temp, 0)
+    for row in range(len(q)):
+        n, (k, ks, v, vs) = lens[row // new] + row % new, seqs[row // new]
+        want, want_l, mean, top = o_paged.attend(q[row].reshape(H, D), q_scale[row], k[:n], ks[:n], v[:n], vs[:n], sk, sv, temp, 0)
+        _check(got[row], want, _bound(n, top, mean, v[:n], None, 256))   # a weight's two bf16 numbers: 2^-16
+        assert (np.abs(got_l[row] - want_l) <= (16 * top + n + 128) * 2.0 ** -23).all()

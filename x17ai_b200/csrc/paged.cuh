@@ -341,14 +341,15 @@ paged_append_kernel(const PagedAppendParams p) {
 // 0.6 to 4 % of the bf16 outputs were not those of the exact value, with both 0.02 to 0.07 %, as with f32 weights and f32 products;
 // it costs 1.3 % (2.15 GB), 3 % (one user) to 6 % (64 heads of width 32, five rows). For a FixedI8 output sums of 16 keys are added in
 // f32, so that its codes are those of the exact value but for near ties: of 14.8 million codes 9 differ, 18 with f32 weights and
-// matrix products in f32 (with the products' own long sums, which round toward zero, 37). A scaled cache's weights carry the value's
-// scale and are rounded to f16's 11 bits.
+// matrix products in f32 (with the products' own long sums, which round toward zero, 37).
+// A scaled cache's weights are multiplied by the value's scale in f32 and become two bf16 numbers: 16 bits in the whole range of f32,
+// so that no scale, however large, takes another key's bits. Values of up to 2^112 / keys do not overflow.
 //
 // Measured (L2 does not hold the cache but in the first two): 1500 keys x 32 heads of width 128 6.5 us, of which launch and the
 // chain length - page - keys - join - store are all but 2; 48 ragged sequences in windows of 1024 (8 key heads) 19.3 us, 4.6
 // TB/s; 64 x 4096 x 32 heads 2.15 GB, 320 to 330 us, 6.5 TB/s; 128 ragged ones 543 MB, 102 us, 5.3 TB/s (SMs read at different
 // rates, and the list's end is 8 KB a warp); one sequence of 131072 keys with scales 277 MB, 58 us, 4.8 TB/s, of which the merge
-// is 4. With three tiles of rows, 24 ragged sequences of 54 MB in 24 rows of width 64 with scales take 34 us: latency of the products'
+// is 4. With three tiles of rows, 24 ragged sequences of 54 MB in 24 rows of width 64 with scales take 36.7 us: latency of the products'
 // chain at three warps a scheduler, not HBM.
 
 namespace paged_cfg {
@@ -423,18 +424,26 @@ X17_DEV void mma_s8(i32 (&c)[4], u32 const (&a)[4], u32 b0, u32 b1) {
 			: "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 	}
 }
-template <bool FIRST>
-X17_DEV void mma_f16(f32 (&c)[4], u32 const (&a)[4], u32 b0, u32 b1) {
-	if constexpr (FIRST) {
-		asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-			: "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-			: "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
-		return;
+// the same layout with K = 16: f16, or BF16, in f32 sums
+#define X17_MMA_VALUES(TYPE)                                                                                                                  \
+	if constexpr (FIRST) {                                                                                                                    \
+		asm("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE ".f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"   \
+			: "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])                                                                                    \
+			: "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));                                                         \
+	} else {                                                                                                                                  \
+		asm("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE ".f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"       \
+			: "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                                                                    \
+			: "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));                                                                    \
 	}
-	asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-		: "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-		: "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+template <bool BF16, bool FIRST>
+X17_DEV void mma_values(f32 (&c)[4], u32 const (&a)[4], u32 b0, u32 b1) {
+	if constexpr (BF16) {
+		X17_MMA_VALUES("bf16")
+	} else {
+		X17_MMA_VALUES("f16")
+	}
 }
+#undef X17_MMA_VALUES
 X17_DEV u32 f32x2_to_f16x2(f32 lo, f32 hi) {
 	u32 r;
 	asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -443,12 +452,21 @@ X17_DEV u32 f32x2_to_f16x2(f32 lo, f32 hi) {
 X17_DEV void f16x2_values(u32 h2, f32 &lo, f32 &hi) {
 	asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}" : "=f"(lo), "=f"(hi) : "r"(h2));
 }
-// byte J of a and of b, signed, as f16x2: the bits 0x6400 + (code + 128) are 1024 + 128 + code
-template <u32 J>
-X17_DEV u32 codes_to_f16x2(u32 a, u32 b) {
+// byte J of a and of b, signed, as f16x2 (the bits 0x6400 + (code + 128) are 1024 + 128 + code) or as bf16x2, whose eight bits hold
+// a code but not 128 more of it (128 + the lower seven bits, less 128 or, for a negative code, 256)
+template <bool BF16, u32 J>
+X17_DEV u32 codes_to_x2(u32 a, u32 b) {
+	u32 const w = __byte_perm(a, b, (J + 4) << 8 | J);
 	u32 r;
-	asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(r) : "r"(__byte_perm(a, b, (J + 4) << 8 | J)), "r"(0x00FF00FFu), "r"(0x64806480u));
-	asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(r), "r"(0xE480E480u));
+	if constexpr (BF16) {
+		u32 low, less;
+		asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(low) : "r"(w), "r"(0x007F007Fu), "r"(0x43004300u));
+		asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(less) : "r"(w), "r"(0x00800080u), "r"(0x43004300u));
+		asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(low), "r"(less));
+	} else {
+		asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(r) : "r"(w), "r"(0x00FF00FFu), "r"(0x64806480u));
+		asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(r), "r"(0xE480E480u));
+	}
 	return r;
 }
 // N words (1, 2, 4 or 8) from shared memory
@@ -776,7 +794,6 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 			u32 (&q4)[4] = qa[k / (KW / 2)][k % (KW / 2)];
 			asm volatile("" : "+r"(q4[0]), "+r"(q4[1]), "+r"(q4[2]), "+r"(q4[3]));
 		}
-		f32 v_unit = 0.0f, v_inv = 0.0f;   // SCALED: weights carry v_scale / v_unit, a power of two no smaller than any seen
 #pragma unroll
 		for (u32 j = 0; j < D / 16; ++j) {
 #pragma unroll
@@ -890,46 +907,26 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 						}
 					}
 				}
-				if constexpr (SCALED) {
-					f32 most = vs[0][0];
-#pragma unroll
-					for (u32 n8 = 0; n8 < KS / 8; ++n8) most = fmaxf(most, fmaxf(vs[n8][0], vs[n8][1]));
-					if (__any_sync(0xffffffffu, most > v_unit)) {
-#pragma unroll
-						for (u32 mask = 16; mask > 0; mask >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, mask));
-						f32 const unit = __uint_as_float(__float_as_uint(fminf(most, 0x1p125f)) & 0x7F800000u) * 2.0f;
-						f32 const a = v_unit * __frcp_rn(unit);   // powers of two
-						v_unit = unit;
-						v_inv = __frcp_rn(unit);
-#pragma unroll
-						for (u32 j = 0; j < D / 16; ++j) {
-#pragma unroll
-							for (u32 e = 0; e < 4 * RT; ++e) o[j][e / 4][e % 4] *= a;
-						}
-					}
-				}
 				// ---- weights and values ----
 #pragma unroll
 				for (u32 j = 0; j < 2; ++j) {
 					u32 hi[RT][2], low[RT][2];
 #pragma unroll
 					for (u32 h = 0; h < 2; ++h) {
-						f32 vw[2] = {1.0f, 1.0f};
-						if constexpr (SCALED) {
-							vw[0] = vs[2 * j + h][0] * v_inv;
-							vw[1] = vs[2 * j + h][1] * v_inv;
-						}
 #pragma unroll
 						for (u32 r = 0; r < RT; ++r) {
 							f32 e0 = ex2_approx(arg[2 * j + h][r][0]), e1 = ex2_approx(arg[2 * j + h][r][1]);
 							sum[r] += e0 + e1;
+							f32 h0, h1;
 							if constexpr (SCALED) {
-								e0 *= vw[0];
-								e1 *= vw[1];
-							}
-							hi[r][h] = f32x2_to_f16x2(e0, e1);
-							if constexpr (!SCALED) {
-								f32 h0, h1;
+								e0 *= vs[2 * j + h][0];
+								e1 *= vs[2 * j + h][1];
+								hi[r][h] = cvt_bf16x2(e0, e1);
+								h0 = __uint_as_float(hi[r][h] << 16);
+								h1 = __uint_as_float(hi[r][h] & 0xFFFF0000u);
+								low[r][h] = cvt_bf16x2(e0 - h0, e1 - h1);
+							} else {
+								hi[r][h] = f32x2_to_f16x2(e0, e1);
 								f16x2_values(hi[r][h], h0, h1);
 								low[r][h] = f32x2_to_f16x2(e0 - h0, e1 - h1);
 							}
@@ -943,10 +940,10 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 					ld_shared_words(v1 + 8 * RB, vd);
 #pragma unroll
 					for (u32 k = 0; k < VW; ++k) {
-						u32 const v[2][4] = {{codes_to_f16x2<0>(va[k], vb[k]), codes_to_f16x2<1>(va[k], vb[k]), codes_to_f16x2<0>(vc[k], vd[k]),
-											  codes_to_f16x2<1>(vc[k], vd[k])},
-											 {codes_to_f16x2<2>(va[k], vb[k]), codes_to_f16x2<3>(va[k], vb[k]), codes_to_f16x2<2>(vc[k], vd[k]),
-											  codes_to_f16x2<3>(vc[k], vd[k])}};
+						u32 const v[2][4] = {{codes_to_x2<SCALED, 0>(va[k], vb[k]), codes_to_x2<SCALED, 1>(va[k], vb[k]), codes_to_x2<SCALED, 0>(vc[k], vd[k]),
+											  codes_to_x2<SCALED, 1>(vc[k], vd[k])},
+											 {codes_to_x2<SCALED, 2>(va[k], vb[k]), codes_to_x2<SCALED, 3>(va[k], vb[k]), codes_to_x2<SCALED, 2>(vc[k], vd[k]),
+											  codes_to_x2<SCALED, 3>(vc[k], vd[k])}};
 #pragma unroll
 						for (u32 r = 0; r < RT; ++r) {
 							if constexpr (SUMS) {
@@ -954,18 +951,16 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 #pragma unroll
 								for (u32 h = 0; h < 2; ++h) {
 									f32 c[4];
-									mma_f16<true>(c, v[h], low[r][0], low[r][1]);
-									mma_f16<false>(c, v[h], hi[r][0], hi[r][1]);
+									mma_values<SCALED, true>(c, v[h], low[r][0], low[r][1]);
+									mma_values<SCALED, false>(c, v[h], hi[r][0], hi[r][1]);
 #pragma unroll
 									for (u32 e = 0; e < 4; ++e) o[2 * k + h][r][e] += c[e];
 								}
 							} else {
-								if constexpr (!SCALED) {
 #pragma unroll
-									for (u32 h = 0; h < 2; ++h) mma_f16<false>(o[2 * k + h][r], v[h], low[r][0], low[r][1]);
-								}
+								for (u32 h = 0; h < 2; ++h) mma_values<SCALED, false>(o[2 * k + h][r], v[h], low[r][0], low[r][1]);
 #pragma unroll
-								for (u32 h = 0; h < 2; ++h) mma_f16<false>(o[2 * k + h][r], v[h], hi[r][0], hi[r][1]);
+								for (u32 h = 0; h < 2; ++h) mma_values<SCALED, false>(o[2 * k + h][r], v[h], hi[r][0], hi[r][1]);
 							}
 						}
 					}
@@ -984,7 +979,7 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 			}
 			if (!whole) items[warp * 2 + at_end] = make_uint2(b * n_x + x, THERE | (began ? BEGAN : 0u) | (ended ? ENDED : 0u));
 		}
-		f32 const unit = SCALED ? v_unit : 0.125f;
+		constexpr f32 unit = SCALED ? 1.0f : 0.125f;
 #pragma unroll
 		for (u32 r = 0; r < RT; ++r) {
 			sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
