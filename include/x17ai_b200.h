@@ -356,7 +356,7 @@ typedef struct x17ai_PagedConfig {
 
 x17ai_DiagnosticBuffer *x17ai_b200_paged_check_config(x17ai_PagedConfig const *cfg);
 
-/* Bytes of scratch memory that a decode call of this shape on the stream's device needs. */
+/* Bytes of scratch memory that suffice for decode calls on the stream's device of up to `batch` sequences with up to `n_tokens` new tokens each. */
 x17ai_DiagnosticBuffer *x17ai_b200_paged_scratch_bytes(
 	x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, size_t *bytes);
 
@@ -398,7 +398,7 @@ x17ai_DiagnosticBuffer *x17ai_b200_paged_append_scaled(
  * by at most 2^-33 of the total; over a scaled cache their products with the scales keep 16 bits, whatever the scales are. The work is dealt out evenly whatever the
  * lengths are, and the parts of a long sequence meet in scratch memory: with scratch NULL it is taken from and given back to a pool of the
  * library in stream order (in a captured graph it belongs to the graph); otherwise x17ai_b200_paged_scratch_bytes says how many
- * bytes it must have (16-byte aligned), nothing is allocated, and calls that may run at the same time need one each.
+ * bytes suffice (16-byte aligned; fewer than a call of its own shape may need are refused), nothing is allocated, and calls that may run at the same time need one each.
  */
 x17ai_DiagnosticBuffer *x17ai_b200_paged_decode(
 	x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, int8_t const *q,

@@ -1679,7 +1679,13 @@ x17ai_DiagnosticBuffer *x17ai_b200_paged_scratch_bytes(
 	if (bytes == nullptr) return make_diag("x17ai_b200: null argument", who, ": null argument");
 	StreamScope scope(stream, who);
 	if (scope.diag) return scope.diag;
-	*bytes = paged_plan(cfg, batch, n_tokens, ANY_KEYS, scope.state().sm_count).bytes;
+	// one buffer for calls of fewer new tokens too, whose chunks may have more rows and their grids more CTAs (25 rows of a key head are
+	// chunks of 13, 24 are one; a second tile at width 128 takes the third CTA of an SM); fewer sequences need no more
+	*bytes = 0;
+	for (size_t n = 1; n <= n_tokens; ++n) {
+		size_t const need = paged_plan(cfg, batch, n, ANY_KEYS, scope.state().sm_count).bytes;
+		if (need > *bytes) *bytes = need;
+	}
 	return nullptr;
 }
 

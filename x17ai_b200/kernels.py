@@ -488,8 +488,8 @@ class PagedAttnKernel(_Configured):
             _ptr(q_scale)))
 
     def scratch(self, stream, sequences: int, n_tokens: int = 1, device="cuda") -> torch.Tensor:
-        """Memory for the parts of a decode call of this shape, for hosts that allocate nothing while
-        they serve. Calls that may run at the same time need one each."""
+        """Memory for the parts of decode calls of up to `sequences` sequences with up to `n_tokens` new tokens each, for hosts that
+        allocate nothing while they serve. Calls that may run at the same time need one each."""
         out, cfg = ctypes.c_size_t(), self.config._c()
         check(self._lib.x17ai_b200_paged_scratch_bytes(stream.handle, ctypes.byref(cfg), sequences, n_tokens, ctypes.byref(out)))
         return torch.empty(out.value, dtype=torch.uint8, device=device)
@@ -526,7 +526,7 @@ class PagedAttnKernel(_Configured):
         0 = all) and the sink, as AttnKernel.decode does. `out` [rows, o_stride] int8 (FixedI8) or bf16; `l` [rows, n_heads].
         Lengths are taken as 0 to max_pages * page_size.
         A sequence of length 0 sees the sink alone (a row of padding costs no more). `scratch`: memory from scratch() for this
-        call's shape, used by one call at a time; without it the call takes its own from the library's pool, in stream order."""
+        call's shape or a larger one, used by one call at a time; without it the call takes its own from the library's pool, in stream order."""
         held = self._c_config   # the C form lives as long as the call
         if _launched(self._native.paged_decode(held[2], stream.handle, q, pages, page_table, kv_lens, sink_k, sink_v, attn_temperature, out, l,
                                                window_size, scratch)):
