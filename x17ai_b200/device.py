@@ -76,6 +76,10 @@ class TorchStream:
             raise _lib.X17Error("the legacy default stream has no context of its own: pass a created stream")
         self._torch_stream = s
 
+    @property
+    def device_id(self) -> int:
+        return self._torch_stream.device.index
+
     def synchronize(self) -> None:
         check(self._lib.x17ai_cuda_synchronize(self.handle))
 

@@ -487,12 +487,12 @@ class PagedAttnKernel(_Configured):
             max_pages, _ptr(rope), 0 if rope is None else rope.shape[0], _ptr(pages), _ptr(page_scales), n_pages, _ptr(q_out),
             _ptr(q_scale)))
 
-    def scratch(self, stream, sequences: int, n_tokens: int = 1, device="cuda") -> torch.Tensor:
+    def scratch(self, stream, sequences: int, n_tokens: int = 1, device=None) -> torch.Tensor:
         """Memory for the parts of decode calls of up to `sequences` sequences with up to `n_tokens` new tokens each, for hosts that
-        allocate nothing while they serve. Calls that may run at the same time need one each."""
+        allocate nothing while they serve, on the stream's device. Calls that may run at the same time need one each."""
         out, cfg = ctypes.c_size_t(), self.config._c()
         check(self._lib.x17ai_b200_paged_scratch_bytes(stream.handle, ctypes.byref(cfg), sequences, n_tokens, ctypes.byref(out)))
-        return torch.empty(out.value, dtype=torch.uint8, device=device)
+        return torch.empty(out.value, dtype=torch.uint8, device=f"cuda:{stream.device_id}" if device is None else device)
 
     @staticmethod
     def _scratch_bytes(scratch):
