@@ -502,8 +502,10 @@ class PagedAttnKernel(_Configured):
             raise X17Error("paged decode scratch must be a contiguous uint8 vector on device cuda")
         return scratch.numel()
 
-    def _decode_shapes(self, q, pages, page_scales, page_table, kv_lens, sink_k, sink_v, attn_temperature, out, l, out_dtype):
+    def _decode_shapes(self, q, pages, page_scales, page_table, kv_lens, sink_k, sink_v, attn_temperature, out, l, out_dtype, window_size):
         c, op = self.config, "paged decode"
+        if not 0 <= window_size < 1 << 64 or window_size % 16 != 0:   # (as a size_t, -16 would be a window without end)
+            raise X17Error(f"{op}: attention window_size must be zero or divisible by 16, got {window_size}")
         batch = kv_lens.shape[0] if kv_lens.dim() == 1 else 0
         if batch == 0 or kv_lens.dtype != torch.int32 or not kv_lens.is_cuda or not kv_lens.is_contiguous():
             raise X17Error(f"{op} input kv_lens must be a contiguous int32 [sequences] on device cuda, got {kv_lens.dtype} {list(kv_lens.shape)}")
@@ -533,7 +535,7 @@ class PagedAttnKernel(_Configured):
             return
         out_dtype = DTYPE_BF16 if out.dtype == torch.bfloat16 else DTYPE_INT8
         batch, n, n_pages, max_pages = self._decode_shapes(
-            q, pages, None, page_table, kv_lens, sink_k, sink_v, attn_temperature, out, l, out_dtype)
+            q, pages, None, page_table, kv_lens, sink_k, sink_v, attn_temperature, out, l, out_dtype, window_size)
         cfg = self.config._c()
         check(self._lib.x17ai_b200_paged_decode(
             stream.handle, ctypes.byref(cfg), batch, n, _ptr(q), _ptr(pages), n_pages, _ptr(page_table), max_pages, _ptr(kv_lens),
@@ -548,7 +550,7 @@ class PagedAttnKernel(_Configured):
                                                       sink_v, attn_temperature, out, l, window_size, scratch)):
             return
         batch, n, n_pages, max_pages = self._decode_shapes(
-            q, pages, page_scales, page_table, kv_lens, sink_k, sink_v, attn_temperature, out, l, DTYPE_BF16)
+            q, pages, page_scales, page_table, kv_lens, sink_k, sink_v, attn_temperature, out, l, DTYPE_BF16, window_size)
         matrix_shape("paged decode", "q_scale", q_scale, (batch * n, self.config.n_heads), DTYPE_F32)
         cfg = self.config._c()
         check(self._lib.x17ai_b200_paged_decode_scaled(
