@@ -87,8 +87,9 @@ X17_DEV bool paged_slot(PagedPool const &pool, i32 seq, i32 pos, u32 &page, u32 
 // Measured: 8192 tokens of 32 + 32 heads of width 128, with a copy of the keys and values, 271 MB, 49.4 us: 5.5 TB/s. Scaled, 13001
 // tokens of 64 + 8 heads of width 64, 205 MB, 41.0 us: 5.0 TB/s, with the issue slots half taken. One token 2.0 us, 121 tokens 3.0.
 //
-// FixedI8: x' = (x cos - y sin + 2^13) >> 14 is one dp2a (two products of 16 by 8 bits and a sum) and a shift, exact in 32 bits.
-// Scaled: x' in f32, two pairs an instruction (46.0 us -> 41.6 for the second case); bf16 times a 15-bit table value is exact, so x'
+// FixedI8: x' = (x cos - y sin + 2^13) >> 14 is one dp2a (two products of 16 by 8 bits and a sum), a dp4a for the y that -sin - 1
+// leaves over, and a shift, exact in 32 bits for every int16 in the table.
+// Scaled: x' in f32, two pairs an instruction (46.0 us -> 41.6 for the second case); bf16 times a table value is exact, so x'
 // has one rounding and is the same however it is fused; absmax over the lanes of a head; code = rint(x' * (127 / absmax)) by
 // adding 1.5 * 2^23 (|code| <= 127, so its low byte is it).
 
@@ -215,8 +216,10 @@ paged_append_kernel(const PagedAppendParams p) {
 #pragma unroll
 					for (u32 e = 0; e < 2; ++e) {
 						u32 const c = cs[2 * w + e];
-						u32 const minus = (c & 0xFFFFu) | (0u - (c & 0xFFFF0000u)), swapped = __byte_perm(c, c, 0x1032);   // (cos, -sin), (sin, cos)
-						x[2 * w + e] = e == 0 ? dp2a_s16_s8<0>(minus, b, 8192) : dp2a_s16_s8<1>(minus, b, 8192);
+						// (cos, -sin - 1), and y on top, since -sin has no 16 bits where sin is -2^15; (sin, cos)
+						u32 const minus = c ^ 0xFFFF0000u, swapped = __byte_perm(c, c, 0x1032);
+						i32 const y1 = __dp4a(i32(b), e == 0 ? 0x100 : 0x1000000, 8192);
+						x[2 * w + e] = e == 0 ? dp2a_s16_s8<0>(minus, b, y1) : dp2a_s16_s8<1>(minus, b, y1);
 						y[2 * w + e] = e == 0 ? dp2a_s16_s8<0>(swapped, b, 8192) : dp2a_s16_s8<1>(swapped, b, 8192);
 					}
 				}
