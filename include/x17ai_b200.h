@@ -394,11 +394,14 @@ x17ai_DiagnosticBuffer *x17ai_b200_paged_append_scaled(
  *   q, out: row b * n_tokens + i, strides q_stride and o_stride; page_table [batch][max_pages]; kv_lens int32 [batch] (clamped to
  *   0 .. max_pages * page_size); out FixedI8 (X17AI_DTYPE_INT8) or bf16 (X17AI_DTYPE_BF16, value = code / 8);
  *   l [batch * n_tokens][n_heads] or NULL: log2(255 * sum) + max, as the other int8 kernels write it.
- * Scores are exact integer products, sums are f32; probabilities keep 22 bits down to 2^-10 of the largest, smaller ones are off
- * by at most 2^-33 of the total; over a scaled cache their products with the scales keep 16 bits, whatever the scales are. The work is dealt out evenly whatever the
- * lengths are, and the parts of a long sequence meet in scratch memory: with scratch NULL it is taken from and given back to a pool of the
- * library in stream order (in a captured graph it belongs to the graph); otherwise x17ai_b200_paged_scratch_bytes says how many
- * bytes suffice (16-byte aligned; fewer than a call of its own shape may need are refused), nothing is allocated, and calls that may run at the same time need one each.
+ * Outputs must not overlap inputs. Scores are exact integer products, sums are f32; probabilities keep 22 bits down to 2^-10 of
+ * the largest, smaller ones are off by at most 2^-33 of the total; over a scaled cache their products with the values' scales keep 16
+ * bits, whatever the scales are. The work is dealt out evenly whatever the lengths are, in one of two forms that max_pages (or the
+ * window), batch and heads decide between: a sequence's bits may depend on them, by the order of f32 sums. The parts of a long sequence
+ * meet in scratch memory: with scratch NULL it is taken from and given back to a pool of the library in stream order (in a captured
+ * graph it belongs to the graph), and the pool keeps its memory, tens of MB for every stream that decodes at the same time, until the
+ * context ends; otherwise x17ai_b200_paged_scratch_bytes says how many bytes suffice (16-byte aligned; fewer than a call of its own
+ * shape may need are refused), nothing is allocated, and calls that may run at the same time need one each.
  */
 x17ai_DiagnosticBuffer *x17ai_b200_paged_decode(
 	x17ai_CudaStreamHandle *stream, x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens, int8_t const *q,

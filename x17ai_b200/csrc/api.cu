@@ -980,8 +980,9 @@ PagedPlan paged_plan(x17ai_PagedConfig const *cfg, size_t batch, size_t n_tokens
 	using namespace x17::paged_cfg;
 	PagedPlan plan{};
 	// The rows of a key head in one chunk of up to three tiles, else in as few of up to two as they need, evenly. 20 rows of width 128
-	// as one chunk 51 us, as two 66; 24 of width 64 with scales 33.8 and 37.4, of width 32 21 and 26.6; of short calls 12.9 and 12.0. More
-	// rows in chunks of three tiles: 48 of width 128 56 us, in chunks of two 52; 36 24.6 and 21.7.
+	// (16 sequences of 4000 keys, 4 key heads) as one chunk 34.5 us, as two 36.0; 24 of width 64 with scales (24 of 8000, 2) 35.6 and 36.3,
+	// of width 32 23.8 and 29.9; of short calls (20 of width 64, 4 of 700, 4) 9.6 and 7.5. More rows in chunks of three tiles (8 of 4000, 4):
+	// 48 of width 128 35.0 us, in chunks of two 32.5; 36 34.0 and 31.7.
 	size_t const rows = cfg->n_heads / cfg->n_kv_heads * n_tokens;
 	size_t const most = rows <= MOST_TILES * ROWS ? 1 : (rows + 2 * ROWS - 1) / (2 * ROWS);
 	plan.chunk_rows = uint32_t((rows + most - 1) / most);
@@ -1032,10 +1033,14 @@ uint32_t paged_clusters(StreamScope const &on, uint32_t size) {
 	return n - 1;
 }
 
-// CTAs for every (sequence, x), and warps of each, where the whole call finds place on the chip at once and that is not slower than
-// the list; splits 0: the list. With 8 key heads of width 128, apart and as a list, in us:
+// CTAs for every (sequence, x), and warps of each, where the warps of the whole call find place on the chip at once and that is not
+// slower than the list; splits 0: the list. Keys are what the table has room for (or the window): lengths are not known here.
+// Memory is not counted: with scales or two and more tiles, what a CTA keeps for its end lets 11 or 10 CTAs of one warp on an SM
+// where 12 have warps, and 5 of two where 6 have. The last ones then wait: 1628 pairs of 500 keys of width 64 with scales 25
+// us, 1636 32; the list's 38 is slower all the same, at 1000 keys (42.8, 56.1, 55.4) no more than 4 % faster. With 8 key heads
+// of width 128, apart and as a list, in us:
 //   sequences x keys   1 x 2000    1 x 64000   2 x 16000   3 x 32000   16 x 2000   16 x 8000   128 x 500   19 x 4000
-//   apart / list       6.8 / 9.5   37 / 31.6   17 / 20.8   35 / 41     15 / 20.5   42 / 50     28 / 36     34 / 37
+//   apart / list       7.4 / 10    39 / 30.5   17.8 / 19.8 35.4 / 40   15.2 / 20.2 43 / 51     25.6 / 35   37 / 38
 // Over 54 shapes, half of them ragged, the rule takes the faster form or one that is no more than 7 % slower.
 struct PagedPlaces {
 	uint32_t splits, warps;

@@ -328,7 +328,7 @@ paged_append_kernel(const PagedAppendParams p) {
 // twenty-four at a time, so a key is read once for all of them. A warp works alone: it fills a ring of two steps of 8 KB (32 keys at
 // width 128) in shared memory (cp.async; page table entries are fetched 32 runs of keys at once). A page of a head is one run of
 // memory, so pages cost no more than a contiguous cache. The work is dealt out in one of two ways (paged_places in api.cu):
-//   - Where the call finds place on the chip at once, every (sequence, x) has a CTA of up to 12 warps or a cluster of up to 8 of
+//   - Where the call's warps find place on the chip at once, every (sequence, x) has a CTA of up to 12 warps or a cluster of up to 8 of
 //     them, x being a key head's chunk of rows. Its warps take equal runs of its steps; parts meet in shared memory.
 //   - Else the work of a call is the list of all steps of all (sequence, x), and the warps of a grid that fills the chip take equal
 //     runs of it: one sequence of 131072 keys and 128 ragged ones keep the chip equally busy, and no length has to be known on
@@ -342,17 +342,17 @@ paged_append_kernel(const PagedAppendParams p) {
 // score passes it by 6; m starts at the sink's score, so no key and no row leaves it undefined. A FixedI8 cache's are two f16
 // numbers, hi + lo: 22 bits down to 2^-10 of m's weight, below that an error of at most 2^-33 of the total. With hi alone (11 bits)
 // 0.6 to 4 % of the bf16 outputs were not those of the exact value, with both 0.02 to 0.07 %, as with f32 weights and f32 products;
-// it costs 1.3 % (2.15 GB), 3 % (one user) to 6 % (64 heads of width 32, five rows). For a FixedI8 output sums of 16 keys are added in
+// it costs 1.3 % (2.15 GB), 3 % (one user) to 6 % (64 heads of width 32, five rows), 9 % where 24 rows of width 64 are bound by it. For a FixedI8 output sums of 16 keys are added in
 // f32, so that its codes are those of the exact value but for near ties: of 14.8 million codes 9 differ, 18 with f32 weights and
 // matrix products in f32 (with the products' own long sums, which round toward zero, 37).
 // A scaled cache's weights are multiplied by the value's scale in f32 and become two bf16 numbers: 16 bits in the whole range of f32,
 // so that no scale, however large, takes another key's bits. Values of up to 2^112 / keys do not overflow.
 //
-// Measured (L2 does not hold the cache but in the first two): 1500 keys x 32 heads of width 128 6.5 us, of which launch and the
-// chain length - page - keys - join - store are all but 2; 48 ragged sequences in windows of 1024 (8 key heads) 19.3 us, 4.6
-// TB/s; 64 x 4096 x 32 heads 2.15 GB, 320 to 330 us, 6.5 TB/s; 128 ragged ones 543 MB, 102 us, 5.3 TB/s (SMs read at different
-// rates, and the list's end is 8 KB a warp); one sequence of 131072 keys with scales 277 MB, 58 us, 4.8 TB/s, of which the merge
-// is 4. With three tiles of rows, 24 ragged sequences of 54 MB in 24 rows of width 64 with scales take 36.7 us: latency of the products'
+// Measured, bf16 output (L2 does not hold the cache but in the first two): 1500 keys x 32 heads of width 128 6.9 us, of which launch
+// and the chain length - page - keys - join - store are all but 2; 48 ragged sequences in windows of 1024 (8 key heads) 20 us, 4.5
+// TB/s; 64 x 4096 x 32 heads 2.15 GB, 337 to 346 us, 6.2 to 6.4 TB/s; 128 ragged ones 543 MB, 105 to 108 us, 5.0 to 5.2 TB/s (SMs
+// read at different rates, and the list's end is 8 KB a warp); one sequence of 131072 keys with scales 277 MB, 57 to 59 us, 4.8 TB/s,
+// of which the merge is 4. With three tiles of rows, 24 ragged sequences of 54 MB in 24 rows of width 64 with scales take 36.7 us: latency of the products'
 // chain at three warps a scheduler, not HBM.
 
 namespace paged_cfg {
@@ -549,8 +549,8 @@ X17_DEV void paged_finish(PagedDecodeParams const &p, u64 out_row, u32 head, u32
 
 // The list dealt out to CTAs in order. SMs do not read equally fast: with equal runs of 350 us the first are done 60 to 90 us before
 // the last. From 30 steps a warp on, the CTAs that are there from the beginning get nine tenths of the work, and as many smaller
-// ones the rest, each where one has ended: 64 x 4096 keys x 32 heads (148 steps a warp) 362 -> 328 us, 128 ragged sequences of 543 MB
-// (37 steps) 104 -> 102; 131072 keys of one sequence (18 steps) 58.5 -> 75 us, so shorter runs stay equal.
+// ones the rest, each where one has ended: 64 x 4096 keys x 32 heads (148 steps a warp) 356 -> 344 us, 128 ragged sequences of 543 MB
+// (37 steps) 109.3 -> 107.8; 131072 keys of one sequence (18 steps) 57.9 -> 72.3 us, so shorter runs stay equal.
 struct PagedRuns {
 	u32 total, first, large, small;
 	PagedRuns() = default;
@@ -621,7 +621,7 @@ paged_decode_kernel(const PagedDecodeParams p, const PagedScratch scratch) {
 	enum : u32 { THERE = 1, BEGAN = 2, ENDED = 4 };
 	__shared__ uint2 items[MAX_WARPS * 2];   // (sequence, x), flags
 	// m, sum and the sink's score of each row of those; behind the values in the ring where an SM would else not hold three CTAs (only
-	// there: 128 ragged sequences of width 128 take 103 us this way and 107 with all of it in the ring)
+	// there: 128 ragged sequences of width 128 take 108 us this way and 111 with all of it in the ring)
 	constexpr bool MS_IN_RING = SM_WARPS<D, RT> / WARPS * (RING_BYTES<D, SCALED> * WARPS + MAX_WARPS * (RT * ROWS + 1) * 16 + 1024) > 228 * 1024;
 	static_assert(!MS_IN_RING || RT * ROWS * (D + 4) * 4 <= RING_BYTES<D, SCALED>);
 	__shared__ float4 item_ms[MS_IN_RING ? 1 : MAX_WARPS][RT * ROWS];
