@@ -350,7 +350,7 @@ paged_append_kernel(const PagedAppendParams p) {
 //
 // Measured, bf16 output (L2 does not hold the cache but in the first two): 1500 keys x 32 heads of width 128 6.9 us, of which launch
 // and the chain length - page - keys - join - store are all but 2; 48 ragged sequences in windows of 1024 (8 key heads) 20 us, 4.5
-// TB/s; 64 x 4096 x 32 heads 2.15 GB, 337 to 346 us, 6.2 to 6.4 TB/s; 128 ragged ones 543 MB, 105 to 108 us, 5.0 to 5.2 TB/s (SMs
+// TB/s; 64 x 4096 x 32 heads 2.15 GB, 337 to 347 us, 6.2 to 6.4 TB/s; 128 ragged ones 543 MB, 105 to 108 us, 5.0 to 5.2 TB/s (SMs
 // read at different rates, and the list's end is 8 KB a warp); one sequence of 131072 keys with scales 277 MB, 57 to 59 us, 4.8 TB/s,
 // of which the merge is 4. With three tiles of rows, 24 ragged sequences of 54 MB in 24 rows of width 64 with scales take 36.7 us: latency of the products'
 // chain at three warps a scheduler, not HBM.
